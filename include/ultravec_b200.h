@@ -539,6 +539,130 @@ int uv_coset_export(const uv_coset *coset, uint8_t *codes, float *rescale, float
 int uv_coset_reconstruct(const uv_coset *coset, const float *rows, int64_t n, float *out,
                          void *stream);
 
+/* ---- serving a model over the index: a cache held in 4 bits, and attention
+ *
+ * The codec's rotation and rescaled estimator on keys and values: a row of a
+ * token and head is rotated (seeded signs and Hadamard transforms, as the
+ * vectors of the index are), held as 4-bit levels l_i = n_i - 7.5 and one f32
+ * scale s = |y|^2 / <l, y>, and scored without being decoded:
+ * <q, x> ~ s <R q, l>.
+ *
+ * The caller owns every buffer, all of it device memory of `device`.  Calls
+ * are ordered on `stream` and never wait for the device (uv_kv_check excepted),
+ * so a serving step can be captured in a CUDA graph.  Calls that change a
+ * cache must be ordered one after the other and against those that read it;
+ * attention and reads may overlap.  The calls hold nothing of their own:
+ * attention takes scratch (or allocates it in stream order).
+ *
+ * What the device alone can see to be wrong (a sequence number out of range or
+ * listed twice, no free page) does not change the cache: the call sets bits of
+ * a status word, and every later call that would change the cache does nothing
+ * until uv_kv_check has read it. */
+#define UV_F16 0
+#define UV_BF16 1
+
+#define UV_KV_NO_PAGES 1   /* fewer free pages than the call needs */
+#define UV_KV_BAD_SEQ 2    /* a sequence out of range or listed twice, a negative count or length */
+#define UV_KV_TOO_LONG 4   /* more tokens than a row of the table holds */
+#define UV_KV_NOT_EMPTY 8  /* the target of a fork or a copy has tokens */
+#define UV_KV_SHARED 16    /* rows appended to a page that others hold: extend comes first */
+#define UV_KV_TIMEOUT 32   /* a bounded device wait gave up: outputs are not valid */
+
+typedef struct uv_kv {
+    int32_t device;
+    int32_t head_dim;    /* 64, 128 or 256 */
+    int32_t kv_heads;
+    int32_t layers;      /* layers that share the table, each with its own pages' data */
+    int32_t page_tokens; /* 32, 64, 128 or 256 */
+    int32_t n_pages;
+    int32_t max_seqs;
+    int32_t max_pages;   /* table columns: pages of the longest sequence */
+    int32_t rounds;      /* rotation rounds, 1 to 3 */
+    int32_t reserved;
+    uint32_t signs[3][8]; /* bit i % 32 of word i / 32: coordinate i is negated in that round */
+    void *pool;          /* layers x n_pages x kv_heads x page_tokens / 32 tiles of
+                          * 32 (head_dim + 8) bytes: 32 keys' codes (head_dim / 2 bytes each,
+                          * dimension i in nibble i), their 32 f32 scales, 32 values' codes
+                          * (16-bit granules of 4 dimensions, those of tokens 2p and 2p + 1
+                          * alternating), their 32 f32 scales */
+    int32_t *table;      /* max_seqs x max_pages: page numbers, -1 past the sequence's end */
+    int32_t *lens;       /* max_seqs: tokens */
+    int32_t *refs;       /* n_pages: sequences that hold the page; 0 = free */
+    int32_t *work;       /* uv_kv_work_words() words, kept between calls */
+} uv_kv;
+
+int uv_kv_pool_bytes(const uv_kv *kv, int64_t *bytes);
+int uv_kv_work_words(const uv_kv *kv, int64_t *words);
+/* The rotation's signs from a seed, as the codec's (src/lib.rs:428-463). */
+int uv_kv_seed(uv_kv *kv, uint64_t seed);
+/* An empty cache (the pool's bytes are left as they are). */
+int uv_kv_reset(const uv_kv *kv, void *stream);
+/* The work words of a table, lengths and counts that the caller has filled. */
+int uv_kv_recount(const uv_kv *kv, void *stream);
+/* Waits for the stream; *status = the bits set since the last check, which it clears. */
+int uv_kv_check(const uv_kv *kv, int32_t *status, void *stream);
+
+/* Room for counts[i] more tokens of sequence seqs[i], which its length then
+ * includes: the lowest free pages, in the order of the list.  A last page that
+ * other sequences hold too is replaced by a copy, in every layer.  All or
+ * nothing. */
+int uv_kv_extend(const uv_kv *kv, const int32_t *seqs, const int32_t *counts, int32_t n,
+                 void *stream);
+/* The empty sequence dst[i] holds the pages of src[i]'s first lens[i] tokens
+ * too (NULL: all of them). */
+int uv_kv_fork(const uv_kv *kv, const int32_t *src, const int32_t *dst, const int32_t *lens,
+               int32_t n, void *stream);
+/* The same with pages of its own, copied in every layer. */
+int uv_kv_copy(const uv_kv *kv, const int32_t *src, const int32_t *dst, int32_t n, void *stream);
+/* Sequence seqs[i] keeps its first lens[i] tokens (NULL: none); pages that no
+ * sequence holds any more are free. */
+int uv_kv_truncate(const uv_kv *kv, const int32_t *seqs, const int32_t *lens, int32_t n,
+                   void *stream);
+/* The used pages become the lowest ones, in their order as far as they stay,
+ * so that the pool's used part is one block of memory. */
+int uv_kv_compact(const uv_kv *kv, void *stream);
+
+/* The last rows of sequences, packed: seqs[b] owns rows [starts[b],
+ * starts[b + 1]) (one each when starts is NULL), its last tokens in order.
+ * Element [row][head][i] of an input is at row * row_stride + head *
+ * head_stride + i; strides are multiples of 8, bases 16-byte aligned.
+ * append writes them (extend has made the room); read returns them as they are
+ * held, dense (rows without a token as zeros). */
+int uv_kv_append(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int32_t *starts,
+                 int32_t n, int32_t rows, int32_t dtype, const void *k, int64_t k_row_stride,
+                 int64_t k_head_stride, const void *v, int64_t v_row_stride,
+                 int64_t v_head_stride, void *stream);
+int uv_kv_read(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int32_t *starts,
+               int32_t n, int32_t rows, int32_t dtype, void *k, void *v, void *stream);
+
+/* Attention of those rows over the cache: row i of n rows of a sequence of len
+ * tokens sees tokens 0 .. len - n + i; q_heads / kv_heads query heads share a
+ * key head.  out: rows x q_heads x head_dim, dense; lse (may be NULL): rows x
+ * q_heads, the natural logarithm of the sum of exp(score), whose error is that
+ * of queries rounded to 11 bits.  A row that sees nothing has out 0 and lse
+ * -inf.  most: rows of the longest entry (a hint: it picks the tile).
+ * scratch: uv_kv_attend_bytes() bytes, 128-byte aligned, or NULL. */
+int uv_kv_attend_bytes(const uv_kv *kv, int32_t n, int32_t rows, int32_t most, int32_t q_heads,
+                       int64_t *bytes);
+int uv_kv_attend(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int32_t *starts,
+                 int32_t n, int32_t rows, int32_t most, int32_t dtype, const void *q,
+                 int64_t q_row_stride, int64_t q_head_stride, int32_t q_heads, float scale,
+                 void *out, float *lse, void *scratch, int64_t scratch_bytes, void *stream);
+
+/* Attention over whole packed prompts: sequence b has query rows
+ * [starts_q[b], starts_q[b + 1]) and key rows [starts_k[b], starts_k[b + 1])
+ * (NULL: the same), its queries being the last of its keys: with causal, row i
+ * sees keys 0 .. i + keys - queries.  head_dim 64 or 128; strides, out and lse
+ * as above.  What a row does not see has no influence on it, whatever it
+ * holds. */
+int uv_prompt_attention(int32_t device, const int32_t *starts_q, const int32_t *starts_k,
+                        int32_t n, int32_t rows_q, int32_t rows_k, int32_t q_heads,
+                        int32_t kv_heads, int32_t head_dim, int32_t causal, float scale,
+                        int32_t dtype, const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                        const void *k, int64_t k_row_stride, int64_t k_head_stride, const void *v,
+                        int64_t v_row_stride, int64_t v_head_stride, void *out, float *lse,
+                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,168 @@
+"""Attention over packed prompts against a 64-bit model."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import kv_model as M
+
+pytestmark = pytest.mark.gpu
+
+UNIT = {"float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}  # half an ulp, relative
+
+
+def starts(counts):
+    import torch
+
+    return torch.tensor(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), device="cuda")
+
+
+def rows(rng, n, heads, d, typ, size=1.0):
+    import torch
+
+    return torch.tensor(size * rng.standard_normal((n, heads, d)), dtype=torch.float32,
+                        device="cuda").to(getattr(torch, typ))
+
+
+def f64(x):
+    return x.double().cpu().numpy()
+
+
+def tolerance(out, size, reach, typ):
+    """Products of the inputs are exact and add up in f32: scores err by less
+    than 2^-17 of sum |q_i k_i| and the exponential, with its argument, by less
+    than 2^-14; a weight rounds to the type, the sum takes it unrounded; the
+    output rounds."""
+    eps = UNIT[typ] + 2 * (2.0 ** -17 * reach + 2.0 ** -14)
+    return eps[..., None] * size * 1.02 + UNIT[typ] * np.abs(out) * 1.01 + 2.0 ** -24
+
+
+def compare(out, lse, q, k, v, nq, nk, causal, typ, scale):
+    a = b = 0
+    for n, m in zip(nq, nk):
+        want, wl, size, reach = M.prompt(f64(q[a:a + n]), f64(k[b:b + m]), f64(v[b:b + m]), causal, scale)
+        err, tol = np.abs(f64(out[a:a + n]) - want), tolerance(want, size, reach, typ)
+        assert (err <= tol).all(), float((err / tol).max())
+        got, seen = f64(lse[a:a + n]), np.isfinite(wl)
+        assert (np.isneginf(got) == ~seen).all()
+        assert (np.abs(got - wl)[seen] <= (2.0 ** -17 * reach + 2.0 ** -13)[seen]).all()
+        a, b = a + n, b + m
+
+
+CASES = [  # d, q heads, kv heads, queries, keys, causal, type
+    (64, 8, 2, [77], [77], True, "float16"),
+    (128, 4, 4, [1, 2, 63, 64, 65], [1, 2, 63, 64, 65], True, "bfloat16"),
+    (128, 4, 1, [127, 128, 129, 1], [127, 128, 129, 1], True, "float16"),
+    (64, 3, 3, [255, 256, 257], [255, 256, 257], False, "bfloat16"),
+    (128, 2, 2, [33, 5, 200], [333, 5, 201], True, "bfloat16"),
+    (64, 6, 2, [10, 130], [300, 131], False, "float16"),
+    (128, 3, 1, [300], [300], True, "bfloat16"),
+    (128, 6, 3, [0, 40, 0, 0, 9, 0], [0, 40, 0, 7, 9, 0], True, "float16"),
+    (64, 2, 1, [513], [600], True, "float16"),
+]
+
+
+@pytest.mark.parametrize("d,hq,hk,nq,nk,causal,typ", CASES)
+def test_prompt(uv, d, hq, hk, nq, nk, causal, typ):
+    rng = np.random.default_rng(d + hq + len(nq))
+    q, k, v = rows(rng, sum(nq), hq, d, typ, 1.5), rows(rng, sum(nk), hk, d, typ), rows(rng, sum(nk), hk, d, typ)
+    out, lse = uv.prompt_attention(q, k, v, starts(nq), starts(nk), causal=causal, lse=True)
+    compare(out, lse, q, k, v, nq, nk, causal, typ, 1 / math.sqrt(d))
+
+
+def test_more_queries_than_keys_leaves_rows_empty(uv):
+    rng = np.random.default_rng(1)
+    for d in (64, 128):
+        q, k, v = (rows(rng, n, 2, d, "bfloat16") for n in (200, 70, 70))
+        out, lse = uv.prompt_attention(q, k, v, starts([150, 50]), starts([70, 0]), lse=True)
+        compare(out, lse, q, k, v, [150, 50], [70, 0], True, "bfloat16", 1 / math.sqrt(d))
+        assert (f64(out)[:80] == 0).all() and (f64(out)[150:] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan"), 3e38])
+def test_what_a_row_does_not_see_does_not_reach_it(uv, d, bad):
+    """Infinities and NaN in the keys and values of later tokens and of the next
+    sequence leave a row's bits as they are; rows that see a NaN have one."""
+    import torch
+
+    rng = np.random.default_rng(2)
+    n = [150, 90, 64]
+    for hk in (1, 2):
+        q, k, v = (rows(rng, sum(n), h, d, "bfloat16") for h in (2, hk, hk))
+        want = uv.prompt_attention(q, k, v, starts(n))
+        for which in (0, 1):
+            kv = [k.clone(), v.clone()]
+            kv[which][100:150, :, 3] = bad   # rows 100.. of the first sequence see it
+            kv[which][150 + 90:, :, 5] = bad  # the third sequence
+            got = uv.prompt_attention(q, *kv, starts(n))
+            assert torch.equal(got[:100], want[:100])
+            assert torch.equal(got[150:240], want[150:240])
+            if math.isnan(bad):
+                where = slice(None) if which == 0 else 3
+                assert bool(got[100:150, :, where].isnan().all())
+            elif which == 1 and math.isinf(bad):
+                assert bool((got[100:150, :, 3] == bad).all())
+                assert torch.isfinite(got[100:150, :, :3]).all()
+
+
+def test_large_scores_and_a_scale(uv):
+    rng = np.random.default_rng(3)
+    for d in (64, 128):
+        q, k, v = rows(rng, 300, 2, d, "bfloat16", 30.0), rows(rng, 300, 2, d, "bfloat16", 5.0), \
+            rows(rng, 300, 2, d, "bfloat16")
+        out, lse = uv.prompt_attention(q, k, v, starts([300]), scale=0.3, lse=True)
+        a, wl, size, reach = M.prompt(f64(q), f64(k), f64(v), True, 0.3)
+        eps = np.expm1(2 * (2.0 ** -17 * reach + 2.0 ** -14)) + UNIT["bfloat16"]
+        assert (np.abs(f64(out) - a) <= eps[..., None] * size * 1.02 + 2.0 ** -8 * np.abs(a) * 1.01).all()
+        assert (np.abs(f64(lse) - wl) <= 2.0 ** -17 * reach + 2.0 ** -13).all()
+
+
+def test_strides_streams_and_repeats(uv):
+    import torch
+
+    rng = np.random.default_rng(4)
+    n = starts([200, 57])
+    q, k, v = rows(rng, 257, 4, 128, "bfloat16"), rows(rng, 257, 2, 128, "bfloat16"), rows(rng, 257, 2, 128, "bfloat16")
+    want = uv.prompt_attention(q, k, v, n)
+    assert torch.equal(want, uv.prompt_attention(q, k, v, n))
+    one = torch.cat([q, k, v], 1)  # as a fused projection gives them
+    assert torch.equal(want, uv.prompt_attention(one[:, :4], one[:, 4:6], one[:, 6:], n))
+    qt = q.transpose(0, 1).contiguous().transpose(0, 1)
+    off = torch.zeros(257 * 2 * 128 + 3, dtype=torch.bfloat16, device="cuda")[3:].view(257, 2, 128)
+    off.copy_(v)
+    assert torch.equal(want, uv.prompt_attention(qt, k, off, n))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = uv.prompt_attention(q, k, v, n)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(want, got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = uv.prompt_attention(q, k, v, n)
+    got.zero_()
+    graph.replay()
+    assert torch.equal(want, got)
+
+
+def test_refused_arguments(uv):
+    import torch
+
+    rng = np.random.default_rng(5)
+    q = rows(rng, 10, 4, 128, "bfloat16")
+    n = starts([10])
+    for a in ((q, q[:, :3], q[:, :3]), (q, q, q[:, :2]), (q, q.half(), q), (q.float(), q.float(), q.float()),
+              (q[:, :, :96], q[:, :, :96], q[:, :, :96]), (q, q, q[:5]), (q.cpu(), q.cpu(), q.cpu())):
+        with pytest.raises((ValueError, uv.UVError)):
+            uv.prompt_attention(*a, n)
+    with pytest.raises(ValueError):
+        uv.prompt_attention(q, q, q, n.long())
+    with pytest.raises(ValueError):
+        uv.prompt_attention(q, q, q, n, torch.cat([n, n]))
+    with pytest.raises(uv.UVError):
+        uv.prompt_attention(q, q[:5], q[:5], n)
+    none = uv.prompt_attention(q[:0], q[:0], q[:0], starts([0]))
+    assert none.shape == (0, 4, 128)

@@ -9,3 +9,4 @@ from .binding import (Codec, CosetIndex, Index, IvfIndex, PreparedQueries, Shard
                       UVError, build, check, ivf_assign, kmeans, lib, topk_merge,
                       topk_merge_packed, topk_pack, topk_unpack, profile_enable, profile_read,
                       set_tuning, UV_SEARCH_COSINE, UV_SEARCH_MIPS, SYMBOLS)
+from .kv import KvCache, KvError, prompt_attention  # noqa: F401

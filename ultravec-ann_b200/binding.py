@@ -43,6 +43,10 @@ SYMBOLS = [
     "uv_index_search_begin", "uv_search_set_bounds", "uv_search_finish", "uv_search_destroy",
     "uv_search_finish_deferred", "uv_search_check",
     "uv_topk_pack", "uv_topk_merge_packed", "uv_search_bounds_per_query", "uv_topk_unpack",
+    "uv_kv_pool_bytes", "uv_kv_work_words", "uv_kv_seed", "uv_kv_reset", "uv_kv_recount",
+    "uv_kv_check", "uv_kv_extend", "uv_kv_fork", "uv_kv_copy", "uv_kv_truncate",
+    "uv_kv_compact", "uv_kv_append", "uv_kv_read", "uv_kv_attend_bytes", "uv_kv_attend",
+    "uv_prompt_attention",
 ]
 
 
@@ -69,7 +73,7 @@ def lib():
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH} is missing: run `make -C {HERE}` (nvcc, sm_100a)")
         L = C.CDLL(str(LIB_PATH))
-        vp, i32, i64, u64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
+        vp, i32, i64, u64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
         vpp = C.POINTER(C.c_void_p)
         sig = {
             "uv_abi_version": (C.c_int, []),
@@ -158,6 +162,26 @@ def lib():
             "uv_topk_unpack": (C.c_int, [i32, vp, i64, vp, vp, vp]),
             "uv_topk_merge_packed": (C.c_int, [i32, vp, i64, i32, i32, i64, i64, i32, vp, vp,
                                                vp]),
+            "uv_kv_pool_bytes": (C.c_int, [vp, C.POINTER(i64)]),
+            "uv_kv_work_words": (C.c_int, [vp, C.POINTER(i64)]),
+            "uv_kv_seed": (C.c_int, [vp, u64]),
+            "uv_kv_reset": (C.c_int, [vp, vp]),
+            "uv_kv_recount": (C.c_int, [vp, vp]),
+            "uv_kv_check": (C.c_int, [vp, C.POINTER(i32), vp]),
+            "uv_kv_extend": (C.c_int, [vp, vp, vp, i32, vp]),
+            "uv_kv_fork": (C.c_int, [vp, vp, vp, vp, i32, vp]),
+            "uv_kv_copy": (C.c_int, [vp, vp, vp, i32, vp]),
+            "uv_kv_truncate": (C.c_int, [vp, vp, vp, i32, vp]),
+            "uv_kv_compact": (C.c_int, [vp, vp]),
+            "uv_kv_append": (C.c_int, [vp, i32, vp, vp, i32, i32, i32, vp, i64, i64, vp, i64,
+                                       i64, vp]),
+            "uv_kv_read": (C.c_int, [vp, i32, vp, vp, i32, i32, i32, vp, vp, vp]),
+            "uv_kv_attend_bytes": (C.c_int, [vp, i32, i32, i32, i32, C.POINTER(i64)]),
+            "uv_kv_attend": (C.c_int, [vp, i32, vp, vp, i32, i32, i32, i32, vp, i64, i64, i32,
+                                       f32, vp, vp, vp, i64, vp]),
+            "uv_prompt_attention": (C.c_int, [i32, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32,
+                                              i32, vp, i64, i64, vp, i64, i64, vp, i64, i64, vp,
+                                              vp, vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)

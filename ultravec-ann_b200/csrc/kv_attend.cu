@@ -1,0 +1,709 @@
+// kv_attend.cu -- attention of one or more query rows a sequence over the
+// cache held in 4 bits: for a query head with rotated row q and its key
+// head's tokens j (scales s_j, levels l_j),
+//   e_j = scale * s_j <q, l_j>,   out = R^T sum_j softmax(e)_j s'_j l'_j,
+// over the tokens the row may see (its own position and those before it).
+//
+// Bound: HBM, D + 8 bytes a token and key head; the work behind each byte is
+// unpacking (9 instructions for 8 codes) and two products with 8 columns.
+// The columns of a block are (row, query head of the group) pairs of one
+// sequence and key head, so the codes are read and unpacked once for the whole
+// group.  Codes are the A operand of m16n8k16 (keys as rows for q k, dimensions
+// as rows for p v): with 8 query columns no row of the product is padding,
+// while a 128-row tcgen05 tile would be 94% padding on one side.
+//
+// Split: all tiles (32 tokens) of all (sequence, column tile, head) jobs lie in
+// one line, cut into equal pieces, one for each block of a single wave,
+// whatever the lengths are: the host need not know them.  A piece may hold the
+// end of a job, whole jobs and the start of another; each part leaves its
+// maximum, sum and unnormalised output in scratch, and a second kernel joins a
+// job's parts in order, rotates back and rounds.
+//
+// Numbers: q is rotated in f32 and rounded once to a half, after a power of
+// two that brings its row to size 1 (2^-11 relative, below the 4-bit keys'
+// error by 2^6); levels are exact halves; scores, maxima and sums are f32.  The
+// weights are rounded to halves after the multiplication by their token's
+// value scale, itself divided by a power of two that follows the largest scale
+// seen, so they neither overflow nor lose more than 2^-11.  The running
+// maximum moves only when a score exceeds it by 2^8, which keeps the weights
+// below 2^8 and the rescaling of the sums rare.
+#include <cfloat>
+
+#include "uv_kv.h"
+
+namespace uvb {
+namespace kv {
+
+constexpr int kWarps = 4, kAttendThreads = 32 * kWarps;
+constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int D>
+__host__ __device__ constexpr int stages() {  // 4 warps' rings fit a third of an SM's shared memory
+  return 512 / D;
+}
+
+// Scratch: per entry the first tile and the first job, tiles per worker, then
+// one part for every (job + worker): it grows with either, so it is theirs.
+struct Parts {
+  int64_t *head;  // [0] tiles per worker; first tiles from [1], first jobs from [n + 2]
+  float *o;       // slots x columns x D
+  float2 *ml;     // slots x columns: maximum (log2) and sum
+};
+__host__ __device__ __forceinline__ int64_t head_bytes(int n) {
+  return ((2 * (int64_t)n + 4) * 8 + 127) & ~127ll;
+}
+__device__ __forceinline__ Parts carve(void *p, int n, int64_t slots, int cols, int D) {
+  float *o = (float *)((char *)p + head_bytes(n));
+  return {(int64_t *)p, o, (float2 *)(o + slots * cols * D)};
+}
+
+struct Job {
+  int seq, first, n, len, tiles, col_tiles;
+};
+__device__ __forceinline__ Job load_entry(const Cache &c, const Rows &r, int b, int group,
+                                          int cols) {
+  Job j;
+  j.seq = r.seq(b, c.max_seqs);
+  j.first = r.first(b);
+  j.n = r.count(b);
+  j.len = j.seq < 0 ? 0 : c.length(j.seq);
+  j.tiles = (j.len + kTile - 1) / kTile;
+  j.col_tiles = (int)(((int64_t)j.n * group + cols - 1) / cols);
+  return j;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes,
+                                          uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(tc::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <int D>
+struct Words {
+  uint32_t w[D / 32];
+};
+template <int D>
+__device__ __forceinline__ Words<D> load_words(const uint8_t *p) {
+  Words<D> r;
+  if (D == 64) {
+    const uint2 v = *(const uint2 *)p;
+    r.w[0] = v.x;
+    r.w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < D / 128; i++) {
+      const uint4 v = ((const uint4 *)p)[i];
+      r.w[4 * i] = v.x;
+      r.w[4 * i + 1] = v.y;
+      r.w[4 * i + 2] = v.z;
+      r.w[4 * i + 3] = v.w;
+    }
+  }
+  return r;
+}
+
+// Shared memory of a block: the warps' rings of tiles; between segments the
+// same bytes join the warps' outputs.
+template <int D, int NT>
+struct AttendSmem {
+  static constexpr int kTileBytes = kTile * (D + 8);
+  static constexpr int kRing = kWarps * stages<D>() * kTileBytes;
+  static constexpr int kJoin = 8 * NT * (D + 4) * 4;
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+};
+
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(kAttendThreads, 3)
+    attend_kernel(Cache c, int layer, Rows rows, AttendArgs a, int64_t slots) {
+  constexpr int kCols = 8 * NT, kStages = stages<D>(), kTileBytes = AttendSmem<D, NT>::kTileBytes;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ int64_t sums[2][kWarps];
+  __shared__ int64_t begin[3];  // first entry of the piece, its first tile, its first job
+  __shared__ float join_m[kWarps][kCols], join_l[kWarps][kCols];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int group = a.q_heads / c.heads;
+  const Parts sc = carve(a.scratch, rows.n, slots, kCols, D);
+
+  if (lane == 0)
+    for (int i = 0; i < kStages; i++) tc::mbar_init(&full[warp][i], 1);
+  tc::mbar_fence_init();
+
+  // ---- this block's piece of the line of tiles ----
+  const int per_thread = (rows.n + kAttendThreads - 1) / kAttendThreads;
+  const int e0 = min(tid * per_thread, rows.n), e1 = min(e0 + per_thread, rows.n);
+  int64_t my_tiles = 0, my_jobs = 0;
+  for (int b = e0; b < e1; b++) {
+    const Job j = load_entry(c, rows, b, group, kCols);
+    const int64_t jobs = (int64_t)j.col_tiles * c.heads;
+    my_jobs += jobs;
+    my_tiles += jobs * j.tiles;
+  }
+  int64_t x = my_tiles, y = my_jobs;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) x += u, y += v;
+  }
+  if (lane == 31) sums[0][warp] = x, sums[1][warp] = y;
+  __syncthreads();
+  int64_t total = 0, before_t = x - my_tiles, before_j = y - my_jobs;
+  for (int w = 0; w < kWarps; w++) {
+    total += sums[0][w];
+    if (w < warp) before_t += sums[0][w], before_j += sums[1][w];
+  }
+  // at least one tile for every warp of a block
+  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kWarps);
+  const int64_t T0 = per * blockIdx.x, T1 = min(T0 + per, total);
+  if (blockIdx.x == 0) {  // for the join
+    int64_t bt = before_t, bj = before_j;
+    for (int b = e0; b < e1; b++) {
+      const Job j = load_entry(c, rows, b, group, kCols);
+      sc.head[1 + b] = bt;
+      sc.head[2 + rows.n + b] = bj;
+      bj += (int64_t)j.col_tiles * c.heads;
+      bt += (int64_t)j.col_tiles * c.heads * j.tiles;
+    }
+    if (e0 < rows.n && e1 == rows.n) {
+      sc.head[1 + rows.n] = bt;
+      sc.head[2 + 2 * rows.n] = bj;
+    }
+    if (tid == 0) sc.head[0] = per;
+  }
+  pdl_launch();
+  if (T0 >= T1) return;
+  if (T0 >= before_t && T0 < before_t + my_tiles) {
+    int64_t bt = before_t, bj = before_j;
+    for (int b = e0; b < e1; b++) {
+      const Job j = load_entry(c, rows, b, group, kCols);
+      const int64_t jobs = (int64_t)j.col_tiles * c.heads;
+      if (T0 < bt + jobs * j.tiles) {
+        begin[0] = b;
+        begin[1] = bt;
+        begin[2] = bj;
+        break;
+      }
+      bt += jobs * j.tiles;
+      bj += jobs;
+    }
+  }
+  __syncthreads();
+  int entry = (int)begin[0];
+  int64_t base_t = begin[1], base_j = begin[2];
+  Job job = load_entry(c, rows, entry, group, kCols);
+
+  uint8_t *ring = smem + warp * kStages * kTileBytes;
+  uint32_t issued = 0, taken = 0;  // tiles of this warp's ring
+  bool dead = false;
+
+  for (int64_t T = T0; T < T1;) {
+    while (T >= base_t + (int64_t)job.col_tiles * c.heads * job.tiles) {
+      base_t += (int64_t)job.col_tiles * c.heads * job.tiles;
+      base_j += (int64_t)job.col_tiles * c.heads;
+      entry++;
+      job = load_entry(c, rows, entry, group, kCols);
+    }
+    const int64_t local = T - base_t;
+    const int64_t jl = local / job.tiles;
+    const int j0 = (int)(local % job.tiles);
+    const int nj = (int)min((int64_t)(job.tiles - j0), T1 - T);
+    const int ct = (int)(jl / c.heads), head = (int)(jl % c.heads);
+    T += nj;
+
+    const int ncol = job.n * group, c0 = ct * kCols;
+    const int offset = job.len - job.n;  // position of the entry's first row
+    // the exclusive ends of what the tile's first and last rows may see
+    const int lim_first = offset + c0 / group + 1;
+    const int lim_last = offset + min((c0 + kCols - 1) / group, job.n - 1) + 1;
+    const int todo = max(0, min(nj, (lim_last + kTile - 1) / kTile - j0));
+    const int mine = todo > warp ? (todo - warp + kWarps - 1) / kWarps : 0;
+
+    // ---- start the ring ----
+    const int per_page = c.page_tokens / kTile;
+    const uint8_t *src = nullptr;
+    auto lookup = [&](int from) {  // tiles from .. from + 31 of this warp, one a lane
+      const int i = from + lane;
+      if (i < mine) {
+        const int j = j0 + warp + i * kWarps;
+        src = c.tile_at(layer, c.page_at(job.seq, j / per_page), head, j % per_page);
+      }
+    };
+    auto issue = [&](int i) {
+      const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)src, i & 31);
+      if (lane == 0 && !dead) {
+        const int slot = issued % kStages;
+        tc::mbar_arrive_expect_tx(&full[warp][slot], kTileBytes);
+        bulk_load(ring + slot * kTileBytes, p, kTileBytes, &full[warp][slot]);
+      }
+      issued++;
+    };
+    lookup(0);
+    for (int i = 0; i < min(mine, kStages); i++) issue(i);
+
+    // ---- the query columns, rotated, as B fragments ----
+    uint32_t qf[NT][D / 32][4];
+    float cs[NT][2], hs[NT][2];  // of the columns 2t, 2t + 1 of each 8
+    int lim[NT][2];
+#pragma unroll
+    for (int half = 0; half < (NT + 1) / 2; half++) {
+      uint32_t raw[2][D / 8];
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int col = c0 + 16 * half + 8 * r + g;
+        const bool live = (2 * half + r < NT) && col < ncol;
+        const int row = job.first + (live ? col / group : 0), hq = head * group + (live ? col % group : 0);
+        const uint4 *q = (const uint4 *)((const uint16_t *)a.q.p + (int64_t)row * a.q.row +
+                                         (int64_t)hq * a.q.head + t * (D / 4));
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          const uint4 v = live ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+          raw[r][4 * i] = v.x;
+          raw[r][4 * i + 1] = v.y;
+          raw[r][4 * i + 2] = v.z;
+          raw[r][4 * i + 3] = v.w;
+        }
+      }
+      float y[2][D / 4];
+      rotate_rows<D, BF16>(c, raw, y);
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        if (2 * half + r >= NT) break;
+        const int nt = 2 * half + r;
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) m = fmaxf(m, fabsf(y[r][j]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = max(-100, min(log2i(m), 126));
+        const float down = exp2i(-e);
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < D / 32; w++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t h = pack2<false>(__fmul_rn(y[r][8 * w + i], down),
+                                            __fmul_rn(y[r][8 * w + i + 4], down));
+            const float2 f = unpack2<false>(h);
+            sum = __fadd_rn(sum, __fadd_rn(f.x, f.y));
+            qf[nt][w][i] = h;
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // levels are codes - 7.5 and the unpacked halves codes - 8
+        const float h = __fmul_rn(0.5f, sum), cc = __fmul_rn(__fmul_rn(a.scale, kLog2e), exp2i(e));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          hs[nt][k] = __shfl_sync(0xffffffffu, h, 4 * (2 * t + k));
+          cs[nt][k] = __shfl_sync(0xffffffffu, cc, 4 * (2 * t + k));
+          const int col = c0 + 8 * nt + 2 * t + k;
+          lim[nt][k] = offset + min(col / group, job.n - 1) + 1;
+        }
+      }
+    }
+
+    float o[D / 16][NT][4], half_sum[NT][4], m[NT][2], l[NT][2];
+    int ve[NT][2];  // a column's value scales are divided by 2^ve
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int mt = 0; mt < D / 16; mt++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[mt][nt][k] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) half_sum[nt][k] = 0.0f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+      ve[nt][0] = ve[nt][1] = -100;
+    }
+
+    // ---- one pass over the warp's tiles ----
+    for (int i = 0; i < mine; i++) {
+      const int slot = taken % kStages;
+      if (!dead && !__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (taken / kStages) & 1,
+                                                          kWaitLimit))) {
+        // give up: note it, let the copies in flight land, load no more
+        if (lane == 0) atomicOr(&c.work[kStatus], kTimeout);
+        for (; taken < issued; taken++)
+          tc::mbar_wait(&full[warp][taken % kStages], (taken / kStages) & 1, kWaitLimit);
+        dead = true;
+      }
+      if (dead) break;
+      taken++;
+      const uint8_t *tile = ring + slot * kTileBytes;
+      const int key0 = (j0 + warp + i * kWarps) * kTile;
+
+      float s[2][NT][4];
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) s[sb][nt][k] = hs[nt][k & 1];
+        const uint8_t *rowp = tile + (16 * sb + g) * (D / 2) + t * (D / 8);
+        const Words<D> ka = load_words<D>(rowp), kb = load_words<D>(rowp + 8 * (D / 2));
+#pragma unroll
+        for (int w = 0; w < D / 32; w++) {
+          uint32_t xa[4], xb[4];
+          unpack8(ka.w[w], xa);
+          unpack8(kb.w[w], xb);
+#pragma unroll
+          for (int k = 0; k < 4; k += 2)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              mma16816<false>(s[sb][nt], xa[k], xb[k], xa[k + 1], xb[k + 1], qf[nt][w][k],
+                              qf[nt][w][k + 1]);
+        }
+      }
+      float ks[2][2], vs[2][2];
+      const float *kscale = (const float *)(tile + kTile * (D / 2));
+      const float *vscale = (const float *)(tile + kTile * (D + 4));
+      const bool whole = key0 + kTile <= lim_first;  // every column sees every token
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          ks[sb][r] = kscale[16 * sb + 8 * r + g];
+          vs[sb][r] = vscale[16 * sb + 8 * r + g];
+        }
+      // A column's largest score and largest finite value scale here, over the
+      // tokens that it sees: what it does not see must not move its references.
+      auto seen = [&](int nt, int k, int sb, int r) {
+        return whole || key0 + 16 * sb + 8 * r + g < lim[nt][k];
+      };
+      auto value_top = [&](int nt, int k) {
+        float v = 0.0f;
+#pragma unroll
+        for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+          for (int r = 0; r < 2; r++)
+            if (seen(nt, k, sb, r) && vs[sb][r] <= FLT_MAX) v = fmaxf(v, vs[sb][r]);
+        return v;
+      };
+      const float vall = value_top(0, 0);
+      bool jump = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              float &v = s[sb][nt][2 * r + k];
+              v = __fmul_rn(v, __fmul_rn(cs[nt][k], ks[sb][r]));
+              if (!seen(nt, k, sb, r)) v = -INFINITY;
+              top = fmaxf(top, v);
+            }
+          jump |= top > m[nt][k] + 8.0f;
+          jump |= (whole ? vall : value_top(nt, k)) > exp2i(min(ve[nt][k] + 4, 127));
+        }
+      if (__any_sync(0xffffffffu, jump)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            float top = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k]));
+            float vtop = value_top(nt, k);
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
+            }
+            const float nm = fmaxf(m[nt][k], top);
+            const int ne = max(ve[nt][k], min(log2i(vtop), 126));
+            const float f = nm == -INFINITY ? 1.0f : exp2_fast(__fsub_rn(m[nt][k], nm));
+            const float both = __fmul_rn(f, exp2_fast((float)(ve[nt][k] - ne)));
+            m[nt][k] = nm;
+            ve[nt][k] = ne;
+            l[nt][k] = __fmul_rn(l[nt][k], f);
+            half_sum[nt][k] = __fmul_rn(half_sum[nt][k], both);
+            half_sum[nt][2 + k] = __fmul_rn(half_sum[nt][2 + k], both);
+#pragma unroll
+            for (int mt = 0; mt < D / 16; mt++) {
+              o[mt][nt][k] = __fmul_rn(o[mt][nt][k], both);
+              o[mt][nt][2 + k] = __fmul_rn(o[mt][nt][2 + k], both);
+            }
+          }
+      }
+#pragma unroll
+      for (int sb = 0; sb < 2; sb++) {
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float w[4];
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float base = m[nt][k] == -INFINITY ? 0.0f : m[nt][k], down = exp2i(-ve[nt][k]);
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+              const float e = exp2_fast(__fsub_rn(s[sb][nt][2 * r + k], base));
+              l[nt][k] = __fadd_rn(l[nt][k], e);
+              // a token that is not seen weighs nothing even if its scale is no number
+              w[2 * r + k] = seen(nt, k, sb, r) ? __fmul_rn(e, __fmul_rn(vs[sb][r], down)) : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 2; r++) p[nt][r] = transpose8x8(pack2<false>(w[2 * r], w[2 * r + 1]));
+          mma16816<false>(half_sum[nt], 0x38003800u, 0x38003800u, 0x38003800u, 0x38003800u, p[nt][0],
+                          p[nt][1]);
+        }
+        const uint8_t *pairp = tile + kTile * (D / 2 + 4) + (8 * sb + t) * D + g * (D / 8);
+        const Words<D> va = load_words<D>(pairp), vb = load_words<D>(pairp + 4 * D);
+#pragma unroll
+        for (int w = 0; w < D / 32; w++) {
+          uint32_t xa[4], xb[4];
+          unpack8(va.w[w], xa);
+          unpack8(vb.w[w], xb);
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              mma16816<false>(o[2 * w + k][nt], xa[2 * k], xa[2 * k + 1], xb[2 * k], xb[2 * k + 1],
+                              p[nt][0], p[nt][1]);
+        }
+      }
+      __syncwarp();  // every lane has read the slot
+      const int next = i + kStages;
+      if (next < mine) {
+        if ((next & 31) == 0) lookup(next);
+        issue(next);
+      }
+    }
+
+    // ---- join the warps' parts ----
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2)
+          l[nt][k] = __fadd_rn(l[nt][k], __shfl_xor_sync(0xffffffffu, l[nt][k], x));
+        if (g == 0) {
+          join_m[warp][8 * nt + 2 * t + k] = m[nt][k];
+          join_l[warp][8 * nt + 2 * t + k] = l[nt][k];
+        }
+      }
+    __syncthreads();  // also: every ring is empty, its bytes are the join's
+    float *out = (float *)smem;
+    constexpr int kRow = D + 4;
+    for (int w = 0; w < kWarps; w++) {
+      if (w == warp) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const int col = 8 * nt + 2 * t + k;
+            float top = join_m[0][col];
+            for (int v = 1; v < kWarps; v++) top = fmaxf(top, join_m[v][col]);
+            const float f = m[nt][k] == -INFINITY
+                                ? 0.0f
+                                : __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
+#pragma unroll
+            for (int mt = 0; mt < D / 16; mt++) {
+              float2 *at = (float2 *)(out + col * kRow + g * (D / 8) + 2 * mt);
+              const float2 was = w == 0 ? make_float2(0.0f, 0.0f) : *at;
+              // a warp without a visible token adds nothing, whatever its sums hold
+              const float u = m[nt][k] == -INFINITY
+                                  ? 0.0f
+                                  : __fmul_rn(__fadd_rn(o[mt][nt][k], half_sum[nt][k]), f);
+              const float v = m[nt][k] == -INFINITY
+                                  ? 0.0f
+                                  : __fmul_rn(__fadd_rn(o[mt][nt][2 + k], half_sum[nt][k]), f);
+              *at = make_float2(__fadd_rn(was.x, u), __fadd_rn(was.y, v));
+            }
+          }
+      }
+      __syncthreads();
+    }
+    // (starts that do not rise give more jobs than rows allow: no slot, no part)
+    const int64_t slot = base_j + jl + blockIdx.x;
+    const bool fits = slot < slots;
+    for (int i = fits ? tid : kCols * D; i < kCols * (D / 4); i += kAttendThreads) {
+      const int col = i / (D / 4), d4 = i % (D / 4);
+      ((float4 *)(sc.o + (slot * kCols + col) * D))[d4] = *(const float4 *)(out + col * kRow + 4 * d4);
+    }
+    if (fits && tid < kCols) {
+      float top = join_m[0][tid], sum = 0.0f;
+      for (int v = 1; v < kWarps; v++) top = fmaxf(top, join_m[v][tid]);
+      for (int v = 0; v < kWarps; v++)
+        if (join_m[v][tid] != -INFINITY)
+          sum = __fmaf_rn(join_l[v][tid], exp2_fast(__fsub_rn(join_m[v][tid], top)), sum);
+      sc.ml[slot * kCols + tid] = make_float2(top, sum);
+    }
+    tc::fence_async_smem();  // the next bulk copies write where this joined
+    __syncthreads();
+  }
+}
+
+// ---- joining a job's parts ----
+template <int D, int NT, bool BF16>
+__global__ void __launch_bounds__(256) join_kernel(Cache c, Rows rows, AttendArgs a, int64_t slots) {
+  constexpr int kCols = 8 * NT, V = D / 32;
+  __shared__ float x[kCols][D + 4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int group = a.q_heads / c.heads;
+  const Parts sc = carve(a.scratch, rows.n, slots, kCols, D);
+  pdl_wait();
+  const int64_t *tiles = sc.head + 1, *jobs = sc.head + 2 + rows.n;
+  const int64_t J = blockIdx.x, per = sc.head[0];
+  if (J >= jobs[rows.n]) return;
+  int lo = 0, hi = rows.n - 1;  // the last entry whose first job is <= J
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (jobs[mid] <= J) lo = mid;
+    else hi = mid - 1;
+  }
+  const int b = lo;
+  const int64_t jl = J - jobs[b], nj = jobs[b + 1] - jobs[b];
+  const int64_t n_tiles = (tiles[b + 1] - tiles[b]) / nj, first = tiles[b] + jl * n_tiles;
+  const int64_t w0 = first / per;
+  const int parts = n_tiles == 0 ? 0 : (int)((first + n_tiles - 1) / per - w0) + 1;
+  const int ct = (int)(jl / c.heads), head = (int)(jl % c.heads);
+  const int ncol = rows.count(b) * group, row0 = rows.first(b);
+
+  for (int col = warp; col < kCols; col += 8) {
+    float top = -INFINITY, sum = 0.0f;
+    for (int i = lane; i < parts; i += 32)
+      top = fmaxf(top, sc.ml[(J + w0 + i) * kCols + col].x);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float acc[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) acc[v] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+      float f = 0.0f;
+      if (i0 + lane < parts) {
+        const float2 ml = sc.ml[(J + w0 + i0 + lane) * kCols + col];
+        f = ml.x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(ml.x, top));
+        sum = __fmaf_rn(ml.y, f, sum);
+      }
+      const int n = min(32, parts - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; i++) {
+        const float w = __shfl_sync(0xffffffffu, f, i);
+        const float *from = sc.o + ((J + w0 + i0 + i) * kCols + col) * D + lane * V;
+        float z[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) z[v] = from[v];
+#pragma unroll
+        for (int v = 0; v < V; v++) acc[v] = __fmaf_rn(z[v], w, acc[v]);
+      }
+    }
+    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+    const bool none = top == -INFINITY;  // no token to see: zeros
+    const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
+#pragma unroll
+    for (int v = 0; v < V; v++) x[col][lane * V + v] = none ? 0.0f : __fmul_rn(acc[v], inv);
+    const int at = ct * kCols + col;
+    if (lane == 0 && a.lse != nullptr && at < ncol)
+      a.lse[(int64_t)(row0 + at / group) * a.q_heads + head * group + at % group] =
+          none ? -INFINITY : __fmul_rn(__fadd_rn(top, __log2f(sum)), kLn2);
+  }
+  __syncthreads();
+  for (int half = warp; half < (NT + 1) / 2; half += 8) {
+    float y[2][D / 4];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int j = 0; j < D / 4; j++) {
+        const int col = 16 * half + 8 * r + g;
+        y[r][j] = col < kCols ? x[col < kCols ? col : 0][t * (D / 4) + j] : 0.0f;
+      }
+    rotate_back<D, 2>(c, y, true);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int col = 16 * half + 8 * r + g, at = ct * kCols + col;
+      if (col >= kCols || at >= ncol) continue;
+      uint4 *to = (uint4 *)((uint16_t *)a.out +
+                            ((int64_t)(row0 + at / group) * a.q_heads + head * group + at % group) * D +
+                            t * (D / 4));
+#pragma unroll
+      for (int i = 0; i < D / 32; i++)
+        to[i] = make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
+                           pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
+                           pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
+                           pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7]));
+    }
+  }
+}
+
+// ---- launches ----
+// Columns of a tile: the fewest eights that hold a sequence's usual columns,
+// so that one row of a group of 8 does not pay for 16; more columns than 16
+// (32 at D = 64) would not leave registers for three blocks an SM.
+static int column_eights(int D, int64_t cols) {
+  if (D == 256 || cols <= 8) return 1;
+  if (D == 128 || cols <= 16) return 2;
+  return 4;
+}
+
+AttendPlan attend_plan(const Cache &c, int n, int rows, int most, int q_heads, int sms) {
+  AttendPlan p;
+  const int group = q_heads / c.heads;
+  p.cols = 8 * column_eights(c.head_dim, (int64_t)group * most);
+  p.jobs = ((int64_t)rows * group / p.cols + n) * c.heads;
+  p.workers = 3 * sms;
+  const int64_t slots = p.jobs + p.workers;
+  p.bytes = head_bytes(n) + slots * p.cols * (c.head_dim + 2) * 4;
+  return p;
+}
+
+template <int D, int NT, bool BF16>
+static cudaError_t attend_nt(const Cache &c, int layer, const Rows &rows, const AttendArgs &a,
+                             const AttendPlan &plan, cudaStream_t st) {
+  const int64_t slots = plan.jobs + plan.workers;
+  const int smem = AttendSmem<D, NT>::kBytes;
+  static const cudaError_t set = cudaFuncSetAttribute(
+      attend_kernel<D, NT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (set != cudaSuccess) return set;
+  attend_kernel<D, NT, BF16><<<plan.workers, kAttendThreads, smem, st>>>(c, layer, rows, a, slots);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)plan.jobs);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D, NT, BF16>, c, rows, a, slots);
+}
+
+template <bool BF16>
+static cudaError_t attend_t(const Cache &c, int layer, const Rows &rows, const AttendArgs &a,
+                            const AttendPlan &p, cudaStream_t st) {
+  if (c.head_dim == 256) return attend_nt<256, 1, BF16>(c, layer, rows, a, p, st);
+  if (c.head_dim == 128)
+    return p.cols == 8 ? attend_nt<128, 1, BF16>(c, layer, rows, a, p, st)
+                       : attend_nt<128, 2, BF16>(c, layer, rows, a, p, st);
+  if (p.cols == 8) return attend_nt<64, 1, BF16>(c, layer, rows, a, p, st);
+  if (p.cols == 16) return attend_nt<64, 2, BF16>(c, layer, rows, a, p, st);
+  return attend_nt<64, 4, BF16>(c, layer, rows, a, p, st);
+}
+
+cudaError_t attend_launch(const Cache &c, int layer, const Rows &rows, const AttendArgs &a,
+                          const AttendPlan &plan, bool bf16, cudaStream_t st) {
+  return bf16 ? attend_t<true>(c, layer, rows, a, plan, st)
+              : attend_t<false>(c, layer, rows, a, plan, st);
+}
+
+}  // namespace kv
+}  // namespace uvb

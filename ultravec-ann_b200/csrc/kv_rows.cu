@@ -1,0 +1,324 @@
+// kv_rows.cu -- rows into the cache held in 4 bits (rotate, quantise, write
+// into the pages) and back out of it (levels, rotate back).
+//
+// A warp takes 16 consecutive token positions of one head, aligned to 16, of
+// the keys or of the values: lane (g, t) holds a quarter of rows g and g + 8.
+// The rotation's first four index bits go through the tensor core (16 m16n8k16
+// for 16 rows of 128), the others are register butterflies; a row's sums cross
+// 4 lanes.  Positions outside the call's rows are computed as zeros and not
+// stored.
+//
+// Bound: HBM for prompts (2 D bytes of a row in, D / 2 + 4 out, and the
+// reverse), latency for a token each.
+#include "uv_kv.h"
+
+namespace uvb {
+namespace kv {
+
+constexpr int kRowThreads = 128;
+
+// Block u of 16 positions: its entry's sequence, the block's first position,
+// the first position that a row has, and the row of position x, first + x.
+// Entry b has starts[b + 1] / 16 - starts[b] / 16 + 2 blocks, never fewer than
+// its rows can touch, so the map needs the starts alone.  blank: rows of the
+// entry before the sequence's first token, told to its first block alone.
+struct Block {
+  int seq, len, pos0, begin, first, blank, row0;
+};
+__device__ __forceinline__ Block find_block(const Rows &r, const Cache &c, int64_t u) {
+  int b;
+  int64_t k = 0;
+  if (r.starts == nullptr) {
+    b = (int)u;
+  } else {
+    int lo = 0, hi = r.n - 1;  // the last entry whose first block is <= u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (r.first(mid) / 16 + 2 * (int64_t)mid <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    k = u - (r.first(b) / 16 + 2 * (int64_t)b);
+  }
+  Block x;
+  x.seq = r.seq(b, c.max_seqs);
+  x.row0 = r.first(b);
+  const int n = r.count(b);
+  x.len = x.seq < 0 ? 0 : c.length(x.seq);
+  const int start = x.len - n;
+  x.begin = max(start, 0);
+  x.first = x.row0 - start;
+  x.blank = k == 0 ? max(-start, 0) : 0;
+  const int64_t p = (int64_t)(x.begin / 16 + k) * 16;
+  x.pos0 = (int)min(p, (int64_t)x.len);  // past the end: no position
+  return x;
+}
+
+// 8 f32 codes -> word; t[j] = code + 1.5 * 2^23 exactly.
+__device__ __forceinline__ uint32_t pack_codes(const float *t) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; j--) w = w * 16u + __float_as_uint(t[j]);
+  // every term carried 0x4b400000: take the sum of its shifted copies out
+  return w - 0x4b400000u * 0x11111111u;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer, Rows rows,
+                                                             Strided kin, Strided vin,
+                                                             int64_t blocks) {
+  if (c.work[kStatus] != 0) return;  // an extend failed: these rows have no place
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int parts = 2 * c.heads;
+  if (item >= blocks * parts) return;
+  const int part = (int)(item % parts), head = part >> 1;
+  const bool value = part & 1;
+  const Block at = find_block(rows, c, item / parts);
+  const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
+  if (s < 0 && lane == 0) atomicOr(&c.work[kStatus], kBadSeq);
+  if (pos0 >= len) return;
+  const Strided &in = value ? vin : kin;
+  const uint16_t *src = (const uint16_t *)in.p + (int64_t)head * in.head + t * (D / 4);
+
+  uint32_t a[2][D / 8];
+  bool live[2];
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    const int p = pos0 + g + 8 * r;
+    live[r] = p >= begin && p < len;
+    const uint4 *q = (const uint4 *)(src + (int64_t)(first + p) * in.row);
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      const uint4 w = live[r] ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+      a[r][4 * i] = w.x;
+      a[r][4 * i + 1] = w.y;
+      a[r][4 * i + 2] = w.z;
+      a[r][4 * i + 3] = w.w;
+    }
+  }
+  const int page = c.page_at(s, pos0 / c.page_tokens);
+  if (c.refs[page] != 1) {  // others hold it: extend has not made room
+    if (lane == 0) atomicOr(&c.work[kStatus], kShared);
+    return;
+  }
+  float y[2][D / 4];
+  rotate_rows<D, BF16>(c, a, y);
+
+  uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
+                  (value ? kTile * (D / 2 + 4) : 0);
+  const int row0 = pos0 % kTile;
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    // a power of two takes the row's size out, so that squares neither
+    // overflow nor vanish
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 4; j++) m = fmaxf(m, fabsf(y[r][j]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int e = max(-100, min(log2i(m), 126));
+    const float down = exp2i(-e);
+    float square = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 4; j++) {
+      y[r][j] = __fmul_rn(y[r][j], down);
+      square = __fmaf_rn(y[r][j], y[r][j], square);
+    }
+    square += __shfl_xor_sync(0xffffffffu, square, 1);
+    square += __shfl_xor_sync(0xffffffffu, square, 2);
+    const float inv = square > 0.0f
+                          ? __fdiv_rn(1.0f, __fmul_rn(kStep, __fsqrt_rn(__fmul_rn(square, 1.0f / D))))
+                          : 0.0f;
+    float ly = 0.0f;
+    uint32_t w[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      float n[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float z = fminf(fmaxf(__fmul_rn(y[r][8 * i + j], inv), -8.0f), 7.0f);
+        n[j] = __fadd_rd(z, 12582920.0f);  // 1.5 * 2^23 + 8, rounded down: floor(z) + 8
+        ly = __fmaf_rn(__fadd_rn(__fsub_rn(n[j], 12582920.0f), 0.5f), y[r][8 * i + j], ly);
+      }
+      w[i] = pack_codes(n);
+    }
+    ly += __shfl_xor_sync(0xffffffffu, ly, 1);
+    ly += __shfl_xor_sync(0xffffffffu, ly, 2);
+    // |y| finite and not zero: ly > 0, since every level has its value's sign
+    // (a row of zeros has the scale zero; one with an infinity or a NaN gets NaN)
+    const float scale = square == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(square, ly), exp2i(e));
+    const int row = row0 + g + 8 * r;
+    if (live[r] && t == 0) ((float *)(tile + kTile * (D / 2)))[row] = scale;
+    if (!value) {
+      if (live[r]) {
+        uint32_t *to = (uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
+        if (D == 128) {
+          *(uint4 *)to = make_uint4(w[0], w[1], w[2], w[D / 32 - 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 32; i++) to[i] = w[i];
+        }
+      }
+      continue;
+    }
+    // Tokens 2p and 2p + 1 are lanes g and g ^ 1: the even one takes the
+    // granules of dimensions 0..3 of each word, the odd one those of 4..7.
+    const bool odd = g & 1;
+    const bool other = __shfl_xor_sync(0xffffffffu, (int)live[r], 4);
+    uint16_t *pair = (uint16_t *)(tile + (row >> 1) * D) + t * (D / 8);
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      const uint32_t x = __shfl_xor_sync(0xffffffffu, w[i], 4);
+      if (live[r] && other) {
+        ((uint32_t *)pair)[2 * i + odd] =
+            odd ? (x >> 16) | (w[i] & 0xffff0000u) : (w[i] & 0xffffu) | (x << 16);
+      } else if (live[r]) {
+        pair[4 * i + odd] = (uint16_t)w[i];
+        pair[4 * i + 2 + odd] = (uint16_t)(w[i] >> 16);
+      }
+    }
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kRowThreads) read_kernel(Cache c, int layer, Rows rows,
+                                                           uint16_t *kout, uint16_t *vout,
+                                                           int64_t blocks) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int parts = 2 * c.heads;
+  if (item >= blocks * parts) return;
+  const int part = (int)(item % parts), head = part >> 1;
+  const bool value = part & 1;
+  const Block at = find_block(rows, c, item / parts);
+  const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
+  uint16_t *out = (value ? vout : kout) + head * D;
+  for (int i = lane; i < at.blank * (D / 8); i += 32)  // rows without a token read as zeros
+    ((uint4 *)(out + (int64_t)(at.row0 + i / (D / 8)) * c.heads * D))[i % (D / 8)] =
+        make_uint4(0, 0, 0, 0);
+  if (pos0 >= len) return;
+  const int page = c.page_at(s, pos0 / c.page_tokens);
+  const uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
+                        (value ? kTile * (D / 2 + 4) : 0);
+  const int row0 = pos0 % kTile;
+  bool live[2];
+  float scale[2];
+  uint32_t w[2][D / 32];
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    const int row = row0 + g + 8 * r, p = pos0 + g + 8 * r;
+    live[r] = p >= begin && p < len;
+    scale[r] = live[r] ? ((const float *)(tile + kTile * (D / 2)))[row] : 0.0f;
+    if (!value) {
+      const uint32_t *from = (const uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) w[r][i] = from[i];
+    } else {
+      const bool odd = g & 1;
+      const uint32_t *pair = (const uint32_t *)(tile + (row >> 1) * D) + t * (D / 16);
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const uint32_t x = pair[2 * i], y = pair[2 * i + 1];
+        w[r][i] = __byte_perm(x, y, odd ? 0x7632 : 0x5410);
+      }
+    }
+  }
+  // The levels are exact halves, so the first transform needs one product.
+  // A half2 holds the nibbles i and i + 4 of a word: with the element's bits
+  // renamed (2, 0, 1 for 0, 1, 2) the owner of every output stays the same.
+  float y[2][D / 4];
+#pragma unroll
+  for (int j = 0; j < D / 4; j++) y[0][j] = y[1][j] = 0.0f;
+  uint32_t a[2][D / 8];
+#pragma unroll
+  for (int r = 0; r < 2; r++)
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+      uint32_t o[4];
+      unpack8(w[r][i], o);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const __half2 h = __hadd2(*reinterpret_cast<__half2 *>(&o[k]), __float2half2_rn(0.5f));
+        a[r][4 * i + k] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+  hadamard_mma<D, false>(y, a, Hadamard::make<false>());
+  hadamard_rest<D>(y);
+#pragma unroll
+  for (int r = 0; r < 2; r++)
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {  // element 2 k + h of a word -> k + 4 h
+      float o[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) o[(k >> 1) + 4 * (k & 1)] = y[r][8 * i + k];
+#pragma unroll
+      for (int k = 0; k < 8; k++) y[r][8 * i + k] = __fmul_rn(o[k], scale[r]);
+    }
+  rotate_back<D, 3>(c, y, false);
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    if (!live[r]) continue;
+    uint4 *to = (uint4 *)(out + (int64_t)(first + pos0 + g + 8 * r) * c.heads * D + t * (D / 4));
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+      __stcs(to + i, make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
+                                pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
+                                pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
+                                pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7])));
+  }
+}
+
+static int64_t block_bound(const Rows &r) {
+  return r.starts == nullptr ? r.n : r.rows / 16 + 2 * (int64_t)r.n;
+}
+
+template <int D, bool BF16>
+static cudaError_t append_d(const Cache &c, int layer, const Rows &rows, const Strided &k,
+                            const Strided &v, cudaStream_t st) {
+  const int64_t blocks = block_bound(rows), warps = blocks * 2 * c.heads;
+  const int64_t grid = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
+  append_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, k, v, blocks);
+  return cudaGetLastError();
+}
+template <int D, bool BF16>
+static cudaError_t read_d(const Cache &c, int layer, const Rows &rows, void *k, void *v,
+                          cudaStream_t st) {
+  const int64_t blocks = block_bound(rows), warps = blocks * 2 * c.heads;
+  const int64_t grid = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
+  read_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, (uint16_t *)k,
+                                                               (uint16_t *)v, blocks);
+  return cudaGetLastError();
+}
+
+cudaError_t append_launch(const Cache &c, int layer, const Rows &rows, const Strided &k,
+                          const Strided &v, bool bf16, cudaStream_t st) {
+  switch (c.head_dim) {
+    case 64:
+      return bf16 ? append_d<64, true>(c, layer, rows, k, v, st)
+                  : append_d<64, false>(c, layer, rows, k, v, st);
+    case 128:
+      return bf16 ? append_d<128, true>(c, layer, rows, k, v, st)
+                  : append_d<128, false>(c, layer, rows, k, v, st);
+    default:
+      return bf16 ? append_d<256, true>(c, layer, rows, k, v, st)
+                  : append_d<256, false>(c, layer, rows, k, v, st);
+  }
+}
+cudaError_t read_launch(const Cache &c, int layer, const Rows &rows, void *k, void *v, bool bf16,
+                        cudaStream_t st) {
+  switch (c.head_dim) {
+    case 64:
+      return bf16 ? read_d<64, true>(c, layer, rows, k, v, st)
+                  : read_d<64, false>(c, layer, rows, k, v, st);
+    case 128:
+      return bf16 ? read_d<128, true>(c, layer, rows, k, v, st)
+                  : read_d<128, false>(c, layer, rows, k, v, st);
+    default:
+      return bf16 ? read_d<256, true>(c, layer, rows, k, v, st)
+                  : read_d<256, false>(c, layer, rows, k, v, st);
+  }
+}
+
+}  // namespace kv
+}  // namespace uvb
