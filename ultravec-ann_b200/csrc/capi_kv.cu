@@ -366,7 +366,7 @@ int uv_prompt_attention(int32_t device, const int32_t *starts_q, const int32_t *
   a.lse = lse;
   DeviceGuard g(device);
   ProfScope ps("prompt_attention", (cudaStream_t)stream);
-  UV_CK(prompt::launch(a, sm_count(device), (cudaStream_t)stream));
+  UV_CK(prompt::launch(a, (cudaStream_t)stream));
   return UV_OK;
 }
 

@@ -5,200 +5,595 @@
 // j <= i + (keys - queries).  out = softmax(scale q k^T) v, a row that sees
 // nothing is zero.
 //
-// A warp holds 16 query rows; scores, maxima and sums stay in registers (f32)
-// over one pass of 64-key tiles in shared memory.
+// A block holds two tiles of 128 query rows that share their keys: two heads of
+// a group, or 256 consecutive rows where the group is odd.  Per 128 keys and
+// tile: S = Q K^T into TMEM (tcgen05, M = N = 128), a warpgroup with one row a
+// thread takes S into registers (maximum, exponentials and sum without any
+// shuffle), writes P back over S, and O += P V takes P from TMEM.  While one
+// tile is in its softmax the tensor core works for the other.
+//
+//   warps 0-3, 4-7   softmax and output of the two tiles
+//   warp 8           issues the products (one lane), owns the TMEM
+//   warp 9           loads Q, K, V by TMA (one lane)
+//   warps 10, 11     mend the values of blocks with masked keys (below)
+//
+// Blocks of keys go from the last, masked ones to the first.  O is rescaled
+// only when a row's maximum grows by more than 2^8, in TMEM by its own warp.
 //
 // What a row does not see must not reach it, but a weight of zero times a value
-// of infinity or NaN is a NaN.  So in tiles with a masked key such values are
-// taken out, and for every column the first key that held one is kept: rows
-// that see that key get it added to their output.
+// of infinity or NaN is a NaN.  So in blocks with a masked key such values are
+// taken out (as are the next sequence's rows), and for every column the first
+// key that held one is kept: rows that see that key get it added to their
+// output.
+//
+// Bound: per 128 x 128 tile and D = 128 the two products take 1024 cycles of
+// the tensor core and the exponentials 1024 of the MUFU (16 a cycle), so part of
+// the exponentials is computed by a polynomial in the FMA pipe instead.
+#include <cfloat>
 #include <climits>
+#include <cuda.h>
 
+#include "capi_internal.h"
 #include "uv_prompt.h"
 
 namespace uvb {
 namespace prompt {
 
-using kv::mma16816;
-using kv::pack2;
-
-constexpr int kRows = 64, kKeys = 64, kThreads = 128;
+constexpr int kRows = 128, kKeys = 128, kThreads = 384, kSlots = 5;
+constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// 2^f on [-1/2, 1/2], relative error below 2.7e-6: a least-squares fit of the relative
+// error with weights that drive it to its minimax, made for this file
+constexpr float kC0 = 0.9999992847442627f, kC1 = 0.6931217908859253f, kC2 = 0.240247443318367f,
+                kC3 = 0.05591785907745361f, kC4 = 0.009570101276040077f;
+constexpr int kPoly = 2, kPolyOf = 8;  // of kPolyOf columns, kPoly take the polynomial
+constexpr float kGrow = 8.0f;  // log2 of the growth that a maximum may leave unanswered
 
+__device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(tc::smem_u32(p)));
-}
-__device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads) simple_kernel(Args a) {
-  constexpr int kPitch = D + 8;  // halves: rows 16 bytes apart modulo 128
-  __shared__ __align__(16) uint16_t ks[kKeys][kPitch], vs[kKeys][kPitch];
-  __shared__ int odd[3][D];  // the first key whose value is NaN, +inf, -inf
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  // entry b has starts_q[b + 1] / 64 - starts_q[b] / 64 + 1 tiles
-  const int64_t u = blockIdx.x;
+// ---- pairs of floats ----
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x for two x in the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by the
+// polynomial of degree 4, n added to the exponent.  x below -126 gives 2^-126
+// (the caller makes masked weights exact zeros) and so does NaN (the caller's
+// row has NaN from its other columns then).
+__device__ __forceinline__ float2 exp2_poly(f2 x) {
+  const float2 v = split(x);
+  x = pair(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  const f2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
+  const f2 n = add2(x, magic), whole = add2(n, minus);
+  const f2 f = fma2(whole, pair(-1.0f, -1.0f), x);
+  f2 p = pair(kC4, kC4);
+  p = fma2(p, f, pair(kC3, kC3));
+  p = fma2(p, f, pair(kC2, kC2));
+  p = fma2(p, f, pair(kC1, kC1));
+  p = fma2(p, f, pair(kC0, kC0));
+  const float2 pf = split(p), nf = split(n);
+  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(nf.x) << 23)),
+                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(nf.y) << 23)));
+}
+
+// ---- tensor core plumbing beside uv_tc.cuh ----
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z,
+                                            uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(tc::smem_u32(dst)),
+      "l"((uint64_t)map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// D += A B with A in TMEM (row i in lane i, K pairs low half first).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of a B operand whose N index is contiguous (values as they lie:
+// rows are keys): 64 columns (128 bytes, 128-byte swizzle) a block of N, blocks
+// `block` bytes apart, 8 keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc_n(uint32_t addr, uint32_t block) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)(block >> 4) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// kind::f16 with f32 accumulators: format of A and B in [7,10) and [10,13)
+// (1 = bfloat), bit 16: B's N index is the contiguous one.
+__device__ __forceinline__ constexpr uint32_t idesc(int M, int N, bool bf16, bool b_n) {
+  return tc::idesc_f16_f32(M, N) | (bf16 ? (1u << 7 | 1u << 10) : 0u) | (b_n ? 1u << 16 : 0u);
+}
+
+template <int D>
+struct Shape {
+  static constexpr int kTile = 128 * D * 2;  // bytes of 128 rows
+  static constexpr int kQ = 0, kRing = 2 * kTile, kOdd = kRing + kSlots * kTile;
+  static constexpr int kBars = kOdd + 3 * D * 4;
+  static constexpr int kBytes = kBars + 256;
+  static constexpr int kO = 256;  // TMEM: S of both tiles, then O of both
+};
+
+// What a block works on.
+struct Item {
+  int q0, nq, k0, nk;     // the sequence's rows
+  int head[2], i0[2];     // a tile's head and first row in the sequence
+  int blocks[2], n;       // key blocks of a tile, and of the longer one
+  int whole;              // blocks below this one have no masked key
+};
+
+__device__ __forceinline__ int limit(const Args &a, const Item &it, int row) {
+  return a.causal ? max(0, min(it.nk, row + it.nk - it.nq + 1)) : it.nk;
+}
+
+__device__ __forceinline__ bool find_item(const Args &a, Item *it) {
+  const int group = a.q_heads / a.heads;
+  const bool twins = group % 2 == 0;  // two heads of a group, or two tiles of rows
+  const int rows = twins ? kRows : 2 * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
+  const int64_t tiles = a.rows_q / rows + a.n;
+  // the last tiles, which see the most keys, start first
+  const int64_t u = tiles - 1 - blockIdx.x / heads;
+  const int h = blockIdx.x % heads;
+  // entry b has starts_q[b + 1] / rows - starts_q[b] / rows + 1 tiles
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (bounded(a.starts_q[mid], a.rows_q) / kRows + mid <= u) lo = mid;
+    if (bounded(a.starts_q[mid], a.rows_q) / rows + mid <= u) lo = mid;
     else hi = mid - 1;
   }
-  const int b = lo, q0 = bounded(a.starts_q[b], a.rows_q);
-  const int nq = bounded(a.starts_q[b + 1], a.rows_q) - q0;
-  const int i0 = (int)(u - (q0 / kRows + b)) * kRows;
-  if (i0 >= nq) return;
-  const int k0 = bounded(a.starts_k[b], a.rows_k);
-  const int nk = max(0, bounded(a.starts_k[b + 1], a.rows_k) - k0);
-  const int head = blockIdx.y, kh = head / (a.q_heads / a.heads);
-  const uint16_t *kp = (const uint16_t *)a.k.p + (int64_t)kh * a.k.head;
-  const uint16_t *vp = (const uint16_t *)a.v.p + (int64_t)kh * a.v.head;
-
-  uint32_t qf[D / 16][4];
-  const int row[2] = {i0 + 16 * warp + g, i0 + 16 * warp + g + 8};
-#pragma unroll
-  for (int s = 0; s < D / 16; s++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int i = row[r & 1];
-      qf[s][r] = i < nq ? *(const uint32_t *)((const uint16_t *)a.q.p + (int64_t)(q0 + i) * a.q.row +
-                                              (int64_t)head * a.q.head + 16 * s + 2 * t + 8 * (r >> 1))
-                        : 0u;
+  it->q0 = bounded(a.starts_q[lo], a.rows_q);
+  it->nq = bounded(a.starts_q[lo + 1], a.rows_q) - it->q0;
+  const int64_t i0 = (u - (it->q0 / rows + lo)) * rows;
+  if (i0 < 0 || i0 >= it->nq) return false;
+  it->k0 = bounded(a.starts_k[lo], a.rows_k);
+  it->nk = max(0, bounded(a.starts_k[lo + 1], a.rows_k) - it->k0);
+  int first = INT_MAX;
+  it->n = 0;
+  for (int t = 0; t < 2; t++) {
+    it->head[t] = twins ? 2 * h + t : h;
+    it->i0[t] = (int)i0 + (twins ? 0 : t * kRows);
+    it->blocks[t] = 0;
+    if (it->i0[t] < it->nq) {
+      it->blocks[t] =
+          (limit(a, *it, min(it->i0[t] + kRows, it->nq) - 1) + kKeys - 1) / kKeys;
+      first = min(first, limit(a, *it, it->i0[t]));
     }
-  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int d = 0; d < D / 8; d++)
-#pragma unroll
-    for (int k = 0; k < 4; k++) o[d][k] = 0.0f;
-  int lim[2];
-#pragma unroll
-  for (int r = 0; r < 2; r++) lim[r] = a.causal ? min(nk, row[r] + nk - nq + 1) : nk;
-  const int end = a.causal ? min(nk, i0 + kRows + nk - nq) : nk;
-  const float c = __fmul_rn(a.scale, kLog2e);
+    it->n = max(it->n, it->blocks[t]);
+  }
+  it->whole = first / kKeys;
+  return true;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const Args a, const __grid_constant__ CUtensorMap qmap,
+                  const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap) {
+  using L = Shape<D>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  int(*odd)[D] = (int(*)[D])(sm + L::kOdd);  // the first key whose value is NaN, +inf, -inf
+  uint64_t *bars = (uint64_t *)(sm + L::kBars);
+  uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + kSlots;
+  uint64_t *s_full = kv_empty + kSlots, *p_ready = s_full + 2, *o_done = p_ready + 2;
+  uint64_t *mended = o_done + 2, *drained = mended + 1;
+  uint32_t *tmem_s = (uint32_t *)(drained + 1);
+  volatile int *abort_s = (volatile int *)(tmem_s + 1);
+
+  Item it;
+  if (!find_item(a, &it)) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kv_head = it.head[0] / (a.q_heads / a.heads);
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_ready[i], 4);
+      tc::mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < kSlots; i++) {
+      tc::mbar_init(&kv_full[i], 1);
+      tc::mbar_init(&kv_empty[i], 1);
+    }
+    tc::mbar_init(mended, 64);
+    tc::mbar_init(drained, 1);
+    *abort_s = 0;
+    tc::mbar_fence_init();
+  }
   for (int i = tid; i < 3 * D; i += kThreads) odd[i / D][i % D] = INT_MAX;
+  if (warp == 8) tc::tmem_alloc(tmem_s, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_s;
+  const int n = it.n, flagged = max(0, n - it.whole);
 
-  for (int j0 = 0; j0 < end; j0 += kKeys) {
-    __syncthreads();
-    for (int i = tid; i < kKeys * (D / 8); i += kThreads) {
-      const int j = i / (D / 8), d = i % (D / 8) * 8;
-      uint4 x = make_uint4(0, 0, 0, 0), y = x;
-      if (j0 + j < nk) {
-        x = *(const uint4 *)(kp + (int64_t)(k0 + j0 + j) * a.k.row + d);
-        y = *(const uint4 *)(vp + (int64_t)(k0 + j0 + j) * a.v.row + d);
+  if (warp < 8) {
+    // ================= softmax: thread = row =================
+    const int t = warp >> 2, row = it.i0[t] + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
+    const int blocks = it.blocks[t], lim = limit(a, it, row);
+    const int first = limit(a, it, it.i0[t]);
+    const float c = __fmul_rn(a.scale, kLog2e);
+    float m = -INFINITY;
+    f2 l0 = 0, l1 = 0;
+    bool ok = true;
+    for (int j = blocks - 1, i = 0; j >= 0; j--, i++) {
+      ok = ok && tc::mbar_wait(&s_full[t], i & 1, kWaitLimit) && !*abort_s;
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        *abort_s = 1;
+        break;
       }
-      *(uint4 *)&ks[j][d] = x;
-      *(uint4 *)&vs[j][d] = y;
-    }
-    __syncthreads();
-    if (a.causal ? j0 + kKeys > i0 + nk - nq + 1 : j0 + kKeys > nk) {  // some row does not see all
-      constexpr uint16_t kExp = BF16 ? 0x7f80 : 0x7c00;
-      for (int i = tid; i < kKeys * D; i += kThreads) {
-        const uint16_t x = vs[i / D][i % D];
-        if ((x & kExp) == kExp) {
-          atomicMin(&odd[(x & 0x7fff) != kExp ? 0 : x >> 15 ? 2 : 1][i % D], j0 + i / D);
-          vs[i / D][i % D] = 0;
+      tc::tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; q++) tc::tmem_ld32(s_at + 32 * q, r[q]);
+      tc::tmem_ld_wait();
+      const bool masked = (j + 1) * kKeys > first;
+      const int seen = lim - j * kKeys;  // columns of this block that the row sees
+      if (masked) {
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (32 * q + e >= seen) r[q][e] = 0xff800000u;
+      }
+      float top[4];
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        top[q] = __uint_as_float(r[q][0]);
+#pragma unroll
+        for (int e = 1; e < 32; e++) top[q] = max_nan(top[q], __uint_as_float(r[q][e]));
+      }
+      const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+      const bool grow = !(__fmul_rn(__fsub_rn(high, m), c) <= kGrow);  // or is NaN
+      if (i == 0) {
+        m = high;
+      } else if (__any_sync(0xffffffffu, grow)) {
+        // PV of the block before is done: S of this one was issued after it
+        const float nm = max_nan(m, high);
+        const float f = nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
+        m = nm;
+        const f2 ff = pair(f, f);
+        l0 = fma2(l0, ff, 0);
+        l1 = fma2(l1, ff, 0);
+#pragma unroll 1
+        for (int q = 0; q < D / 32; q++) {
+          uint32_t o[32];
+          tc::tmem_ld32(o_at + 32 * q, o);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
+          tmem_st32(o_at + 32 * q, o);
         }
       }
-      __syncthreads();
-    }
-    float s[kKeys / 8][4];
+      // a row that sees a score of +inf or NaN is NaN
+      const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
+      const f2 cc = pair(c, c), bb = pair(base, base);
 #pragma unroll
-    for (int nt = 0; nt < kKeys / 8; nt++) {
+      for (int h = 0; h < 2; h++) {
+        uint32_t p[32];
 #pragma unroll
-      for (int k = 0; k < 4; k++) s[nt][k] = 0.0f;
-#pragma unroll
-      for (int k = 0; k < D / 16; k++)
-        mma16816<BF16>(s[nt], qf[k][0], qf[k][1], qf[k][2], qf[k][3],
-                       *(const uint32_t *)&ks[8 * nt + g][16 * k + 2 * t],
-                       *(const uint32_t *)&ks[8 * nt + g][16 * k + 2 * t + 8]);
-    }
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int nt = 0; nt < kKeys / 8; nt++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int j = j0 + 8 * nt + 2 * t + (k & 1);
-        s[nt][k] = j < lim[k >> 1] ? __fmul_rn(s[nt][k], c) : -INFINITY;
-        top[k >> 1] = fmaxf(top[k >> 1], s[nt][k]);
-      }
-    float base[2];
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      const float nm = fmaxf(m[r], top[r]);
-      base[r] = nm == -INFINITY ? 0.0f : nm;
-      const float f = exp2_fast(__fsub_rn(m[r], base[r]));
-      m[r] = nm;
-      l[r] = __fmul_rn(l[r], f);
-#pragma unroll
-      for (int d = 0; d < D / 8; d++) {
-        o[d][2 * r] = __fmul_rn(o[d][2 * r], f);
-        o[d][2 * r + 1] = __fmul_rn(o[d][2 * r + 1], f);
-      }
-    }
-#pragma unroll
-    for (int kk = 0; kk < kKeys / 16; kk++) {
-      uint32_t p[4];
-#pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-          const float x = exp2_fast(__fsub_rn(s[2 * kk + h][2 * r], base[r]));
-          const float y = exp2_fast(__fsub_rn(s[2 * kk + h][2 * r + 1], base[r]));
-          l[r] = __fadd_rn(l[r], __fadd_rn(x, y));
-          p[2 * h + r] = pack2<BF16>(x, y);
+        for (int e = 0; e < 64; e += 2) {
+          const f2 x = fma2(pair(__uint_as_float(r[2 * h + e / 32][e % 32]),
+                                 __uint_as_float(r[2 * h + e / 32][e % 32 + 1])),
+                            cc, bb);
+          float2 y;
+          if (e % kPolyOf < kPoly) {
+            y = exp2_poly(x);
+          } else {
+            const float2 v = split(x);
+            y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+          }
+          if (e % 4) l1 = add2(l1, pair(y.x, y.y));
+          else l0 = add2(l0, pair(y.x, y.y));
+          p[e / 2] = kv::pack2<BF16>(y.x, y.y);
         }
+        if (masked) {
 #pragma unroll
-      for (int d = 0; d < D / 16; d++) {
-        uint32_t f[4];
-        ldsm4t(f, &vs[16 * kk + (lane & 15)][16 * d + 8 * (lane >> 4)]);
-        mma16816<BF16>(o[2 * d], p[0], p[1], p[2], p[3], f[0], f[1]);
-        mma16816<BF16>(o[2 * d + 1], p[0], p[1], p[2], p[3], f[2], f[3]);
+          for (int e = 0; e < 64; e += 2) {
+            if (64 * h + e >= seen) p[e / 2] &= 0xffff0000u;
+            if (64 * h + e + 1 >= seen) p[e / 2] &= 0x0000ffffu;
+          }
+        }
+        tmem_st32(s_at + 32 * h, p);
       }
+      tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_ready[t]);
+    }
+    // ---- output ----
+    if (blocks > 0 && ok) ok = tc::mbar_wait(&o_done[t], 0, kWaitLimit);
+    if (flagged > 0 && ok) ok = tc::mbar_wait(mended, (flagged - 1) & 1, kWaitLimit);
+    ok = __all_sync(0xffffffffu, ok && !*abort_s);
+    if (!ok) *abort_s = 1;
+    tc::tc_fence_after();
+    const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
+    const float2 la = split(l0), lb = split(l1);
+    const float l = __fadd_rn(__fadd_rn(la.x, la.y), __fadd_rn(lb.x, lb.y));
+    const float inv = none ? 0.0f : __fdiv_rn(1.0f, l);
+    uint16_t *to = (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D;
+#pragma unroll 1
+    for (int q = 0; q < D / 32; q++) {
+      uint32_t o[32];
+      if (blocks > 0 && ok) {
+        tc::tmem_ld32(o_at + 32 * q, o);
+        tc::tmem_ld_wait();
+      }
+      float v[32];
+#pragma unroll
+      for (int e = 0; e < 32; e++) {
+        v[e] = none ? 0.0f : __fmul_rn(__uint_as_float(o[e]), inv);
+        if (!ok) v[e] = NAN;  // a wait gave up
+      }
+      if (flagged > 0 && !none) {
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          const int d = 32 * q + e;
+          if (odd[1][d] < lim) v[e] = __fadd_rn(v[e], INFINITY);
+          if (odd[2][d] < lim) v[e] = __fadd_rn(v[e], -INFINITY);
+          if (odd[0][d] < lim) v[e] = NAN;
+        }
+      }
+      if (live) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+          *(uint4 *)(to + 32 * q + e) =
+              make_uint4(kv::pack2<BF16>(v[e], v[e + 1]), kv::pack2<BF16>(v[e + 2], v[e + 3]),
+                         kv::pack2<BF16>(v[e + 4], v[e + 5]), kv::pack2<BF16>(v[e + 6], v[e + 7]));
+      }
+    }
+    if (live && a.lse != nullptr)
+      a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
+          none ? -INFINITY
+               : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(l)), kLn2) : NAN;
+    tc::tc_fence_before();
+  } else if (warp == 8) {
+    if (lane == 0) {
+      // ================= products =================
+      constexpr uint32_t ds = idesc(128, 128, BF16, false), dp = idesc(128, D, BF16, true);
+      const uint32_t q_base = tc::smem_u32(sm + L::kQ), ring = tc::smem_u32(sm + L::kRing);
+      bool ok = true;
+      auto wait = [&](uint64_t *bar, int phase) {
+        if (ok && (!tc::mbar_wait(bar, phase & 1, kWaitLimit) || *abort_s)) {
+          *abort_s = 1;
+          ok = false;
+        }
+        return ok;
+      };
+      auto scores = [&](int t, int seq) {  // S_t = Q_t K^T
+        const uint32_t kb = ring + (seq % kSlots) * L::kTile;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+          const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
+          tc::mma_f16(tmem + 128 * t, tc::sw128_desc(q_base + t * L::kTile + off),
+                      tc::sw128_desc(kb + off), ds, k > 0);
+        }
+        tc::mma_commit(&s_full[t]);
+      };
+      for (int j = n; j >= 0 && ok; j--) {
+        // block j's values (none for j = n), then block j - 1's scores
+        const int sv = 2 * (n - 1 - j) + 1, sk = sv + 1;
+        if (j < n) {
+          if (!wait(&kv_full[sv % kSlots], sv / kSlots)) break;
+          if (j >= it.whole && !wait(mended, n - 1 - j)) break;
+        }
+        bool have_k = false;
+        for (int t = 0; t < 2 && ok; t++) {
+          if (j < it.blocks[t]) {
+            if (!wait(&p_ready[t], it.blocks[t] - 1 - j)) break;
+            tc::tc_fence_after();
+            const uint32_t vb = ring + (sv % kSlots) * L::kTile;
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; k++)
+              mma_ts(tmem + L::kO + 128 * t, tmem + 128 * t + 8 * k,
+                     sw128_desc_n(vb + k * 16 * 128, 128 * 128), dp,
+                     k > 0 || j < it.blocks[t] - 1);
+            if (j == 0) tc::mma_commit(&o_done[t]);
+          }
+          if (j > 0 && j - 1 < it.blocks[t]) {
+            if (!have_k && !wait(&kv_full[sk % kSlots], sk / kSlots)) break;
+            have_k = true;
+            if (j == it.blocks[t] && !wait(&q_full[t], 0)) break;
+            tc::tc_fence_after();
+            scores(t, sk);
+          }
+        }
+        if (!ok) break;
+        if (j < n) tc::mma_commit(&kv_empty[sv % kSlots]);
+        if (j > 0) tc::mma_commit(&kv_empty[sk % kSlots]);
+      }
+      // every product done before the TMEM goes
+      tc::mma_commit(drained);
+      tc::mbar_wait(drained, 0, kWaitLimit);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0) {
+      // ================= loads =================
+      for (int t = 0; t < 2; t++) {
+        if (it.blocks[t] == 0) continue;
+        tc::mbar_arrive_expect_tx(&q_full[t], L::kTile);
+        for (int x = 0; x < D; x += 64)
+          tma_load_3d(sm + L::kQ + t * L::kTile + x * 256, &qmap, x, it.head[t], it.q0 + it.i0[t],
+                      &q_full[t]);
+      }
+      int64_t issued = 0;
+      for (int seq = 0; seq < 2 * n; seq++, issued++) {
+        const int s = seq % kSlots, j = n - 1 - seq / 2;
+        if (!tc::mbar_wait(&kv_empty[s], (seq / kSlots & 1) ^ 1, kWaitLimit) || *abort_s) {
+          *abort_s = 1;
+          break;
+        }
+        tc::mbar_arrive_expect_tx(&kv_full[s], L::kTile);
+        for (int x = 0; x < D; x += 64)
+          tma_load_3d(sm + L::kRing + s * L::kTile + x * 256, seq & 1 ? &vmap : &kmap, x, kv_head,
+                      it.k0 + j * kKeys, &kv_full[s]);
+      }
+      if (*abort_s) {  // no copy may land after the block is gone
+        tc::drain_stages(kv_full, kSlots, issued, kWaitLimit);
+        for (int t = 0; t < 2; t++)
+          if (it.blocks[t] > 0) tc::mbar_wait(&q_full[t], 0, kWaitLimit);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ================= mending values =================
+    const int id = tid - 320;
+    for (int f = 0; f < flagged; f++) {
+      const int seq = 2 * f + 1, j = n - 1 - f;
+      const bool ok = tc::mbar_wait(&kv_full[seq % kSlots], seq / kSlots, kWaitLimit) && !*abort_s;
+      if (!__all_sync(0xffffffffu, ok)) {
+        *abort_s = 1;
+        break;
+      }
+      uint8_t *v = sm + L::kRing + (seq % kSlots) * L::kTile;
+      constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
+      for (int i = id; i < 128 * (D / 8); i += 64) {
+        const int r = i / (D / 8), ch = i % (D / 8), key = j * kKeys + r;
+        uint4 *at = (uint4 *)(v + tc::sw128_chunk_offset(r, ch, 128));
+        uint4 x = *at;
+        if (key >= it.nk) {
+          *at = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t bad = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t e = ~w[k] & kExp;  // a half's exponent bits all set: none left here
+          bad |= (uint32_t)((e & 0xffffu) == 0) | (uint32_t)((e >> 16) == 0);
+        }
+        if (bad) {
+          for (int k = 0; k < 8; k++) {
+            const uint32_t half = w[k / 2] >> (16 * (k & 1)) & 0xffffu;
+            if ((~half & (kExp & 0xffffu)) != 0) continue;
+            const int kind = (half & 0x7fffu) != (kExp & 0xffffu) ? 0 : half >> 15 ? 2 : 1;
+            atomicMin(&odd[kind][8 * ch + k], key);
+            w[k / 2] &= k & 1 ? 0x0000ffffu : 0xffff0000u;
+          }
+          *at = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      tc::fence_async_smem();
+      tc::mbar_arrive(mended);
     }
   }
   __syncthreads();
-  auto extra = [&](int r, int d) {
-    float x = odd[1][d] < lim[r] ? INFINITY : 0.0f;
-    if (odd[2][d] < lim[r]) x = __fadd_rn(x, -INFINITY);
-    return odd[0][d] < lim[r] ? NAN : x;
-  };
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    l[r] = __fadd_rn(l[r], __shfl_xor_sync(0xffffffffu, l[r], 1));
-    l[r] = __fadd_rn(l[r], __shfl_xor_sync(0xffffffffu, l[r], 2));
-    if (row[r] >= nq) continue;
-    const bool none = m[r] == -INFINITY;
-    const float inv = none ? 0.0f : __fdiv_rn(1.0f, l[r]);
-    uint16_t *to = (uint16_t *)a.out + ((int64_t)(q0 + row[r]) * a.q_heads + head) * D;
-#pragma unroll
-    for (int d = 0; d < D / 8; d++)
-      *(uint32_t *)(to + 8 * d + 2 * t) =
-          none ? 0u
-               : pack2<BF16>(__fmaf_rn(o[d][2 * r], inv, extra(r, 8 * d + 2 * t)),
-                             __fmaf_rn(o[d][2 * r + 1], inv, extra(r, 8 * d + 2 * t + 1)));
-    if (a.lse != nullptr && t == 0)
-      a.lse[(int64_t)(q0 + row[r]) * a.q_heads + head] =
-          none ? -INFINITY : __fmul_rn(__fadd_rn(m[r], __log2f(l[r])), kLn2);
+  if (warp == 8) {
+    tc::tc_fence_after();
+    tc::tmem_relinquish();
+    tc::tmem_dealloc(tmem, 512);
   }
 }
 
-cudaError_t launch(const Args &a, int sms, cudaStream_t st) {
-  (void)sms;
-  const dim3 grid((unsigned)(a.rows_q / kRows + a.n), (unsigned)a.q_heads);
-  if (a.D == 64)
-    (a.bf16 ? simple_kernel<64, true> : simple_kernel<64, false>)<<<grid, kThreads, 0, st>>>(a);
-  else
-    (a.bf16 ? simple_kernel<128, true> : simple_kernel<128, false>)<<<grid, kThreads, 0, st>>>(a);
+// ---- launch ----
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                                 const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeTiled)p;
+  }();
+  return fn;
+}
+
+// 128 rows of 64 columns of one head at a time
+static bool tile_map(CUtensorMap *m, const kv::Strided &x, int rows, int heads, int D, bool bf16) {
+  const cuuint64_t dim[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t stride[2] = {(cuuint64_t)x.head * 2, (cuuint64_t)x.row * 2};
+  const cuuint32_t box[3] = {64, 1, 128}, one[3] = {1, 1, 1};
+  return encoder()(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                   const_cast<void *>(x.p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16>
+static cudaError_t launch_d(const Args &a, cudaStream_t st) {
+  if (encoder() == nullptr) return cudaErrorNotSupported;
+  CUtensorMap q, k, v;
+  if (!tile_map(&q, a.q, a.rows_q, a.q_heads, D, BF16)) return cudaErrorInvalidValue;
+  if (a.rows_k == 0) {
+    k = v = q;  // never read
+  } else if (!tile_map(&k, a.k, a.rows_k, a.heads, D, BF16) ||
+             !tile_map(&v, a.v, a.rows_k, a.heads, D, BF16)) {
+    return cudaErrorInvalidValue;
+  }
+  const bool twins = (a.q_heads / a.heads) % 2 == 0;
+  const int64_t grid = twins ? ((int64_t)a.rows_q / kRows + a.n) * (a.q_heads / 2)
+                             : ((int64_t)a.rows_q / (2 * kRows) + a.n) * a.q_heads;
+  if (grid > INT_MAX) return cudaErrorInvalidValue;
+  const cudaError_t e = cudaFuncSetAttribute(
+      prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kBytes);
+  if (e != cudaSuccess) return e;
+  prompt_kernel<D, BF16><<<(unsigned)grid, kThreads, Shape<D>::kBytes, st>>>(a, q, k, v);
   return cudaGetLastError();
+}
+
+cudaError_t launch(const Args &a, cudaStream_t st) {
+  if (a.D == 64) return a.bf16 ? launch_d<64, true>(a, st) : launch_d<64, false>(a, st);
+  return a.bf16 ? launch_d<128, true>(a, st) : launch_d<128, false>(a, st);
 }
 
 }  // namespace prompt

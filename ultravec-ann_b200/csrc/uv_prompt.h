@@ -15,7 +15,7 @@ struct Args {
   void *out;   // rows_q x q_heads x D, dense
   float *lse;  // rows_q x q_heads, or null
 };
-cudaError_t launch(const Args &a, int sms, cudaStream_t st);
+cudaError_t launch(const Args &a, cudaStream_t st);
 
 }  // namespace prompt
 }  // namespace uvb
