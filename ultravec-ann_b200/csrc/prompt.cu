@@ -39,7 +39,8 @@
 namespace uvb {
 namespace prompt {
 
-constexpr int kRows = 128, kKeys = 128, kThreads = 384, kSlots = 5;
+constexpr int kRows = 128, kKeys = 128, kSlots = 4;
+constexpr int kSoftmaxWarps = 16, kThreads = 32 * (kSoftmaxWarps + 4);
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^f on [-1/2, 1/2], relative error below 2.7e-6: a least-squares fit of the relative
@@ -114,27 +115,48 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, i
       "l"((uint64_t)map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-// D += A B with A in TMEM (row i in lane i, K pairs low half first).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// D += A B, issued by the lane whose `leader` is set: A in TMEM (row i in lane
+// i, K pairs low half first), or both in shared memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       bool accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          tc::smem_u32(bar)),
+      "r"(leader)
       : "memory");
 }
 // Descriptor of a B operand whose N index is contiguous (values as they lie:
@@ -229,6 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t *tmem_s = (uint32_t *)(drained + 1);
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
 
+  __shared__ float row_max[2][2][2][kRows];  // [turn][tile][half][row]
+
   Item it;
   if (!find_item(a, &it)) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -238,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&q_full[i], 1);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_ready[i], 4);
+      tc::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
       tc::mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < kSlots; i++) {
@@ -251,18 +275,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::mbar_fence_init();
   }
   for (int i = tid; i < 3 * D; i += kThreads) odd[i / D][i % D] = INT_MAX;
-  if (warp == 8) tc::tmem_alloc(tmem_s, 512);
+  if (warp == kSoftmaxWarps) tc::tmem_alloc(tmem_s, 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_s;
   const int n = it.n, flagged = max(0, n - it.whole);
 
-  if (warp < 8) {
-    // ================= softmax: thread = row =================
-    const int t = warp >> 2, row = it.i0[t] + (warp & 3) * 32 + lane;
+  // Registers: 16 warps x 32 x 112 + 4 x 32 x 32 = 61440 = 640 x 96, what the
+  // block was launched with.
+  if (warp < kSoftmaxWarps) {
+    // ================= softmax: two threads a row =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    const int t = warp >> 3, half = warp >> 2 & 1, local = (warp & 3) * 32 + lane;
+    const int row = it.i0[t] + local, pair_id = 1 + 4 * t + (warp & 3);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
+    const uint32_t s_at = tmem + lanes + 128 * t + 64 * half;
+    const uint32_t o_at = tmem + lanes + L::kO + 128 * t + D / 2 * half;
     const int blocks = it.blocks[t], lim = limit(a, it, row);
     const int first = limit(a, it, it.i0[t]);
     const float c = __fmul_rn(a.scale, kLog2e);
@@ -270,34 +299,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     f2 l0 = 0, l1 = 0;
     bool ok = true;
     for (int j = blocks - 1, i = 0; j >= 0; j--, i++) {
-      ok = ok && tc::mbar_wait(&s_full[t], i & 1, kWaitLimit) && !*abort_s;
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        *abort_s = 1;
-        break;
-      }
+      // a warp that gives up goes on without work: its partner waits for it
+      if (ok) ok = tc::mbar_wait(&s_full[t], i & 1, kWaitLimit) && !*abort_s;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) *abort_s = 1;
       tc::tc_fence_after();
-      uint32_t r[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; q++) tc::tmem_ld32(s_at + 32 * q, r[q]);
-      tc::tmem_ld_wait();
+      uint32_t r[2][32];
+      if (ok) {
+        tc::tmem_ld32(s_at, r[0]);
+        tc::tmem_ld32(s_at + 32, r[1]);
+        tc::tmem_ld_wait();
+      }
       const bool masked = (j + 1) * kKeys > first;
-      const int seen = lim - j * kKeys;  // columns of this block that the row sees
+      const int seen = lim - j * kKeys - 64 * half;  // of this thread's columns, those the row sees
       if (masked) {
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (32 * q + e >= seen) r[q][e] = 0xff800000u;
+        for (int e = 0; e < 64; e++)
+          if (e >= seen) r[e / 32][e % 32] = 0xff800000u;
       }
       float top[4];
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        top[q] = __uint_as_float(r[q][0]);
+        top[q] = __uint_as_float(r[q / 2][16 * (q % 2)]);
 #pragma unroll
-        for (int e = 1; e < 32; e++) top[q] = max_nan(top[q], __uint_as_float(r[q][e]));
+        for (int e = 1; e < 16; e++)
+          top[q] = max_nan(top[q], __uint_as_float(r[q / 2][16 * (q % 2) + e]));
       }
-      const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+      float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+      // the row's other half; the buffers alternate, so one barrier is enough
+      row_max[i & 1][t][half][local] = high;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_id) : "memory");
+      high = max_nan(high, row_max[i & 1][t][half ^ 1][local]);
       const bool grow = !(__fmul_rn(__fsub_rn(high, m), c) <= kGrow);  // or is NaN
       if (i == 0) {
         m = high;
@@ -309,14 +341,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const f2 ff = pair(f, f);
         l0 = fma2(l0, ff, 0);
         l1 = fma2(l1, ff, 0);
+        if (ok) {
 #pragma unroll 1
-        for (int q = 0; q < D / 32; q++) {
-          uint32_t o[32];
-          tc::tmem_ld32(o_at + 32 * q, o);
-          tc::tmem_ld_wait();
+          for (int q = 0; q < D / 32; q++) {
+            uint32_t o[16];
+            tc::tmem_ld16(o_at + 16 * q, o);
+            tc::tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
-          tmem_st32(o_at + 32 * q, o);
+            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
+            tmem_st16(o_at + 16 * q, o);
+          }
         }
       }
       // a row that sees a score of +inf or NaN is NaN
@@ -324,12 +358,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const f2 cc = pair(c, c), bb = pair(base, base);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        uint32_t p[32];
+        uint32_t p[16];
 #pragma unroll
-        for (int e = 0; e < 64; e += 2) {
-          const f2 x = fma2(pair(__uint_as_float(r[2 * h + e / 32][e % 32]),
-                                 __uint_as_float(r[2 * h + e / 32][e % 32 + 1])),
-                            cc, bb);
+        for (int e = 0; e < 32; e += 2) {
+          const f2 x = fma2(pair(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), cc, bb);
           float2 y;
           if (e % kPolyOf < kPoly) {
             y = exp2_poly(x);
@@ -343,31 +375,36 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            if (64 * h + e >= seen) p[e / 2] &= 0xffff0000u;
-            if (64 * h + e + 1 >= seen) p[e / 2] &= 0x0000ffffu;
+          for (int e = 0; e < 32; e += 2) {
+            if (32 * h + e >= seen) p[e / 2] &= 0xffff0000u;
+            if (32 * h + e + 1 >= seen) p[e / 2] &= 0x0000ffffu;
           }
         }
-        tmem_st32(s_at + 32 * h, p);
+        if (ok) tmem_st16(s_at + 16 * h, p);
       }
       tmem_st_wait();
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_ready[t]);
     }
-    // ---- output ----
+    // ---- output: each thread half of its row's columns ----
+    const float2 la = split(l0), lb = split(l1);
+    float l = __fadd_rn(__fadd_rn(la.x, la.y), __fadd_rn(lb.x, lb.y));
+    row_max[blocks & 1][t][half][local] = l;
+    asm volatile("bar.sync %0, 64;" ::"r"(pair_id) : "memory");
+    const float other = row_max[blocks & 1][t][half ^ 1][local];
+    l = half ? __fadd_rn(other, l) : __fadd_rn(l, other);
     if (blocks > 0 && ok) ok = tc::mbar_wait(&o_done[t], 0, kWaitLimit);
     if (flagged > 0 && ok) ok = tc::mbar_wait(mended, (flagged - 1) & 1, kWaitLimit);
     ok = __all_sync(0xffffffffu, ok && !*abort_s);
     if (!ok) *abort_s = 1;
     tc::tc_fence_after();
     const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
-    const float2 la = split(l0), lb = split(l1);
-    const float l = __fadd_rn(__fadd_rn(la.x, la.y), __fadd_rn(lb.x, lb.y));
     const float inv = none ? 0.0f : __fdiv_rn(1.0f, l);
-    uint16_t *to = (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D;
+    uint16_t *to =
+        (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D + D / 2 * half;
 #pragma unroll 1
-    for (int q = 0; q < D / 32; q++) {
+    for (int q = 0; q < D / 64; q++) {
       uint32_t o[32];
       if (blocks > 0 && ok) {
         tc::tmem_ld32(o_at + 32 * q, o);
@@ -382,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (flagged > 0 && !none) {
 #pragma unroll
         for (int e = 0; e < 32; e++) {
-          const int d = 32 * q + e;
+          const int d = D / 2 * half + 32 * q + e;
           if (odd[1][d] < lim) v[e] = __fadd_rn(v[e], INFINITY);
           if (odd[2][d] < lim) v[e] = __fadd_rn(v[e], -INFINITY);
           if (odd[0][d] < lim) v[e] = NAN;
@@ -396,72 +433,84 @@ __global__ void __launch_bounds__(kThreads, 1)
                          kv::pack2<BF16>(v[e + 4], v[e + 5]), kv::pack2<BF16>(v[e + 6], v[e + 7]));
       }
     }
-    if (live && a.lse != nullptr)
+    if (live && half == 0 && a.lse != nullptr)
       a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
           none ? -INFINITY
                : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(l)), kLn2) : NAN;
     tc::tc_fence_before();
-  } else if (warp == 8) {
-    if (lane == 0) {
-      // ================= products =================
-      constexpr uint32_t ds = idesc(128, 128, BF16, false), dp = idesc(128, D, BF16, true);
-      const uint32_t q_base = tc::smem_u32(sm + L::kQ), ring = tc::smem_u32(sm + L::kRing);
-      bool ok = true;
-      auto wait = [&](uint64_t *bar, int phase) {
-        if (ok && (!tc::mbar_wait(bar, phase & 1, kWaitLimit) || *abort_s)) {
-          *abort_s = 1;
-          ok = false;
-        }
-        return ok;
-      };
-      auto scores = [&](int t, int seq) {  // S_t = Q_t K^T
-        const uint32_t kb = ring + (seq % kSlots) * L::kTile;
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
-          tc::mma_f16(tmem + 128 * t, tc::sw128_desc(q_base + t * L::kTile + off),
-                      tc::sw128_desc(kb + off), ds, k > 0);
-        }
-        tc::mma_commit(&s_full[t]);
-      };
-      for (int j = n; j >= 0 && ok; j--) {
-        // block j's values (none for j = n), then block j - 1's scores
-        const int sv = 2 * (n - 1 - j) + 1, sk = sv + 1;
-        if (j < n) {
-          if (!wait(&kv_full[sv % kSlots], sv / kSlots)) break;
-          if (j >= it.whole && !wait(mended, n - 1 - j)) break;
-        }
-        bool have_k = false;
-        for (int t = 0; t < 2 && ok; t++) {
-          if (j < it.blocks[t]) {
-            if (!wait(&p_ready[t], it.blocks[t] - 1 - j)) break;
-            tc::tc_fence_after();
-            const uint32_t vb = ring + (sv % kSlots) * L::kTile;
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; k++)
-              mma_ts(tmem + L::kO + 128 * t, tmem + 128 * t + 8 * k,
-                     sw128_desc_n(vb + k * 16 * 128, 128 * 128), dp,
-                     k > 0 || j < it.blocks[t] - 1);
-            if (j == 0) tc::mma_commit(&o_done[t]);
-          }
-          if (j > 0 && j - 1 < it.blocks[t]) {
-            if (!have_k && !wait(&kv_full[sk % kSlots], sk / kSlots)) break;
-            have_k = true;
-            if (j == it.blocks[t] && !wait(&q_full[t], 0)) break;
-            tc::tc_fence_after();
-            scores(t, sk);
-          }
-        }
-        if (!ok) break;
-        if (j < n) tc::mma_commit(&kv_empty[sv % kSlots]);
-        if (j > 0) tc::mma_commit(&kv_empty[sk % kSlots]);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+  }
+  if (warp == kSoftmaxWarps) {
+    // ================= products =================
+    // The whole warp runs this on values that are the same in every lane, so
+    // that addresses and descriptors stay in uniform registers; one lane issues.
+    // (Run by one lane alone, the operands' way into uniform registers took
+    // 70 to 160 cycles a product, and the tensor core idled for it.)
+    constexpr uint32_t ds = idesc(128, 128, BF16, false), dp = idesc(128, D, BF16, true);
+    const uint32_t leader = elect_one();
+    const uint32_t tm = uniform(tmem), q_base = uniform(tc::smem_u32(sm + L::kQ));
+    const uint64_t q_desc = tc::sw128_desc(q_base), k_desc = tc::sw128_desc(q_base + L::kRing);
+    const uint64_t v_desc = sw128_desc_n(q_base + L::kRing, 128 * 128);
+    const int nu = uniform(n), whole = uniform(it.whole);
+    const int nb[2] = {(int)uniform(it.blocks[0]), (int)uniform(it.blocks[1])};
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, int phase) {
+      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(bar, phase & 1, kWaitLimit));
+      return ok;
+    };
+    // block j's values (none for j = n), then block j - 1's scores
+    int v_slot = 1, v_phase = 0, k_slot = 0, k_phase = 0;
+    for (int j = nu; j >= 0 && ok; j--) {
+      if (j < nu) {
+        if (!wait(&kv_full[v_slot], v_phase)) break;
+        if (j >= whole && !wait(mended, nu - 1 - j)) break;
       }
-      // every product done before the TMEM goes
-      tc::mma_commit(drained);
-      tc::mbar_wait(drained, 0, kWaitLimit);
+      bool have_k = false;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        if (j < nb[t]) {
+          if (!wait(&p_ready[t], nb[t] - 1 - j)) break;
+          tc::tc_fence_after();
+          const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; k++)
+            mma_ts(tm + L::kO + 128 * t, tm + 128 * t + 64 * (k >> 2) + 8 * (k & 3),
+                   vd + (k * 16 * 128 >> 4), dp, k > 0 || j < nb[t] - 1, leader);
+          if (j == 0) mma_commit(&o_done[t], leader);
+        }
+        if (j > 0 && j <= nb[t]) {
+          if (!have_k && !wait(&kv_full[k_slot], k_phase)) break;
+          have_k = true;
+          if (j == nb[t] && !wait(&q_full[t], 0)) break;
+          tc::tc_fence_after();
+          const uint64_t kd = k_desc + (uint64_t)(k_slot * (L::kTile >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; k++) {
+            const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+            mma_ss(tm + 128 * t, q_desc + t * (L::kTile >> 4) + off, kd + off, ds, k > 0, leader);
+          }
+          mma_commit(&s_full[t], leader);
+        }
+      }
+      if (!ok) break;
+      if (j < nu) {
+        mma_commit(&kv_empty[v_slot], leader);
+        v_slot += 2;
+        if (v_slot >= kSlots) v_slot -= kSlots, v_phase ^= 1;
+      }
+      if (j > 0) {
+        mma_commit(&kv_empty[k_slot], leader);
+        k_slot += 2;
+        if (k_slot >= kSlots) k_slot -= kSlots, k_phase ^= 1;
+      }
     }
+    if (!ok) *abort_s = 1;
+    // every product done before the TMEM goes
+    mma_commit(drained, leader);
+    tc::mbar_wait(drained, 0, kWaitLimit);
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kSoftmaxWarps + 1) {
     if (lane == 0) {
       // ================= loads =================
       for (int t = 0; t < 2; t++) {
@@ -490,9 +539,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp > kSoftmaxWarps + 1) {
     // ================= mending values =================
-    const int id = tid - 320;
+    const int id = tid - 32 * (kSoftmaxWarps + 2);
     for (int f = 0; f < flagged; f++) {
       const int seq = 2 * f + 1, j = n - 1 - f;
       const bool ok = tc::mbar_wait(&kv_full[seq % kSlots], seq / kSlots, kWaitLimit) && !*abort_s;
@@ -533,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kSoftmaxWarps) {
     tc::tc_fence_after();
     tc::tmem_relinquish();
     tc::tmem_dealloc(tmem, 512);
