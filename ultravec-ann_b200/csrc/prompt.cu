@@ -39,16 +39,15 @@
 namespace uvb {
 namespace prompt {
 
-constexpr int kRows = 128, kKeys = 128, kSlots = 4;
-constexpr int kSoftmaxWarps = 16, kThreads = 32 * (kSoftmaxWarps + 4);
-constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr int kRows = 128, kKeys = 128, kSlots = 5;
+constexpr int kSoftmaxWarps = 8, kThreads = 32 * (kSoftmaxWarps + 4);
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^f on [-1/2, 1/2], relative error below 2.7e-6: a least-squares fit of the relative
 // error with weights that drive it to its minimax, made for this file
 constexpr float kC0 = 0.9999992847442627f, kC1 = 0.6931217908859253f, kC2 = 0.240247443318367f,
                 kC3 = 0.05591785907745361f, kC4 = 0.009570101276040077f;
 constexpr int kPoly = 2, kPolyOf = 8;  // of kPolyOf columns, kPoly take the polynomial
-constexpr float kGrow = 8.0f;  // log2 of the growth that a maximum may leave unanswered
+constexpr float kGrow = 16384.0f;  // weights (sums of 32 of them) up to this stay unanswered
 
 __device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
 
@@ -87,12 +86,13 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
 }
 
 // 2^x for two x in the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by the
-// polynomial of degree 4, n added to the exponent.  x below -126 gives 2^-126
+// polynomial of degree 4, n added to the exponent.  x above 127 gives 2^127 (the
+// caller takes a new reference then), below -126 2^-126
 // (the caller makes masked weights exact zeros) and so does NaN (the caller's
 // row has NaN from its other columns then).
 __device__ __forceinline__ float2 exp2_poly(f2 x) {
   const float2 v = split(x);
-  x = pair(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  x = pair(fminf(fmaxf(v.x, -126.0f), 127.0f), fminf(fmaxf(v.y, -126.0f), 127.0f));
   const f2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
   const f2 n = add2(x, magic), whole = add2(n, minus);
   const f2 f = fma2(whole, pair(-1.0f, -1.0f), x);
@@ -107,12 +107,40 @@ __device__ __forceinline__ float2 exp2_poly(f2 x) {
 }
 
 // ---- tensor core plumbing beside uv_tc.cuh ----
+// A bounded wait (a second at most) whose polls sleep in hardware until the
+// phase ends: polls that come back at once took two fifths of the issue slots
+// from the warps that had work.
+__device__ __forceinline__ bool wait_for(uint64_t *bar, int phase) {
+  for (int i = 0; i < 1 << 16; i++) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(tc::smem_u32(bar)), "r"((uint32_t)phase & 1u)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z,
                                             uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(tc::smem_u32(dst)),
       "l"((uint64_t)map), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
@@ -246,12 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   int(*odd)[D] = (int(*)[D])(sm + L::kOdd);  // the first key whose value is NaN, +inf, -inf
   uint64_t *bars = (uint64_t *)(sm + L::kBars);
   uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + kSlots;
-  uint64_t *s_full = kv_empty + kSlots, *p_ready = s_full + 2, *o_done = p_ready + 2;
-  uint64_t *mended = o_done + 2, *drained = mended + 1;
+  uint64_t *s_full = kv_empty + kSlots, *p_ready = s_full + 2, *o_done = p_ready + 4;
+  uint64_t *h_done = o_done + 2, *mended = h_done + 2, *drained = mended + 1;
   uint32_t *tmem_s = (uint32_t *)(drained + 1);
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
-
-  __shared__ float row_max[2][2][2][kRows];  // [turn][tile][half][row]
 
   Item it;
   if (!find_item(a, &it)) return;
@@ -262,13 +288,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&q_full[i], 1);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
       tc::mbar_init(&o_done[i], 1);
+      tc::mbar_init(&h_done[i], 1);
     }
     for (int i = 0; i < kSlots; i++) {
       tc::mbar_init(&kv_full[i], 1);
       tc::mbar_init(&kv_empty[i], 1);
     }
+    for (int i = 0; i < 4; i++) tc::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
     tc::mbar_init(mended, 64);
     tc::mbar_init(drained, 1);
     *abort_s = 0;
@@ -282,129 +309,142 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_s;
   const int n = it.n, flagged = max(0, n - it.whole);
 
-  // Registers: 16 warps x 32 x 112 + 4 x 32 x 32 = 61440 = 640 x 96, what the
+  // Registers: 8 warps x 32 x 232 + 4 x 32 x 40 = 64512 = 384 x 168, what the
   // block was launched with.
   if (warp < kSoftmaxWarps) {
-    // ================= softmax: two threads a row =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-    const int t = warp >> 3, half = warp >> 2 & 1, local = (warp & 3) * 32 + lane;
-    const int row = it.i0[t] + local, pair_id = 1 + 4 * t + (warp & 3);
+    // ================= softmax: thread = row =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int t = warp >> 2, row = it.i0[t] + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + 128 * t + 64 * half;
-    const uint32_t o_at = tmem + lanes + L::kO + 128 * t + D / 2 * half;
+    const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
     const int blocks = it.blocks[t], lim = limit(a, it, row);
     const int first = limit(a, it, it.i0[t]);
     const float c = __fmul_rn(a.scale, kLog2e);
     float m = -INFINITY;
-    f2 l0 = 0, l1 = 0;
+    f2 l = 0;
     bool ok = true;
-    for (int j = blocks - 1, i = 0; j >= 0; j--, i++) {
-      // a warp that gives up goes on without work: its partner waits for it
-      if (ok) ok = tc::mbar_wait(&s_full[t], i & 1, kWaitLimit) && !*abort_s;
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) *abort_s = 1;
+    auto settle = [&](bool fine) {  // the warp goes on, or gives up as one
+      ok = __all_sync(0xffffffffu, ok && fine);
+      return ok;
+    };
+    for (int j = blocks - 1, i = 0; j >= 0 && ok; j--, i++) {
+      if (!settle(wait_for(&s_full[t], i))) break;
       tc::tc_fence_after();
-      uint32_t r[2][32];
-      if (ok) {
-        tc::tmem_ld32(s_at, r[0]);
-        tc::tmem_ld32(s_at + 32, r[1]);
-        tc::tmem_ld_wait();
-      }
-      const bool masked = (j + 1) * kKeys > first;
-      const int seen = lim - j * kKeys - 64 * half;  // of this thread's columns, those the row sees
-      if (masked) {
+      uint32_t r[4][32];
 #pragma unroll
-        for (int e = 0; e < 64; e++)
+      for (int q = 0; q < 4; q++) tc::tmem_ld32(s_at + 32 * q, r[q]);
+      tc::tmem_ld_wait();
+      const bool masked = (j + 1) * kKeys > first;
+      const int seen = lim - j * kKeys;  // columns of this block that the row sees
+      if (masked) {
+        asm volatile("");  // a branch, not 128 selects in every block
+#pragma unroll
+        for (int e = 0; e < 128; e++)
           if (e >= seen) r[e / 32][e % 32] = 0xff800000u;
       }
-      float top[4];
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        top[q] = __uint_as_float(r[q / 2][16 * (q % 2)]);
+      for (int h = 0; h < 2; h++) {  // 64 keys
+        f2 sum;
+        uint32_t p[2][16];
+        // a row without a reference needs its maximum first; a row that needs
+        // none keeps its own, whoever shares its warp
+        bool need = m == -INFINITY, again = __any_sync(0xffffffffu, need);
+        for (;;) {
+          if (again) {
+            // (opaque here, so that the maximum is not computed ahead of the branch)
 #pragma unroll
-        for (int e = 1; e < 16; e++)
-          top[q] = max_nan(top[q], __uint_as_float(r[q / 2][16 * (q % 2) + e]));
-      }
-      float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
-      // the row's other half; the buffers alternate, so one barrier is enough
-      row_max[i & 1][t][half][local] = high;
-      asm volatile("bar.sync %0, 64;" ::"r"(pair_id) : "memory");
-      high = max_nan(high, row_max[i & 1][t][half ^ 1][local]);
-      const bool grow = !(__fmul_rn(__fsub_rn(high, m), c) <= kGrow);  // or is NaN
-      if (i == 0) {
-        m = high;
-      } else if (__any_sync(0xffffffffu, grow)) {
-        // PV of the block before is done: S of this one was issued after it
-        const float nm = max_nan(m, high);
-        const float f = nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
-        m = nm;
-        const f2 ff = pair(f, f);
-        l0 = fma2(l0, ff, 0);
-        l1 = fma2(l1, ff, 0);
-        if (ok) {
+            for (int e = 0; e < 64; e++) asm volatile("" : "+r"(r[2 * h + e / 32][e % 32]));
+            float top[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+              const uint32_t *x = &r[2 * h + q / 2][16 * (q % 2)];
+              top[q] = __uint_as_float(x[0]);
+#pragma unroll
+              for (int e = 1; e < 16; e++) top[q] = max_nan(top[q], __uint_as_float(x[e]));
+            }
+            const float nm =
+                max_nan(m, max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])));
+            const float f =
+                !need || nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
+            m = need ? nm : m;
+            l = fma2(l, pair(f, f), 0);
+            if (i > 0 || h > 0) {
+              // O holds what the products before this half have added: those of
+              // the block before are done (S came after them), those of this
+              // block's first half say so
+              if (h > 0 && !settle(wait_for(&h_done[t], i))) break;
+              tc::tc_fence_after();
 #pragma unroll 1
-          for (int q = 0; q < D / 32; q++) {
-            uint32_t o[16];
-            tc::tmem_ld16(o_at + 16 * q, o);
-            tc::tmem_ld_wait();
+              for (int q = 0; q < D / 32; q++) {
+                uint32_t o[32];
+                tc::tmem_ld32(o_at + 32 * q, o);
+                tc::tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
-            tmem_st16(o_at + 16 * q, o);
+                for (int e = 0; e < 32; e++)
+                  o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
+                tmem_st32(o_at + 32 * q, o);
+              }
+            }
           }
-        }
-      }
-      // a row that sees a score of +inf or NaN is NaN
-      const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
-      const f2 cc = pair(c, c), bb = pair(base, base);
+          // a row that sees a score of +inf or NaN is NaN
+          const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
+          const f2 cc = pair(c, c), bb = pair(base, base);
+          f2 b0 = 0, b1 = 0;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        uint32_t p[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const f2 x = fma2(pair(__uint_as_float(r[h][e]), __uint_as_float(r[h][e + 1])), cc, bb);
-          float2 y;
-          if (e % kPolyOf < kPoly) {
-            y = exp2_poly(x);
-          } else {
-            const float2 v = split(x);
-            y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+          for (int e = 0; e < 64; e += 2) {
+            const uint32_t *x = &r[2 * h + e / 32][e % 32];
+            const f2 z = fma2(pair(__uint_as_float(x[0]), __uint_as_float(x[1])), cc, bb);
+            float2 y;
+            if (e % kPolyOf < kPoly) {
+              y = exp2_poly(z);
+            } else {
+              const float2 v = split(z);
+              y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+            }
+            if (e % 4) b1 = add2(b1, pair(y.x, y.y));
+            else b0 = add2(b0, pair(y.x, y.y));
+            p[e / 32][e % 32 / 2] = kv::pack2<BF16>(y.x, y.y);
           }
-          if (e % 4) l1 = add2(l1, pair(y.x, y.y));
-          else l0 = add2(l0, pair(y.x, y.y));
-          p[e / 2] = kv::pack2<BF16>(y.x, y.y);
+          sum = add2(b0, b1);
+          if (again) break;
+          // weights beyond 2^14 (or NaN): take a new reference and start over
+          const float2 v = split(sum);
+          need = !(v.x <= kGrow) || !(v.y <= kGrow);
+          again = __any_sync(0xffffffffu, need);
+          if (!again) break;
         }
+        if (!ok) break;
+        l = add2(l, sum);
         if (masked) {
+          asm volatile("");
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            if (32 * h + e >= seen) p[e / 2] &= 0xffff0000u;
-            if (32 * h + e + 1 >= seen) p[e / 2] &= 0x0000ffffu;
+          for (int e = 0; e < 64; e += 2) {
+            if (64 * h + e >= seen) p[e / 32][e % 32 / 2] &= 0xffff0000u;
+            if (64 * h + e + 1 >= seen) p[e / 32][e % 32 / 2] &= 0x0000ffffu;
           }
         }
-        if (ok) tmem_st16(s_at + 16 * h, p);
+        tmem_st16(s_at + 64 * h, p[0]);
+        tmem_st16(s_at + 64 * h + 16, p[1]);
+        tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&p_ready[2 * t + h]);
       }
-      tmem_st_wait();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&p_ready[t]);
     }
-    // ---- output: each thread half of its row's columns ----
-    const float2 la = split(l0), lb = split(l1);
-    float l = __fadd_rn(__fadd_rn(la.x, la.y), __fadd_rn(lb.x, lb.y));
-    row_max[blocks & 1][t][half][local] = l;
-    asm volatile("bar.sync %0, 64;" ::"r"(pair_id) : "memory");
-    const float other = row_max[blocks & 1][t][half ^ 1][local];
-    l = half ? __fadd_rn(other, l) : __fadd_rn(l, other);
-    if (blocks > 0 && ok) ok = tc::mbar_wait(&o_done[t], 0, kWaitLimit);
-    if (flagged > 0 && ok) ok = tc::mbar_wait(mended, (flagged - 1) & 1, kWaitLimit);
-    ok = __all_sync(0xffffffffu, ok && !*abort_s);
+    if (!ok) *abort_s = 1;
+    // ---- output ----
+    const float2 ll = split(l);
+    const float sum = __fadd_rn(ll.x, ll.y);
+    if (blocks > 0 && ok) settle(wait_for(&o_done[t], 0));
+    if (flagged > 0 && ok) settle(wait_for(mended, flagged - 1));
+    settle(!*abort_s);
     if (!ok) *abort_s = 1;
     tc::tc_fence_after();
     const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
-    const float inv = none ? 0.0f : __fdiv_rn(1.0f, l);
-    uint16_t *to =
-        (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D + D / 2 * half;
+    const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
+    uint16_t *to = (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D;
 #pragma unroll 1
-    for (int q = 0; q < D / 64; q++) {
+    for (int q = 0; q < D / 32; q++) {
       uint32_t o[32];
       if (blocks > 0 && ok) {
         tc::tmem_ld32(o_at + 32 * q, o);
@@ -419,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (flagged > 0 && !none) {
 #pragma unroll
         for (int e = 0; e < 32; e++) {
-          const int d = D / 2 * half + 32 * q + e;
+          const int d = 32 * q + e;
           if (odd[1][d] < lim) v[e] = __fadd_rn(v[e], INFINITY);
           if (odd[2][d] < lim) v[e] = __fadd_rn(v[e], -INFINITY);
           if (odd[0][d] < lim) v[e] = NAN;
@@ -433,13 +473,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                          kv::pack2<BF16>(v[e + 4], v[e + 5]), kv::pack2<BF16>(v[e + 6], v[e + 7]));
       }
     }
-    if (live && half == 0 && a.lse != nullptr)
+    if (live && a.lse != nullptr)
       a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
           none ? -INFINITY
-               : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(l)), kLn2) : NAN;
+               : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
     tc::tc_fence_before();
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   }
   if (warp == kSoftmaxWarps) {
     // ================= products =================
@@ -456,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nb[2] = {(int)uniform(it.blocks[0]), (int)uniform(it.blocks[1])};
     bool ok = true;
     auto wait = [&](uint64_t *bar, int phase) {
-      if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(bar, phase & 1, kWaitLimit));
+      if (ok) ok = __all_sync(0xffffffffu, wait_for(bar, phase));
       return ok;
     };
     // block j's values (none for j = n), then block j - 1's scores
@@ -470,13 +510,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         if (j < nb[t]) {
-          if (!wait(&p_ready[t], nb[t] - 1 - j)) break;
-          tc::tc_fence_after();
           const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; k++)
-            mma_ts(tm + L::kO + 128 * t, tm + 128 * t + 64 * (k >> 2) + 8 * (k & 3),
-                   vd + (k * 16 * 128 >> 4), dp, k > 0 || j < nb[t] - 1, leader);
+          for (int h = 0; h < 2; h++) {
+            if (!wait(&p_ready[2 * t + h], nb[t] - 1 - j)) break;
+            tc::tc_fence_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; k++)
+              mma_ts(tm + L::kO + 128 * t, tm + 128 * t + 64 * h + 8 * (k & 3),
+                     vd + (k * 16 * 128 >> 4), dp, k > 0 || j < nb[t] - 1, leader);
+            if (h == 0) mma_commit(&h_done[t], leader);
+          }
+          if (!ok) break;
           if (j == 0) mma_commit(&o_done[t], leader);
         }
         if (j > 0 && j <= nb[t]) {
@@ -508,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) *abort_s = 1;
     // every product done before the TMEM goes
     mma_commit(drained, leader);
-    tc::mbar_wait(drained, 0, kWaitLimit);
+    wait_for(drained, 0);
     __syncwarp();
   } else if (warp == kSoftmaxWarps + 1) {
     if (lane == 0) {
@@ -523,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int64_t issued = 0;
       for (int seq = 0; seq < 2 * n; seq++, issued++) {
         const int s = seq % kSlots, j = n - 1 - seq / 2;
-        if (!tc::mbar_wait(&kv_empty[s], (seq / kSlots & 1) ^ 1, kWaitLimit) || *abort_s) {
+        if (!wait_for(&kv_empty[s], (seq / kSlots & 1) ^ 1) || *abort_s) {
           *abort_s = 1;
           break;
         }
@@ -533,9 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                       it.k0 + j * kKeys, &kv_full[s]);
       }
       if (*abort_s) {  // no copy may land after the block is gone
-        tc::drain_stages(kv_full, kSlots, issued, kWaitLimit);
+        for (int64_t k = issued > kSlots ? issued - kSlots : 0; k < issued; k++)
+          wait_for(&kv_full[k % kSlots], (int)(k / kSlots));
         for (int t = 0; t < 2; t++)
-          if (it.blocks[t] > 0) tc::mbar_wait(&q_full[t], 0, kWaitLimit);
+          if (it.blocks[t] > 0) wait_for(&q_full[t], 0);
       }
     }
     __syncwarp();
@@ -544,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int id = tid - 32 * (kSoftmaxWarps + 2);
     for (int f = 0; f < flagged; f++) {
       const int seq = 2 * f + 1, j = n - 1 - f;
-      const bool ok = tc::mbar_wait(&kv_full[seq % kSlots], seq / kSlots, kWaitLimit) && !*abort_s;
+      const bool ok = wait_for(&kv_full[seq % kSlots], seq / kSlots) && !*abort_s;
       if (!__all_sync(0xffffffffu, ok)) {
         *abort_s = 1;
         break;
