@@ -37,11 +37,21 @@ namespace kv {
 constexpr int kWarps = 4, kAttendThreads = 32 * kWarps;
 constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kJump = 8.0f;     // log2 of what a score may exceed its reference by
+constexpr float kSpread = 16.0f;  // what a value scale may exceed its reference by
 
-template <int D>
-__host__ __device__ constexpr int stages() {  // 4 warps' rings fit a third of an SM's shared memory
-  return 512 / D;
-}
+// Blocks an SM: three where the sums and the query's fragments leave room in
+// 168 registers, else two with the longer rings that then fit.
+template <int D, int NT, bool BF16>
+struct Fit {
+  static constexpr int kParts = BF16 ? 1 : 2;  // halves that a query value is rounded to
+  static constexpr int kBlocks = D / 4 * NT + D / 8 * NT * kParts <= 64 ? 3 : 2;
+  static constexpr int kStages = kBlocks == 3 ? 512 / D : 768 / D;
+  static constexpr int kTileBytes = kTile * (D + 8);
+  // the warps' rings of tiles; between segments the same bytes join their outputs
+  static constexpr int kRing = kWarps * kStages * kTileBytes, kJoin = 8 * NT * (D + 4) * 4;
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+};
 
 // Scratch: per entry the first tile and the first job, tiles per worker, then
 // one part for every (job + worker): it grows with either, so it is theirs.
@@ -118,20 +128,11 @@ __device__ __forceinline__ Words<D> load_words(const uint8_t *p) {
   return r;
 }
 
-// Shared memory of a block: the warps' rings of tiles; between segments the
-// same bytes join the warps' outputs.
-template <int D, int NT>
-struct AttendSmem {
-  static constexpr int kTileBytes = kTile * (D + 8);
-  static constexpr int kRing = kWarps * stages<D>() * kTileBytes;
-  static constexpr int kJoin = 8 * NT * (D + 4) * 4;
-  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
-};
-
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kAttendThreads, 3)
+__global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     attend_kernel(Cache c, int layer, Rows rows, AttendArgs a, int64_t slots) {
-  constexpr int kCols = 8 * NT, kStages = stages<D>(), kTileBytes = AttendSmem<D, NT>::kTileBytes;
+  using F = Fit<D, NT, BF16>;
+  constexpr int kCols = 8 * NT, kStages = F::kStages, kTileBytes = F::kTileBytes, kParts = F::kParts;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ int64_t sums[2][kWarps];
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
     for (int i = 0; i < min(mine, kStages); i++) issue(i);
 
     // ---- the query columns, rotated, as B fragments ----
-    uint32_t qf[NT][D / 32][4];
+    uint32_t qf[kParts][NT][D / 32][4];
     float cs[NT][2], hs[NT][2];  // of the columns 2t, 2t + 1 of each 8
     int lim[NT][2];
 #pragma unroll
@@ -297,16 +298,24 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
         for (int w = 0; w < D / 32; w++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t h = pack2<false>(__fmul_rn(y[r][8 * w + i], down),
-                                            __fmul_rn(y[r][8 * w + i + 4], down));
-            const float2 f = unpack2<false>(h);
-            sum = __fadd_rn(sum, __fadd_rn(f.x, f.y));
-            qf[nt][w][i] = h;
+            // codes of even i come 16 times smaller out of unpack8
+            const float f = __fmul_rn(down, i % 2 ? 1.0f : 16.0f);
+            float lo = __fmul_rn(y[r][8 * w + i], f), hi = __fmul_rn(y[r][8 * w + i + 4], f);
+#pragma unroll
+            for (int part = 0; part < kParts; part++) {
+              const uint32_t h = pack2<false>(lo, hi);
+              const float2 v = unpack2<false>(h);
+              sum = __fmaf_rn(__fadd_rn(v.x, v.y), i % 2 ? 1.0f : 0.0625f, sum);
+              qf[part][nt][w][i] = h;
+              lo = __fsub_rn(lo, v.x);
+              hi = __fsub_rn(hi, v.y);
+            }
           }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        // levels are codes - 7.5 and the unpacked halves codes - 8
-        const float h = __fmul_rn(0.5f, sum), cc = __fmul_rn(__fmul_rn(a.scale, kLog2e), exp2i(e));
+        // the products give 2^-20 <q, n>, levels are n - 7.5
+        const float h = __fmul_rn(-7.5f * 0x1p-20f, sum);
+        const float cc = __fmul_rn(__fmul_rn(a.scale, kLog2e * 0x1p20f), exp2i(e));
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           hs[nt][k] = __shfl_sync(0xffffffffu, h, 4 * (2 * t + k));
@@ -317,8 +326,10 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
       }
     }
 
-    float o[D / 16][NT][4], half_sum[NT][4], m[NT][2], l[NT][2];
-    int ve[NT][2];  // a column's value scales are divided by 2^ve
+    // o: rows of even dimensions in units of 2^-24, of odd ones 2^-20
+    float o[D / 16][NT][4], codes[NT][4], m[NT][2], l[NT][2];
+    int ve[NT][2];         // a column's value scales are divided by 2^ve
+    float down[NT][2];     // 2^-ve
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -326,12 +337,33 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
 #pragma unroll
         for (int k = 0; k < 4; k++) o[mt][nt][k] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; k++) half_sum[nt][k] = 0.0f;
+      for (int k = 0; k < 4; k++) codes[nt][k] = 0.0f;
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
       ve[nt][0] = ve[nt][1] = -100;
+      down[nt][0] = down[nt][1] = exp2i(100);
     }
 
+    // The codes 0 .. 15 stand for levels of mean zero: taking 7.5 times the
+    // weights' sum (a product with ones) off every four tiles keeps the sums as
+    // small as the levels' own, so that nothing cancels over a long sequence.
+    auto recentre = [&] {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float lo = __fmul_rn(codes[nt][k], 7.5f * 0x1p-24f);
+          const float hi = __fmul_rn(codes[nt][k], 7.5f * 0x1p-20f);
+#pragma unroll
+          for (int mt = 0; mt < D / 16; mt++) {
+            o[mt][nt][k] = __fsub_rn(o[mt][nt][k], lo);
+            o[mt][nt][2 + k] = __fsub_rn(o[mt][nt][2 + k], hi);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) codes[nt][k] = 0.0f;
+      }
+    };
     // ---- one pass over the warp's tiles ----
     for (int i = 0; i < mine; i++) {
       const int slot = taken % kStages;
@@ -366,8 +398,10 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
           for (int k = 0; k < 4; k += 2)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-              mma16816<false>(s[sb][nt], xa[k], xb[k], xa[k + 1], xb[k + 1], qf[nt][w][k],
-                              qf[nt][w][k + 1]);
+#pragma unroll
+              for (int part = 0; part < kParts; part++)
+                mma16816<false>(s[sb][nt], xa[k], xb[k], xa[k + 1], xb[k + 1],
+                                qf[part][nt][w][k], qf[part][nt][w][k + 1]);
         }
       }
       float ks[2][2], vs[2][2];
@@ -381,60 +415,82 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
           ks[sb][r] = kscale[16 * sb + 8 * r + g];
           vs[sb][r] = vscale[16 * sb + 8 * r + g];
         }
-      // A column's largest score and largest finite value scale here, over the
-      // tokens that it sees: what it does not see must not move its references.
+      // Scores against the running maximum, in place.  Where every column sees
+      // every token there is nothing to mask; elsewhere a token that a column
+      // does not see neither weighs nor moves that column's references.
       auto seen = [&](int nt, int k, int sb, int r) {
-        return whole || key0 + 16 * sb + 8 * r + g < lim[nt][k];
+        return key0 + 16 * sb + 8 * r + g < lim[nt][k];
       };
-      auto value_top = [&](int nt, int k) {
-        float v = 0.0f;
-#pragma unroll
-        for (int sb = 0; sb < 2; sb++)
-#pragma unroll
-          for (int r = 0; r < 2; r++)
-            if (seen(nt, k, sb, r) && vs[sb][r] <= FLT_MAX) v = fmaxf(v, vs[sb][r]);
-        return v;
-      };
-      const float vall = value_top(0, 0);
       bool jump = false;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          float top = -INFINITY;
+          const float base = m[nt][k] == -INFINITY ? 0.0f : -m[nt][k];
 #pragma unroll
           for (int sb = 0; sb < 2; sb++)
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-              float &v = s[sb][nt][2 * r + k];
-              v = __fmul_rn(v, __fmul_rn(cs[nt][k], ks[sb][r]));
-              if (!seen(nt, k, sb, r)) v = -INFINITY;
-              top = fmaxf(top, v);
-            }
-          jump |= top > m[nt][k] + 8.0f;
-          jump |= (whole ? vall : value_top(nt, k)) > exp2i(min(ve[nt][k] + 4, 127));
+            for (int r = 0; r < 2; r++)
+              s[sb][nt][2 * r + k] =
+                  __fmaf_rn(s[sb][nt][2 * r + k], __fmul_rn(cs[nt][k], ks[sb][r]), base);
         }
+      if (whole) {
+        const float vtop = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float top = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k]));
+            jump |= top > kJump || m[nt][k] == -INFINITY || !(__fmul_rn(vtop, down[nt][k]) <= kSpread);
+          }
+      } else {
+        jump = true;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+              for (int r = 0; r < 2; r++)
+                if (!seen(nt, k, sb, r)) s[sb][nt][2 * r + k] = -INFINITY;
+      }
       if (__any_sync(0xffffffffu, jump)) {
+        // new references, for the columns that need them
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             float top = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k]));
-            float vtop = value_top(nt, k);
+            float vtop = 0.0f;
+#pragma unroll
+            for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+              for (int r = 0; r < 2; r++)
+                if ((whole || seen(nt, k, sb, r)) && vs[sb][r] <= FLT_MAX) vtop = fmaxf(vtop, vs[sb][r]);
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) {
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
               vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
             }
-            const float nm = fmaxf(m[nt][k], top);
-            const int ne = max(ve[nt][k], min(log2i(vtop), 126));
-            const float f = nm == -INFINITY ? 1.0f : exp2_fast(__fsub_rn(m[nt][k], nm));
+            const bool none = m[nt][k] == -INFINITY;
+            const float up = none ? top : top > kJump ? top : 0.0f;  // what m grows by
+            const int ne = __fmul_rn(vtop, down[nt][k]) > kSpread ? min(log2i(vtop), 126) : ve[nt][k];
+            // (a column that has seen nothing has sums of zero: any factor keeps them)
+            const float f = none ? 1.0f : exp2_fast(-up);
             const float both = __fmul_rn(f, exp2_fast((float)(ve[nt][k] - ne)));
-            m[nt][k] = nm;
+            if (none) m[nt][k] = top;
+            else m[nt][k] = __fadd_rn(m[nt][k], up);
             ve[nt][k] = ne;
+            down[nt][k] = exp2i(-ne);
+            if (up != -INFINITY)
+#pragma unroll
+              for (int sb = 0; sb < 2; sb++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) s[sb][nt][2 * r + k] = __fsub_rn(s[sb][nt][2 * r + k], up);
             l[nt][k] = __fmul_rn(l[nt][k], f);
-            half_sum[nt][k] = __fmul_rn(half_sum[nt][k], both);
-            half_sum[nt][2 + k] = __fmul_rn(half_sum[nt][2 + k], both);
+            codes[nt][k] = __fmul_rn(codes[nt][k], both);
+            codes[nt][2 + k] = __fmul_rn(codes[nt][2 + k], both);
 #pragma unroll
             for (int mt = 0; mt < D / 16; mt++) {
               o[mt][nt][k] = __fmul_rn(o[mt][nt][k], both);
@@ -449,19 +505,22 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
         for (int nt = 0; nt < NT; nt++) {
           float w[4];
 #pragma unroll
-          for (int k = 0; k < 2; k++) {
-            const float base = m[nt][k] == -INFINITY ? 0.0f : m[nt][k], down = exp2i(-ve[nt][k]);
+          for (int k = 0; k < 2; k++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-              const float e = exp2_fast(__fsub_rn(s[sb][nt][2 * r + k], base));
+              const float e = exp2_fast(s[sb][nt][2 * r + k]);
               l[nt][k] = __fadd_rn(l[nt][k], e);
-              // a token that is not seen weighs nothing even if its scale is no number
-              w[2 * r + k] = seen(nt, k, sb, r) ? __fmul_rn(e, __fmul_rn(vs[sb][r], down)) : 0.0f;
+              w[2 * r + k] = __fmul_rn(e, __fmul_rn(vs[sb][r], down[nt][k]));
             }
-          }
+          if (!whole)  // a token that is not seen weighs nothing even if its scale is no number
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int r = 0; r < 2; r++)
+                if (!seen(nt, k, sb, r)) w[2 * r + k] = 0.0f;
 #pragma unroll
           for (int r = 0; r < 2; r++) p[nt][r] = transpose8x8(pack2<false>(w[2 * r], w[2 * r + 1]));
-          mma16816<false>(half_sum[nt], 0x38003800u, 0x38003800u, 0x38003800u, 0x38003800u, p[nt][0],
+          mma16816<false>(codes[nt], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, p[nt][0],
                           p[nt][1]);
         }
         const uint8_t *pairp = tile + kTile * (D / 2 + 4) + (8 * sb + t) * D + g * (D / 8);
@@ -479,6 +538,7 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
                               p[nt][0], p[nt][1]);
         }
       }
+      if ((i & 3) == 3) recentre();
       __syncwarp();  // every lane has read the slot
       const int next = i + kStages;
       if (next < mine) {
@@ -487,6 +547,7 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
       }
     }
 
+    recentre();
     // ---- join the warps' parts ----
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
@@ -515,6 +576,7 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
             const float f = m[nt][k] == -INFINITY
                                 ? 0.0f
                                 : __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
+            const float flo = __fmul_rn(f, 0x1p24f), fhi = __fmul_rn(f, 0x1p20f);
 #pragma unroll
             for (int mt = 0; mt < D / 16; mt++) {
               float2 *at = (float2 *)(out + col * kRow + g * (D / 8) + 2 * mt);
@@ -522,10 +584,10 @@ __global__ void __launch_bounds__(kAttendThreads, 3)
               // a warp without a visible token adds nothing, whatever its sums hold
               const float u = m[nt][k] == -INFINITY
                                   ? 0.0f
-                                  : __fmul_rn(__fadd_rn(o[mt][nt][k], half_sum[nt][k]), f);
+                                  : __fmul_rn(o[mt][nt][k], flo);
               const float v = m[nt][k] == -INFINITY
                                   ? 0.0f
-                                  : __fmul_rn(__fadd_rn(o[mt][nt][2 + k], half_sum[nt][k]), f);
+                                  : __fmul_rn(o[mt][nt][2 + k], fhi);
               *at = make_float2(__fadd_rn(was.x, u), __fadd_rn(was.y, v));
             }
           }
@@ -645,8 +707,8 @@ __global__ void __launch_bounds__(256) join_kernel(Cache c, Rows rows, AttendArg
 
 // ---- launches ----
 // Columns of a tile: the fewest eights that hold a sequence's usual columns,
-// so that one row of a group of 8 does not pay for 16; more columns than 16
-// (32 at D = 64) would not leave registers for three blocks an SM.
+// so that one row of a group of 8 does not pay for 16; what is above the
+// largest would not fit in registers.
 static int column_eights(int D, int64_t cols) {
   if (D == 256 || cols <= 8) return 1;
   if (D == 128 || cols <= 16) return 2;
@@ -658,8 +720,8 @@ AttendPlan attend_plan(const Cache &c, int n, int rows, int most, int q_heads, i
   const int group = q_heads / c.heads;
   p.cols = 8 * column_eights(c.head_dim, (int64_t)group * most);
   p.jobs = ((int64_t)rows * group / p.cols + n) * c.heads;
-  p.workers = 3 * sms;
-  const int64_t slots = p.jobs + p.workers;
+  p.sms = sms;
+  const int64_t slots = p.jobs + 3 * sms;
   p.bytes = head_bytes(n) + slots * p.cols * (c.head_dim + 2) * 4;
   return p;
 }
@@ -667,13 +729,14 @@ AttendPlan attend_plan(const Cache &c, int n, int rows, int most, int q_heads, i
 template <int D, int NT, bool BF16>
 static cudaError_t attend_nt(const Cache &c, int layer, const Rows &rows, const AttendArgs &a,
                              const AttendPlan &plan, cudaStream_t st) {
-  const int64_t slots = plan.jobs + plan.workers;
-  const int smem = AttendSmem<D, NT>::kBytes;
-  static const cudaError_t set = cudaFuncSetAttribute(
-      attend_kernel<D, NT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (set != cudaSuccess) return set;
-  attend_kernel<D, NT, BF16><<<plan.workers, kAttendThreads, smem, st>>>(c, layer, rows, a, slots);
-  const cudaError_t e = cudaGetLastError();
+  const int64_t slots = plan.jobs + 3 * plan.sms;
+  using F = Fit<D, NT, BF16>;
+  const int smem = F::kBytes, workers = F::kBlocks * plan.sms;
+  cudaError_t e = cudaFuncSetAttribute(attend_kernel<D, NT, BF16>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  attend_kernel<D, NT, BF16><<<workers, kAttendThreads, smem, st>>>(c, layer, rows, a, slots);
+  e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

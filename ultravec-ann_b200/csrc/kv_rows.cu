@@ -236,12 +236,9 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(Cache c, int layer, R
 #pragma unroll
     for (int i = 0; i < D / 32; i++) {
       uint32_t o[4];
-      unpack8(w[r][i], o);
+      unpack8_levels(w[r][i], o);
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const __half2 h = __hadd2(*reinterpret_cast<__half2 *>(&o[k]), __float2half2_rn(0.5f));
-        a[r][4 * i + k] = *reinterpret_cast<const uint32_t *>(&h);
-      }
+      for (int k = 0; k < 4; k++) a[r][4 * i + k] = o[k];
     }
   hadamard_mma<D, false>(y, a, Hadamard::make<false>());
   hadamard_rest<D>(y);

@@ -141,21 +141,31 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// 8 nibbles of a word as 4 half2 of n - 8: out[i] = (nibble i, nibble i + 4).
-// 0x6400 | n is the half 1024 + n, 0x6400 | 16 n is 1024 + 16 n.
+// 8 nibbles of a word as 4 half2 of codes n, pair i = (nibble i, nibble i + 4):
+// the bits as they stand are subnormal halves, n 2^-24 for i = 0, 2 and
+// n 2^-20 for i = 1, 3, which the matrix instructions take exactly.
 __device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&out)[4]) {
+  const uint32_t u = w >> 8;
+  out[0] = w & 0x000f000fu;
+  out[1] = w & 0x00f000f0u;
+  out[2] = u & 0x000f000fu;
+  out[3] = u & 0x00f000f0u;
+}
+// The same as levels n - 7.5 (0x6400 | n is the half 1024 + n, 0x6400 | 16 n is
+// 1024 + 16 n).
+__device__ __forceinline__ void unpack8_levels(uint32_t w, uint32_t (&out)[4]) {
   constexpr uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, one = 0x64006400u;
   const uint32_t u = w >> 8;
-  uint32_t r0, r1, r2, r3;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r0) : "r"(w), "r"(lo), "r"(one));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r1) : "r"(w), "r"(hi), "r"(one));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r2) : "r"(u), "r"(lo), "r"(one));
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r3) : "r"(u), "r"(hi), "r"(one));
-  constexpr uint32_t m1032 = 0xe408e408u, m72 = 0xd480d480u, sixteenth = 0x2c002c00u;
-  asm("add.f16x2 %0, %1, %2;" : "=r"(out[0]) : "r"(r0), "r"(m1032));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[1]) : "r"(r1), "r"(sixteenth), "r"(m72));
-  asm("add.f16x2 %0, %1, %2;" : "=r"(out[2]) : "r"(r2), "r"(m1032));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[3]) : "r"(r3), "r"(sixteenth), "r"(m72));
+  uint32_t r[4] = {(w & lo) | one, (w & hi) | one, (u & lo) | one, (u & hi) | one};
+  constexpr uint32_t m1032 = 0xe408e408u, m715 = 0xd478d478u, sixteenth = 0x2c002c00u,
+                     half = 0x38003800u;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    uint32_t x;
+    asm("add.f16x2 %0, %1, %2;" : "=r"(x) : "r"(r[i]), "r"(m1032));
+    asm("add.f16x2 %0, %1, %2;" : "=r"(out[i]) : "r"(x), "r"(half));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[i + 1]) : "r"(r[i + 1]), "r"(sixteenth), "r"(m715));
+  }
 }
 
 // ---- the Hadamard transform of 16 rows by one warp ----

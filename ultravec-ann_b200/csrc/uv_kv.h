@@ -33,7 +33,7 @@ cudaError_t read_launch(const Cache &c, int layer, const Rows &rows, void *k, vo
 struct AttendPlan {
   int cols = 0;          // (token, head of the group) pairs a block holds
   int64_t jobs = 0;      // upper bound on (sequence, column tile, head)
-  int workers = 0;       // blocks
+  int sms = 0;
   int64_t bytes = 0;     // scratch
 };
 AttendPlan attend_plan(const Cache &c, int n, int rows, int most, int q_heads, int sms);
