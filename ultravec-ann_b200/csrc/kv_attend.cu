@@ -46,17 +46,17 @@ template <int D, int NT, bool BF16>
 struct Fit {
   static constexpr int kParts = BF16 ? 1 : 2;  // halves that a query value is rounded to
   static constexpr int kBlocks = D / 4 * NT + D / 8 * NT * kParts <= 64 ? 3 : 2;
-  static constexpr int kStages = kBlocks == 3 ? 512 / D : 768 / D;
+  static constexpr int kStages = kBlocks == 3 ? 384 / D : D == 256 ? 2 : 640 / D;
   static constexpr int kTileBytes = kTile * (D + 8);
-  // the warps' rings of tiles; between segments the same bytes join their outputs
-  static constexpr int kRing = kWarps * kStages * kTileBytes, kJoin = 8 * NT * (D + 4) * 4;
-  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kRing = kWarps * kStages * kTileBytes;  // the warps' rings of tiles
+  static constexpr int kRow = D + 4, kJoin = 2 * 8 * NT * kRow * 4;  // two warps' outputs
+  static constexpr int kBytes = kRing + kJoin;
 };
 
-// Scratch: per entry the first tile and the first job, tiles per worker, then
+// Scratch: per entry the first unit and the first job, units per block, then
 // one part for every (job + worker): it grows with either, so it is theirs.
 struct Parts {
-  int64_t *head;  // [0] tiles per worker; first tiles from [1], first jobs from [n + 2]
+  int64_t *head;  // [0] units per block; first units from [1], first jobs from [n + 2]
   float *o;       // slots x columns x D
   float2 *ml;     // slots x columns: maximum (log2) and sum
 };
@@ -68,8 +68,14 @@ __device__ __forceinline__ Parts carve(void *p, int n, int64_t slots, int cols, 
   return {(int64_t *)p, o, (float2 *)(o + slots * cols * D)};
 }
 
+// What a job costs beside its tiles (its queries, the join of its parts), in
+// tiles: the pieces of the line are equal in time, not in tiles.  Measured on
+// 64 sequences of 1k to 20k tokens: 0 116 us, 8 JOBCOST.
+constexpr int kJobCost = 8;
+
 struct Job {
   int seq, first, n, len, tiles, col_tiles;
+  __device__ int64_t units() const { return tiles == 0 ? 0 : tiles + kJobCost; }
 };
 __device__ __forceinline__ Job load_entry(const Cache &c, const Rows &r, int b, int group,
                                           int cols) {
@@ -150,21 +156,21 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   // ---- this block's piece of the line of tiles ----
   const int per_thread = (rows.n + kAttendThreads - 1) / kAttendThreads;
   const int e0 = min(tid * per_thread, rows.n), e1 = min(e0 + per_thread, rows.n);
-  int64_t my_tiles = 0, my_jobs = 0;
+  int64_t my_units = 0, my_jobs = 0;
   for (int b = e0; b < e1; b++) {
     const Job j = load_entry(c, rows, b, group, kCols);
     const int64_t jobs = (int64_t)j.col_tiles * c.heads;
     my_jobs += jobs;
-    my_tiles += jobs * j.tiles;
+    my_units += jobs * j.units();
   }
-  int64_t x = my_tiles, y = my_jobs;
+  int64_t x = my_units, y = my_jobs;
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
     if (lane >= o) x += u, y += v;
   }
   if (lane == 31) sums[0][warp] = x, sums[1][warp] = y;
   __syncthreads();
-  int64_t total = 0, before_t = x - my_tiles, before_j = y - my_jobs;
+  int64_t total = 0, before_t = x - my_units, before_j = y - my_jobs;
   for (int w = 0; w < kWarps; w++) {
     total += sums[0][w];
     if (w < warp) before_t += sums[0][w], before_j += sums[1][w];
@@ -179,7 +185,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       sc.head[1 + b] = bt;
       sc.head[2 + rows.n + b] = bj;
       bj += (int64_t)j.col_tiles * c.heads;
-      bt += (int64_t)j.col_tiles * c.heads * j.tiles;
+      bt += (int64_t)j.col_tiles * c.heads * j.units();
     }
     if (e0 < rows.n && e1 == rows.n) {
       sc.head[1 + rows.n] = bt;
@@ -189,18 +195,18 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   }
   pdl_launch();
   if (T0 >= T1) return;
-  if (T0 >= before_t && T0 < before_t + my_tiles) {
+  if (T0 >= before_t && T0 < before_t + my_units) {
     int64_t bt = before_t, bj = before_j;
     for (int b = e0; b < e1; b++) {
       const Job j = load_entry(c, rows, b, group, kCols);
       const int64_t jobs = (int64_t)j.col_tiles * c.heads;
-      if (T0 < bt + jobs * j.tiles) {
+      if (T0 < bt + jobs * j.units()) {
         begin[0] = b;
         begin[1] = bt;
         begin[2] = bj;
         break;
       }
-      bt += jobs * j.tiles;
+      bt += jobs * j.units();
       bj += jobs;
     }
   }
@@ -213,49 +219,73 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   uint32_t issued = 0, taken = 0;  // tiles of this warp's ring
   bool dead = false;
 
-  for (int64_t T = T0; T < T1;) {
-    while (T >= base_t + (int64_t)job.col_tiles * c.heads * job.tiles) {
-      base_t += (int64_t)job.col_tiles * c.heads * job.tiles;
-      base_j += (int64_t)job.col_tiles * c.heads;
-      entry++;
-      job = load_entry(c, rows, entry, group, kCols);
+  // A segment: the part of a job that lies in this block's piece.
+  struct Segment {
+    Job job;
+    int64_t slot;
+    int j0, todo, mine, c0, head;  // tiles j0 .. j0 + todo, every fourth this warp's
+  };
+  int64_t T = T0;
+  auto next = [&](Segment *seg) {
+    while (T < T1) {
+      while (T >= base_t + (int64_t)job.col_tiles * c.heads * job.units()) {
+        base_t += (int64_t)job.col_tiles * c.heads * job.units();
+        base_j += (int64_t)job.col_tiles * c.heads;
+        entry++;
+        job = load_entry(c, rows, entry, group, kCols);
+      }
+      const int64_t local = T - base_t, units = job.units(), jl = local / units;
+      const int off = (int)(local % units);
+      const int take = (int)min(units - off, T1 - T);
+      T += take;
+      const int j0 = max(0, off - kJobCost), j1 = max(0, off + take - kJobCost);
+      if (j0 == j1) continue;
+      const int ct = (int)(jl / c.heads);
+      seg->job = job;
+      seg->slot = base_j + jl + blockIdx.x;
+      seg->head = (int)(jl % c.heads);
+      seg->c0 = ct * kCols;
+      seg->j0 = j0;
+      // tiles that the last of the columns sees something of
+      const int lim = job.len - job.n + min((seg->c0 + kCols - 1) / group, job.n - 1) + 1;
+      seg->todo = max(0, min(j1, (lim + kTile - 1) / kTile) - j0);
+      seg->mine = seg->todo > warp ? (seg->todo - warp + kWarps - 1) / kWarps : 0;
+      return true;
     }
-    const int64_t local = T - base_t;
-    const int64_t jl = local / job.tiles;
-    const int j0 = (int)(local % job.tiles);
-    const int nj = (int)min((int64_t)(job.tiles - j0), T1 - T);
-    const int ct = (int)(jl / c.heads), head = (int)(jl % c.heads);
-    T += nj;
+    return false;
+  };
+  const int per_page = c.page_tokens / kTile;
+  const uint8_t *src = nullptr;
+  auto lookup = [&](const Segment &seg, int from) {  // this warp's tiles from .. from + 31, one a lane
+    const int i = from + lane;
+    if (i < seg.mine) {
+      const int j = seg.j0 + warp + i * kWarps;
+      src = c.tile_at(layer, c.page_at(seg.job.seq, j / per_page), seg.head, j % per_page);
+    }
+  };
+  auto issue = [&](int i) {
+    const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)src, i & 31);
+    if (lane == 0 && !dead) {
+      const int slot = issued % kStages;
+      tc::mbar_arrive_expect_tx(&full[warp][slot], kTileBytes);
+      bulk_load(ring + slot * kTileBytes, p, kTileBytes, &full[warp][slot]);
+    }
+    issued++;
+  };
+  auto start = [&](const Segment &seg) {
+    lookup(seg, 0);
+    for (int i = 0; i < min(seg.mine, kStages); i++) issue(i);
+  };
 
-    const int ncol = job.n * group, c0 = ct * kCols;
-    const int offset = job.len - job.n;  // position of the entry's first row
+  Segment seg, after;
+  bool more = next(&seg);
+  if (more) start(seg);
+  while (more) {
+    const Job &at = seg.job;
+    const int ncol = at.n * group, c0 = seg.c0, head = seg.head, mine = seg.mine;
+    const int offset = at.len - at.n;  // position of the entry's first row
     // the exclusive ends of what the tile's first and last rows may see
     const int lim_first = offset + c0 / group + 1;
-    const int lim_last = offset + min((c0 + kCols - 1) / group, job.n - 1) + 1;
-    const int todo = max(0, min(nj, (lim_last + kTile - 1) / kTile - j0));
-    const int mine = todo > warp ? (todo - warp + kWarps - 1) / kWarps : 0;
-
-    // ---- start the ring ----
-    const int per_page = c.page_tokens / kTile;
-    const uint8_t *src = nullptr;
-    auto lookup = [&](int from) {  // tiles from .. from + 31 of this warp, one a lane
-      const int i = from + lane;
-      if (i < mine) {
-        const int j = j0 + warp + i * kWarps;
-        src = c.tile_at(layer, c.page_at(job.seq, j / per_page), head, j % per_page);
-      }
-    };
-    auto issue = [&](int i) {
-      const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)src, i & 31);
-      if (lane == 0 && !dead) {
-        const int slot = issued % kStages;
-        tc::mbar_arrive_expect_tx(&full[warp][slot], kTileBytes);
-        bulk_load(ring + slot * kTileBytes, p, kTileBytes, &full[warp][slot]);
-      }
-      issued++;
-    };
-    lookup(0);
-    for (int i = 0; i < min(mine, kStages); i++) issue(i);
 
     // ---- the query columns, rotated, as B fragments ----
     uint32_t qf[kParts][NT][D / 32][4];
@@ -268,7 +298,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       for (int r = 0; r < 2; r++) {
         const int col = c0 + 16 * half + 8 * r + g;
         const bool live = (2 * half + r < NT) && col < ncol;
-        const int row = job.first + (live ? col / group : 0), hq = head * group + (live ? col % group : 0);
+        const int row = at.first + (live ? col / group : 0), hq = head * group + (live ? col % group : 0);
         const uint4 *q = (const uint4 *)((const uint16_t *)a.q.p + (int64_t)row * a.q.row +
                                          (int64_t)hq * a.q.head + t * (D / 4));
 #pragma unroll
@@ -321,7 +351,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
           hs[nt][k] = __shfl_sync(0xffffffffu, h, 4 * (2 * t + k));
           cs[nt][k] = __shfl_sync(0xffffffffu, cc, 4 * (2 * t + k));
           const int col = c0 + 8 * nt + 2 * t + k;
-          lim[nt][k] = offset + min(col / group, job.n - 1) + 1;
+          lim[nt][k] = offset + min(col / group, at.n - 1) + 1;
         }
       }
     }
@@ -378,7 +408,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       if (dead) break;
       taken++;
       const uint8_t *tile = ring + slot * kTileBytes;
-      const int key0 = (j0 + warp + i * kWarps) * kTile;
+      const int key0 = (seg.j0 + warp + i * kWarps) * kTile;
 
       float s[2][NT][4];
 #pragma unroll
@@ -540,15 +570,19 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       }
       if ((i & 3) == 3) recentre();
       __syncwarp();  // every lane has read the slot
-      const int next = i + kStages;
-      if (next < mine) {
-        if ((next & 31) == 0) lookup(next);
-        issue(next);
+      const int ahead = i + kStages;
+      if (ahead < mine) {
+        if ((ahead & 31) == 0) lookup(seg, ahead);
+        issue(ahead);
       }
     }
 
     recentre();
-    // ---- join the warps' parts ----
+    // the next segment's tiles are on their way while this one's parts join
+    more = next(&after);
+    if (more) start(after);
+
+    // ---- join the warps' parts: 2 and 3 leave theirs, 0 and 1 add to them ----
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -561,11 +595,12 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
           join_l[warp][8 * nt + 2 * t + k] = l[nt][k];
         }
       }
-    __syncthreads();  // also: every ring is empty, its bytes are the join's
-    float *out = (float *)smem;
-    constexpr int kRow = D + 4;
-    for (int w = 0; w < kWarps; w++) {
-      if (w == warp) {
+    __syncthreads();
+    constexpr int kRow = F::kRow;
+    float *out = (float *)(smem + F::kRing), *mine_out = out + (warp & 1) * kCols * kRow;
+#pragma unroll
+    for (int step = 0; step < 2; step++) {
+      if (warp / 2 != step) {  // first 2 and 3
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -573,33 +608,30 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
             const int col = 8 * nt + 2 * t + k;
             float top = join_m[0][col];
             for (int v = 1; v < kWarps; v++) top = fmaxf(top, join_m[v][col]);
-            const float f = m[nt][k] == -INFINITY
-                                ? 0.0f
-                                : __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
+            // a warp without a visible token adds nothing, whatever its sums hold
+            const bool none = m[nt][k] == -INFINITY;
+            const float f = __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
             const float flo = __fmul_rn(f, 0x1p24f), fhi = __fmul_rn(f, 0x1p20f);
 #pragma unroll
             for (int mt = 0; mt < D / 16; mt++) {
-              float2 *at = (float2 *)(out + col * kRow + g * (D / 8) + 2 * mt);
-              const float2 was = w == 0 ? make_float2(0.0f, 0.0f) : *at;
-              // a warp without a visible token adds nothing, whatever its sums hold
-              const float u = m[nt][k] == -INFINITY
-                                  ? 0.0f
-                                  : __fmul_rn(o[mt][nt][k], flo);
-              const float v = m[nt][k] == -INFINITY
-                                  ? 0.0f
-                                  : __fmul_rn(o[mt][nt][2 + k], fhi);
-              *at = make_float2(__fadd_rn(was.x, u), __fadd_rn(was.y, v));
+              float2 *to = (float2 *)(mine_out + col * kRow + g * (D / 8) + 2 * mt);
+              const float2 was = step == 0 ? make_float2(0.0f, 0.0f) : *to;
+              const float u = none ? 0.0f : __fmul_rn(o[mt][nt][k], flo);
+              const float v = none ? 0.0f : __fmul_rn(o[mt][nt][2 + k], fhi);
+              *to = make_float2(__fadd_rn(was.x, u), __fadd_rn(was.y, v));
             }
           }
       }
       __syncthreads();
     }
     // (starts that do not rise give more jobs than rows allow: no slot, no part)
-    const int64_t slot = base_j + jl + blockIdx.x;
-    const bool fits = slot < slots;
+    const bool fits = seg.slot < slots;
     for (int i = fits ? tid : kCols * D; i < kCols * (D / 4); i += kAttendThreads) {
       const int col = i / (D / 4), d4 = i % (D / 4);
-      ((float4 *)(sc.o + (slot * kCols + col) * D))[d4] = *(const float4 *)(out + col * kRow + 4 * d4);
+      const float4 u = *(const float4 *)(out + col * kRow + 4 * d4);
+      const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4);
+      ((float4 *)(sc.o + (seg.slot * kCols + col) * D))[d4] =
+          make_float4(__fadd_rn(u.x, v.x), __fadd_rn(u.y, v.y), __fadd_rn(u.z, v.z), __fadd_rn(u.w, v.w));
     }
     if (fits && tid < kCols) {
       float top = join_m[0][tid], sum = 0.0f;
@@ -607,10 +639,10 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       for (int v = 0; v < kWarps; v++)
         if (join_m[v][tid] != -INFINITY)
           sum = __fmaf_rn(join_l[v][tid], exp2_fast(__fsub_rn(join_m[v][tid], top)), sum);
-      sc.ml[slot * kCols + tid] = make_float2(top, sum);
+      sc.ml[seg.slot * kCols + tid] = make_float2(top, sum);
     }
-    tc::fence_async_smem();  // the next bulk copies write where this joined
-    __syncthreads();
+    __syncthreads();  // the join's bytes are free again
+    seg = after;
   }
 }
 
@@ -623,7 +655,7 @@ __global__ void __launch_bounds__(256) join_kernel(Cache c, Rows rows, AttendArg
   const int group = a.q_heads / c.heads;
   const Parts sc = carve(a.scratch, rows.n, slots, kCols, D);
   pdl_wait();
-  const int64_t *tiles = sc.head + 1, *jobs = sc.head + 2 + rows.n;
+  const int64_t *units = sc.head + 1, *jobs = sc.head + 2 + rows.n;
   const int64_t J = blockIdx.x, per = sc.head[0];
   if (J >= jobs[rows.n]) return;
   int lo = 0, hi = rows.n - 1;  // the last entry whose first job is <= J
@@ -634,9 +666,10 @@ __global__ void __launch_bounds__(256) join_kernel(Cache c, Rows rows, AttendArg
   }
   const int b = lo;
   const int64_t jl = J - jobs[b], nj = jobs[b + 1] - jobs[b];
-  const int64_t n_tiles = (tiles[b + 1] - tiles[b]) / nj, first = tiles[b] + jl * n_tiles;
+  const int64_t n_units = (units[b + 1] - units[b]) / nj;
+  const int64_t first = units[b] + jl * n_units + kJobCost, last = units[b] + (jl + 1) * n_units - 1;
   const int64_t w0 = first / per;
-  const int parts = n_tiles == 0 ? 0 : (int)((first + n_tiles - 1) / per - w0) + 1;
+  const int parts = n_units == 0 ? 0 : (int)(last / per - w0) + 1;
   const int ct = (int)(jl / c.heads), head = (int)(jl % c.heads);
   const int ncol = rows.count(b) * group, row0 = rows.first(b);
 
