@@ -20,12 +20,14 @@ int on_device(const void *p, int device, const char *what) {
 
 // bits 0, 2, 4, .. of x in the low half, 1, 3, 5, .. in the high half
 uint32_t split_pairs(uint32_t x) {
-  uint32_t lo = 0, hi = 0;
-  for (int j = 0; j < 16; j++) {
-    lo |= (x >> (2 * j) & 1u) << j;
-    hi |= (x >> (2 * j + 1) & 1u) << j;
-  }
-  return lo | hi << 16;
+  auto even = [](uint32_t v) {
+    v &= 0x55555555u;
+    v = (v | v >> 1) & 0x33333333u;
+    v = (v | v >> 2) & 0x0f0f0f0fu;
+    v = (v | v >> 4) & 0x00ff00ffu;
+    return (v | v >> 8) & 0xffffu;
+  };
+  return even(x) | even(x >> 1) << 16;
 }
 
 int sizes(const uv_kv *kv) {
@@ -301,6 +303,10 @@ int uv_kv_attend(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int3
   a.lse = lse;
   a.q_heads = q_heads;
   a.scale = scale;
+  // Numbers that scratch memory does not hold by chance: mixed, never 0.
+  static std::atomic<uint64_t> calls{0};
+  uint64_t seed = calls.fetch_add(1) ^ 0x6b76617474656e64ull;
+  a.call = splitmix64(&seed) | 1;
   const kv::AttendPlan plan =
       kv::attend_plan(c, n, rows, starts == nullptr ? 1 : most, q_heads, sm_count(kv->device));
   if (plan.jobs > INT32_MAX) return fail(UV_EINVAL, "too many rows for one call");

@@ -16,8 +16,8 @@
 // one line, cut into equal pieces, one for each block of a single wave,
 // whatever the lengths are: the host need not know them.  A piece may hold the
 // end of a job, whole jobs and the start of another; each part leaves its
-// maximum, sum and unnormalised output in scratch, and a second kernel joins a
-// job's parts in order, rotates back and rounds.
+// maximum, sum and unnormalised output in scratch, and the block that finds all
+// of a job's parts written joins them in order, rotates back and rounds.
 //
 // Numbers: q is rotated in f32 and rounded once to a half, after a power of
 // two that brings its row to size 1 (2^-11 relative, below the 4-bit keys'
@@ -53,25 +53,34 @@ struct Fit {
   static constexpr int kBytes = kRing + kJoin;
 };
 
-// Scratch: per entry the first unit and the first job, units per block, then
-// one part for every (job + worker): it grows with either, so it is theirs.
+// Scratch: one part for every (job + block): the sum grows with either along the
+// line, so a part is one block's share of one job.  A part's flag holds the
+// call's number once the part is written.
 struct Parts {
-  int64_t *head;  // [0] units per block; first units from [1], first jobs from [n + 2]
-  float *o;       // slots x columns x D
-  float2 *ml;     // slots x columns: maximum (log2) and sum
+  unsigned long long *flag;  // slots
+  float *o;                  // slots x columns x D
+  float2 *ml;                // slots x columns: maximum (log2) and sum
 };
-__host__ __device__ __forceinline__ int64_t head_bytes(int n) {
-  return ((2 * (int64_t)n + 4) * 8 + 127) & ~127ll;
+__host__ __device__ __forceinline__ int64_t flag_bytes(int64_t slots) {
+  return (slots * 8 + 127) & ~127ll;
 }
-__device__ __forceinline__ Parts carve(void *p, int n, int64_t slots, int cols, int D) {
-  float *o = (float *)((char *)p + head_bytes(n));
-  return {(int64_t *)p, o, (float2 *)(o + slots * cols * D)};
+__device__ __forceinline__ Parts carve(void *p, int64_t slots, int cols, int D) {
+  float *o = (float *)((char *)p + flag_bytes(slots));
+  return {(unsigned long long *)p, o, (float2 *)(o + slots * cols * D)};
+}
+__device__ __forceinline__ void set_flag(unsigned long long *p, unsigned long long v) {
+  asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned long long get_flag(const unsigned long long *p) {
+  unsigned long long v;
+  asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // What a job costs beside its tiles (its queries, the join of its parts), in
 // tiles: the pieces of the line are equal in time, not in tiles.  Measured on
 // 64 sequences of 1k to 20k tokens: 0 116 us, 8 JOBCOST.
-constexpr int kJobCost = 8;
+constexpr int kJobCost = 20;
 
 struct Job {
   int seq, first, n, len, tiles, col_tiles;
@@ -144,10 +153,11 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   __shared__ int64_t sums[2][kWarps];
   __shared__ int64_t begin[3];  // first entry of the piece, its first tile, its first job
   __shared__ float join_m[kWarps][kCols], join_l[kWarps][kCols];
+  __shared__ bool complete;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int group = a.q_heads / c.heads;
-  const Parts sc = carve(a.scratch, rows.n, slots, kCols, D);
+  const Parts sc = carve(a.scratch, slots, kCols, D);
 
   if (lane == 0)
     for (int i = 0; i < kStages; i++) tc::mbar_init(&full[warp][i], 1);
@@ -178,22 +188,17 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   // at least one tile for every warp of a block
   const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kWarps);
   const int64_t T0 = per * blockIdx.x, T1 = min(T0 + per, total);
-  if (blockIdx.x == 0) {  // for the join
-    int64_t bt = before_t, bj = before_j;
-    for (int b = e0; b < e1; b++) {
-      const Job j = load_entry(c, rows, b, group, kCols);
-      sc.head[1 + b] = bt;
-      sc.head[2 + rows.n + b] = bj;
-      bj += (int64_t)j.col_tiles * c.heads;
-      bt += (int64_t)j.col_tiles * c.heads * j.units();
-    }
-    if (e0 < rows.n && e1 == rows.n) {
-      sc.head[1 + rows.n] = bt;
-      sc.head[2 + 2 * rows.n] = bj;
-    }
-    if (tid == 0) sc.head[0] = per;
+  // rows of sequences without a token
+  for (int b = blockIdx.x; b < rows.n; b += gridDim.x) {
+    const Job j = load_entry(c, rows, b, group, kCols);
+    if (j.tiles != 0) continue;
+    uint4 *to = (uint4 *)((uint16_t *)a.out + (int64_t)j.first * a.q_heads * D);
+    for (int64_t i = tid; i < (int64_t)j.n * a.q_heads * (D / 8); i += kAttendThreads)
+      to[i] = make_uint4(0, 0, 0, 0);
+    if (a.lse != nullptr)
+      for (int64_t i = tid; i < (int64_t)j.n * a.q_heads; i += kAttendThreads)
+        a.lse[(int64_t)j.first * a.q_heads + i] = -INFINITY;
   }
-  pdl_launch();
   if (T0 >= T1) return;
   if (T0 >= before_t && T0 < before_t + my_units) {
     int64_t bt = before_t, bj = before_j;
@@ -222,7 +227,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   // A segment: the part of a job that lies in this block's piece.
   struct Segment {
     Job job;
-    int64_t slot;
+    int64_t number;           // of the job
+    int first_block, blocks;  // that have a part of it
     int j0, todo, mine, c0, head;  // tiles j0 .. j0 + todo, every fourth this warp's
   };
   int64_t T = T0;
@@ -242,7 +248,10 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       if (j0 == j1) continue;
       const int ct = (int)(jl / c.heads);
       seg->job = job;
-      seg->slot = base_j + jl + blockIdx.x;
+      const int64_t start = base_t + jl * units;
+      seg->number = base_j + jl;
+      seg->first_block = (int)((start + kJobCost) / per);
+      seg->blocks = (int)((start + units - 1) / per) - seg->first_block + 1;
       seg->head = (int)(jl % c.heads);
       seg->c0 = ct * kCols;
       seg->j0 = j0;
@@ -624,117 +633,139 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       }
       __syncthreads();
     }
+    // ---- the job's result, or this block's part of it ----
     // (starts that do not rise give more jobs than rows allow: no slot, no part)
-    const bool fits = seg.slot < slots;
-    for (int i = fits ? tid : kCols * D; i < kCols * (D / 4); i += kAttendThreads) {
-      const int col = i / (D / 4), d4 = i % (D / 4);
-      const float4 u = *(const float4 *)(out + col * kRow + 4 * d4);
-      const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4);
-      ((float4 *)(sc.o + (seg.slot * kCols + col) * D))[d4] =
-          make_float4(__fadd_rn(u.x, v.x), __fadd_rn(u.y, v.y), __fadd_rn(u.z, v.z), __fadd_rn(u.w, v.w));
-    }
-    if (fits && tid < kCols) {
-      float top = join_m[0][tid], sum = 0.0f;
-      for (int v = 1; v < kWarps; v++) top = fmaxf(top, join_m[v][tid]);
+    const int64_t slot = seg.number + blockIdx.x;
+    const bool fits = seg.number + seg.first_block + seg.blocks <= slots;
+    bool final = seg.blocks == 1 && fits;
+    auto total_of = [&](int col, float *top) {
+      float sum = 0.0f;
+      *top = join_m[0][col];
+      for (int v = 1; v < kWarps; v++) *top = fmaxf(*top, join_m[v][col]);
       for (int v = 0; v < kWarps; v++)
-        if (join_m[v][tid] != -INFINITY)
-          sum = __fmaf_rn(join_l[v][tid], exp2_fast(__fsub_rn(join_m[v][tid], top)), sum);
-      sc.ml[seg.slot * kCols + tid] = make_float2(top, sum);
+        if (join_m[v][col] != -INFINITY)
+          sum = __fmaf_rn(join_l[v][col], exp2_fast(__fsub_rn(join_m[v][col], *top)), sum);
+      return sum;
+    };
+    auto write_lse = [&](int col, float top, float sum) {
+      const int x = c0 + col;
+      if (a.lse != nullptr && x < ncol)
+        a.lse[(int64_t)(at.first + x / group) * a.q_heads + head * group + x % group] =
+            top == -INFINITY ? -INFINITY : __fmul_rn(__fadd_rn(top, __log2f(sum)), kLn2);
+    };
+    if (seg.blocks == 1) {
+      for (int i = tid; i < kCols * (D / 4); i += kAttendThreads) {
+        const int col = i / (D / 4), d4 = i % (D / 4);
+        float4 *u = (float4 *)(out + col * kRow + 4 * d4);
+        const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4), w = *u;
+        float top;
+        const float sum = total_of(col, &top);
+        const float inv = top == -INFINITY ? 0.0f : __fdiv_rn(1.0f, sum);
+        *u = make_float4(__fmul_rn(__fadd_rn(w.x, v.x), inv), __fmul_rn(__fadd_rn(w.y, v.y), inv),
+                         __fmul_rn(__fadd_rn(w.z, v.z), inv), __fmul_rn(__fadd_rn(w.w, v.w), inv));
+        if (d4 == 0 && fits) write_lse(col, top, sum);
+      }
+      __syncthreads();
+    } else if (fits) {
+      for (int i = tid; i < kCols * (D / 4); i += kAttendThreads) {
+        const int col = i / (D / 4), d4 = i % (D / 4);
+        const float4 u = *(const float4 *)(out + col * kRow + 4 * d4);
+        const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4);
+        __stcg((float4 *)(sc.o + (slot * kCols + col) * D) + d4,
+               make_float4(__fadd_rn(u.x, v.x), __fadd_rn(u.y, v.y), __fadd_rn(u.z, v.z),
+                           __fadd_rn(u.w, v.w)));
+      }
+      if (tid < kCols) {
+        float top;
+        const float sum = total_of(tid, &top);
+        __stcg(&sc.ml[slot * kCols + tid], make_float2(top, sum));
+      }
+      __syncthreads();
+      if (tid == 0) set_flag(&sc.flag[slot], a.call);
+      // Whoever finds every part written joins them, in their order.  The block
+      // that finishes last does; two that finish together may both, and write
+      // the same bytes.  Nothing waits, and no counter has to start at zero.
+      const int64_t first = seg.number + seg.first_block;
+      if (warp == 0) {
+        __syncwarp();
+        bool all = true;
+        for (int i = lane; i < seg.blocks; i += 32) all = all && get_flag(&sc.flag[first + i]) == a.call;
+        all = __all_sync(0xffffffffu, all);
+        if (lane == 0) complete = all;
+      }
+      __syncthreads();
+      final = complete;
+      if (final) {
+        // (a replayed graph makes the same call in the same scratch)
+        for (int i = tid; i < seg.blocks; i += kAttendThreads) set_flag(&sc.flag[first + i], 0);
+        constexpr int V = D / 32;
+        for (int col = warp; col < kCols; col += kWarps) {
+          float top = -INFINITY, sum = 0.0f, acc[V];
+          for (int i = lane; i < seg.blocks; i += 32)
+            top = fmaxf(top, __ldcg(&sc.ml[(first + i) * kCols + col]).x);
+          for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+#pragma unroll
+          for (int v = 0; v < V; v++) acc[v] = 0.0f;
+          for (int i0 = 0; i0 < seg.blocks; i0 += 32) {
+            float f = 0.0f;
+            if (i0 + lane < seg.blocks) {
+              const float2 ml = __ldcg(&sc.ml[(first + i0 + lane) * kCols + col]);
+              f = ml.x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(ml.x, top));
+              sum = __fmaf_rn(ml.y, f, sum);
+            }
+            const int n = min(32, seg.blocks - i0);
+#pragma unroll 4
+            for (int i = 0; i < n; i++) {
+              const float w = __shfl_sync(0xffffffffu, f, i);
+              const float2 *from =
+                  (const float2 *)(sc.o + ((first + i0 + i) * kCols + col) * D + lane * V);
+#pragma unroll
+              for (int v = 0; v < V; v += 2) {
+                const float2 z = __ldcg(from + v / 2);
+                acc[v] = __fmaf_rn(z.x, w, acc[v]);
+                acc[v + 1] = __fmaf_rn(z.y, w, acc[v + 1]);
+              }
+            }
+          }
+          for (int x = 16; x; x >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, x));
+          const float inv = top == -INFINITY ? 0.0f : __fdiv_rn(1.0f, sum);
+#pragma unroll
+          for (int v = 0; v < V; v++)
+            out[col * kRow + lane * V + v] = top == -INFINITY ? 0.0f : __fmul_rn(acc[v], inv);
+          if (lane == 0) write_lse(col, top, sum);
+        }
+        __syncthreads();
+      }
+    }
+    if (final) {
+      for (int half = warp; half < (NT + 1) / 2; half += kWarps) {
+        float y[2][D / 4];
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+          for (int j = 0; j < D / 4; j++) {
+            const int col = 16 * half + 8 * r + g;
+            y[r][j] = col < kCols ? out[(col < kCols ? col : 0) * kRow + t * (D / 4) + j] : 0.0f;
+          }
+        rotate_back<D, 2>(c, y, true);
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+          const int col = 16 * half + 8 * r + g, x = c0 + col;
+          if (col >= kCols || x >= ncol) continue;
+          uint4 *to = (uint4 *)((uint16_t *)a.out +
+                                ((int64_t)(at.first + x / group) * a.q_heads + head * group + x % group) * D +
+                                t * (D / 4));
+#pragma unroll
+          for (int i = 0; i < D / 32; i++)
+            to[i] = make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
+                               pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
+                               pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
+                               pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7]));
+        }
+      }
     }
     __syncthreads();  // the join's bytes are free again
     seg = after;
-  }
-}
-
-// ---- joining a job's parts ----
-template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(256) join_kernel(Cache c, Rows rows, AttendArgs a, int64_t slots) {
-  constexpr int kCols = 8 * NT, V = D / 32;
-  __shared__ float x[kCols][D + 4];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int group = a.q_heads / c.heads;
-  const Parts sc = carve(a.scratch, rows.n, slots, kCols, D);
-  pdl_wait();
-  const int64_t *units = sc.head + 1, *jobs = sc.head + 2 + rows.n;
-  const int64_t J = blockIdx.x, per = sc.head[0];
-  if (J >= jobs[rows.n]) return;
-  int lo = 0, hi = rows.n - 1;  // the last entry whose first job is <= J
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (jobs[mid] <= J) lo = mid;
-    else hi = mid - 1;
-  }
-  const int b = lo;
-  const int64_t jl = J - jobs[b], nj = jobs[b + 1] - jobs[b];
-  const int64_t n_units = (units[b + 1] - units[b]) / nj;
-  const int64_t first = units[b] + jl * n_units + kJobCost, last = units[b] + (jl + 1) * n_units - 1;
-  const int64_t w0 = first / per;
-  const int parts = n_units == 0 ? 0 : (int)(last / per - w0) + 1;
-  const int ct = (int)(jl / c.heads), head = (int)(jl % c.heads);
-  const int ncol = rows.count(b) * group, row0 = rows.first(b);
-
-  for (int col = warp; col < kCols; col += 8) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int i = lane; i < parts; i += 32)
-      top = fmaxf(top, sc.ml[(J + w0 + i) * kCols + col].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[V];
-#pragma unroll
-    for (int v = 0; v < V; v++) acc[v] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      float f = 0.0f;
-      if (i0 + lane < parts) {
-        const float2 ml = sc.ml[(J + w0 + i0 + lane) * kCols + col];
-        f = ml.x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(ml.x, top));
-        sum = __fmaf_rn(ml.y, f, sum);
-      }
-      const int n = min(32, parts - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; i++) {
-        const float w = __shfl_sync(0xffffffffu, f, i);
-        const float *from = sc.o + ((J + w0 + i0 + i) * kCols + col) * D + lane * V;
-        float z[V];
-#pragma unroll
-        for (int v = 0; v < V; v++) z[v] = from[v];
-#pragma unroll
-        for (int v = 0; v < V; v++) acc[v] = __fmaf_rn(z[v], w, acc[v]);
-      }
-    }
-    for (int o = 16; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-    const bool none = top == -INFINITY;  // no token to see: zeros
-    const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
-#pragma unroll
-    for (int v = 0; v < V; v++) x[col][lane * V + v] = none ? 0.0f : __fmul_rn(acc[v], inv);
-    const int at = ct * kCols + col;
-    if (lane == 0 && a.lse != nullptr && at < ncol)
-      a.lse[(int64_t)(row0 + at / group) * a.q_heads + head * group + at % group] =
-          none ? -INFINITY : __fmul_rn(__fadd_rn(top, __log2f(sum)), kLn2);
-  }
-  __syncthreads();
-  for (int half = warp; half < (NT + 1) / 2; half += 8) {
-    float y[2][D / 4];
-#pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-      for (int j = 0; j < D / 4; j++) {
-        const int col = 16 * half + 8 * r + g;
-        y[r][j] = col < kCols ? x[col < kCols ? col : 0][t * (D / 4) + j] : 0.0f;
-      }
-    rotate_back<D, 2>(c, y, true);
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const int col = 16 * half + 8 * r + g, at = ct * kCols + col;
-      if (col >= kCols || at >= ncol) continue;
-      uint4 *to = (uint4 *)((uint16_t *)a.out +
-                            ((int64_t)(row0 + at / group) * a.q_heads + head * group + at % group) * D +
-                            t * (D / 4));
-#pragma unroll
-      for (int i = 0; i < D / 32; i++)
-        to[i] = make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
-                           pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
-                           pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
-                           pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7]));
-    }
   }
 }
 
@@ -755,7 +786,7 @@ AttendPlan attend_plan(const Cache &c, int n, int rows, int most, int q_heads, i
   p.jobs = ((int64_t)rows * group / p.cols + n) * c.heads;
   p.sms = sms;
   const int64_t slots = p.jobs + 3 * sms;
-  p.bytes = head_bytes(n) + slots * p.cols * (c.head_dim + 2) * 4;
+  p.bytes = flag_bytes(slots) + slots * p.cols * (c.head_dim + 2) * 4;
   return p;
 }
 
@@ -769,18 +800,7 @@ static cudaError_t attend_nt(const Cache &c, int layer, const Rows &rows, const 
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   attend_kernel<D, NT, BF16><<<workers, kAttendThreads, smem, st>>>(c, layer, rows, a, slots);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)plan.jobs);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<D, NT, BF16>, c, rows, a, slots);
+  return cudaGetLastError();
 }
 
 template <bool BF16>

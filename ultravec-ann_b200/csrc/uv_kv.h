@@ -44,6 +44,7 @@ struct AttendArgs {
   int q_heads;
   float scale;
   void *scratch;
+  unsigned long long call;  // a number that no other call has, not 0
 };
 cudaError_t attend_launch(const Cache &c, int layer, const Rows &rows, const AttendArgs &a,
                           const AttendPlan &plan, bool bf16, cudaStream_t st);

@@ -45,43 +45,53 @@ class KvError(UVError):
         self.status = status
 
 
-def _stream(t):
-    import torch
-
-    return torch.cuda.current_stream(t.device).cuda_stream
+torch = None
+_raw_stream = None
 
 
-def _dtype(*tensors) -> int:
-    import torch
+def _load():
+    """torch and the library, on first use (the rest of the package works
+    without torch); the library's functions by name."""
+    global torch, _raw_stream
+    if torch is None:
+        import torch as t
 
-    d = tensors[0].dtype
-    if any(t.dtype != d for t in tensors) or d not in (torch.float16, torch.bfloat16):
-        raise ValueError("rows must be float16 or bfloat16, all of one type")
-    return 1 if d == torch.bfloat16 else 0
+        # the current stream's handle without a Stream object around it
+        _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: t.cuda.current_stream(i).cuda_stream)
+        torch = t
+    return lib()
 
 
-def _operand(x, heads, dim, device, name):
-    """Pointer and element strides of rows x heads x dim; laid out anew when a
+def _dtype(x) -> int:
+    d = x.dtype
+    if d is torch.bfloat16:
+        return 1
+    if d is torch.float16:
+        return 0
+    raise ValueError("rows must be float16 or bfloat16")
+
+
+def _operand(x, heads, dim, index, name):
+    """Tensor and element strides of rows x heads x dim; laid out anew when a
     row is not dense or not aligned."""
-    if x.dim() != 3 or (heads is not None and x.shape[1] != heads) or x.shape[2] != dim:
-        raise ValueError(f"{name} must be rows x {heads or 'heads'} x {dim}, got {tuple(x.shape)}")
-    if x.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    s = x.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or s[0] < 0 or s[1] < 0 or x.data_ptr() % 16:
-        import torch
-
+    shape = x.shape
+    if len(shape) != 3 or (heads is not None and shape[1] != heads) or shape[2] != dim:
+        raise ValueError(f"{name} must be rows x {heads or 'heads'} x {dim}, got {tuple(shape)}")
+    if x.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}")
+    row, head, one = x.stride()
+    if one != 1 or row % 8 or head % 8 or row <= 0 or head <= 0 or x.data_ptr() % 16:
         # (contiguous() would give a dense but misaligned view back as it is)
-        x = torch.empty(x.shape, dtype=x.dtype, device=device).copy_(x)
-        s = x.stride()
-    return x, s[0], s[1]
+        x = torch.empty(shape, dtype=x.dtype, device=x.device).copy_(x)
+        row, head, one = x.stride()
+    return x, row, head
 
 
-def _ints(x, n, device, name):
-    import torch
-
-    if x.dtype != torch.int32 or x.dim() != 1 or x.device != device or not x.is_contiguous():
-        raise ValueError(f"{name} must be a dense int32 vector on {device}")
+def _ints(x, n, index, name):
+    if (x.dtype is not torch.int32 or x.get_device() != index or x.dim() != 1
+            or not x.is_contiguous()):
+        raise ValueError(f"{name} must be a dense int32 vector on cuda:{index}")
     if n is not None and x.shape[0] != n:
         raise ValueError(f"{name} must have {n} entries, got {x.shape[0]}")
     return x.data_ptr()
@@ -93,8 +103,7 @@ class KvCache:
     def __init__(self, head_dim: int, kv_heads: int, n_pages: int, max_seqs: int, max_len: int, *,
                  layers: int = 1, page_tokens: int = 64, seed: int = 42, rounds: int = 1,
                  device: int = 0):
-        import torch
-
+        _load()
         dev = torch.device("cuda", device)
         max_pages = -(-max_len // page_tokens)
         desc = uv_kv(device, head_dim, kv_heads, layers, page_tokens, n_pages, max_seqs, max_pages,
@@ -116,6 +125,7 @@ class KvCache:
         uint8 [layers, pages, heads, page_tokens / 32, 32 (head_dim + 8)], table
         int32 [sequences, columns], lens and refs int32; signs [rounds,
         head_dim] of +-1."""
+        _load()
         layers, pages, heads, tiles, width = pool.shape
         if tiles * TILE != page_tokens or width != TILE * (head_dim + 8):
             raise ValueError(f"the pool's pages do not have the shape of {page_tokens} tokens of "
@@ -132,12 +142,10 @@ class KvCache:
                 desc.signs[r][i // 32] |= (x < 0) << (i % 32)
         self = cls.__new__(cls)
         self._attach(desc, pool, table, lens, refs)
-        check(lib().uv_kv_recount(self._p, _stream(pool)))
+        check(self._lib.uv_kv_recount(self._p, _raw_stream(self._index)))
         return self
 
     def _attach(self, desc, pool, table, lens, refs):
-        import torch
-
         for x, t, shape, name in (
                 (pool, torch.uint8, None, "pool"),
                 (table, torch.int32, (desc.max_seqs, desc.max_pages), "table"),
@@ -156,18 +164,20 @@ class KvCache:
         self._desc, self._p, self.device = desc, C.addressof(desc), pool.device
         self.head_dim, self.kv_heads, self.layers = desc.head_dim, desc.kv_heads, desc.layers
         self.page_tokens, self.n_pages, self.max_seqs = desc.page_tokens, desc.n_pages, desc.max_seqs
+        self._lib, self._index = lib(), pool.device.index
+        self._scale = 1.0 / math.sqrt(desc.head_dim)
         self._scratch_bytes = {}
 
     def reset(self) -> None:
         """Empty: no sequence has tokens, every page is free."""
-        check(lib().uv_kv_reset(self._p, _stream(self.pool)))
+        check(self._lib.uv_kv_reset(self._p, _raw_stream(self._index)))
 
     def check(self) -> None:
         """Waits for the stream and raises KvError if a call since the last
         check could not be done; until then calls that change the cache do
         nothing."""
         status = C.c_int32()
-        check(lib().uv_kv_check(self._p, C.byref(status), _stream(self.pool)))
+        check(self._lib.uv_kv_check(self._p, C.byref(status), _raw_stream(self._index)))
         if status.value:
             raise KvError(status.value)
 
@@ -176,67 +186,66 @@ class KvCache:
         """Room for counts[i] more tokens of seqs[i], which its length then
         includes.  The lowest free pages are taken, in the list's order; a
         shared last page is copied first.  All or nothing."""
-        n = seqs.shape[0]
-        check(lib().uv_kv_extend(self._p, _ints(seqs, None, self.device, "seqs"),
-                                 _ints(counts, n, self.device, "counts"), n, _stream(self.pool)))
+        n, i = seqs.shape[0], self._index
+        check(self._lib.uv_kv_extend(self._p, _ints(seqs, None, i, "seqs"),
+                                     _ints(counts, n, i, "counts"), n, _raw_stream(i)))
 
     def fork(self, src, dst, lens=None) -> None:
         """The empty sequence dst[i] shares the pages of src[i]'s first
         lens[i] tokens (all of them by default)."""
-        n = dst.shape[0]
-        check(lib().uv_kv_fork(self._p, _ints(src, n, self.device, "src"),
-                               _ints(dst, None, self.device, "dst"),
-                               None if lens is None else _ints(lens, n, self.device, "lens"), n,
-                               _stream(self.pool)))
+        n, i = dst.shape[0], self._index
+        check(self._lib.uv_kv_fork(self._p, _ints(src, n, i, "src"), _ints(dst, None, i, "dst"),
+                                   None if lens is None else _ints(lens, n, i, "lens"), n,
+                                   _raw_stream(i)))
 
     def copy(self, src, dst) -> None:
         """The empty sequence dst[i] gets a copy of src[i] in pages of its own."""
-        n = dst.shape[0]
-        check(lib().uv_kv_copy(self._p, _ints(src, n, self.device, "src"),
-                               _ints(dst, None, self.device, "dst"), n, _stream(self.pool)))
+        n, i = dst.shape[0], self._index
+        check(self._lib.uv_kv_copy(self._p, _ints(src, n, i, "src"), _ints(dst, None, i, "dst"), n,
+                                   _raw_stream(i)))
 
     def truncate(self, seqs, lens) -> None:
         """Sequence seqs[i] keeps its first lens[i] tokens."""
-        n = seqs.shape[0]
-        check(lib().uv_kv_truncate(self._p, _ints(seqs, None, self.device, "seqs"),
-                                   _ints(lens, n, self.device, "lens"), n, _stream(self.pool)))
+        n, i = seqs.shape[0], self._index
+        check(self._lib.uv_kv_truncate(self._p, _ints(seqs, None, i, "seqs"),
+                                       _ints(lens, n, i, "lens"), n, _raw_stream(i)))
 
     def free(self, seqs) -> None:
         """Sequences keep nothing; pages that no sequence holds are free."""
-        check(lib().uv_kv_truncate(self._p, _ints(seqs, None, self.device, "seqs"), None,
-                                   seqs.shape[0], _stream(self.pool)))
+        i = self._index
+        check(self._lib.uv_kv_truncate(self._p, _ints(seqs, None, i, "seqs"), None, seqs.shape[0],
+                                       _raw_stream(i)))
 
     def compact(self) -> None:
         """Moves the used pages to the lowest numbers."""
-        check(lib().uv_kv_compact(self._p, _stream(self.pool)))
+        check(self._lib.uv_kv_compact(self._p, _raw_stream(self._index)))
 
     # -- rows --
     def append(self, seqs, k, v, starts=None, *, layer: int = 0) -> None:
         """Quantises k and v (rows x kv_heads x head_dim) into the last tokens
         of the sequences: rows [starts[b], starts[b + 1]) are the last of
         seqs[b] (one row each without starts)."""
-        dtype, dev, n = _dtype(k, v), self.device, seqs.shape[0]
-        k, kr, kh = _operand(k, self.kv_heads, self.head_dim, dev, "k")
-        v, vr, vh = _operand(v, self.kv_heads, self.head_dim, dev, "v")
-        if k.shape[0] != v.shape[0]:
-            raise ValueError("k and v must have the same number of rows")
-        check(lib().uv_kv_append(
-            self._p, layer, _ints(seqs, None, dev, "seqs"),
-            None if starts is None else _ints(starts, n + 1, dev, "starts"), n, k.shape[0], dtype,
-            k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, _stream(self.pool)))
+        i, n, dtype = self._index, seqs.shape[0], _dtype(k)
+        if v.dtype is not k.dtype or v.shape != k.shape:
+            raise ValueError("k and v must have one type and one shape")
+        k, kr, kh = _operand(k, self.kv_heads, self.head_dim, i, "k")
+        v, vr, vh = _operand(v, self.kv_heads, self.head_dim, i, "v")
+        check(self._lib.uv_kv_append(
+            self._p, layer, _ints(seqs, None, i, "seqs"),
+            None if starts is None else _ints(starts, n + 1, i, "starts"), n, k.shape[0], dtype,
+            k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, _raw_stream(i)))
 
     def read(self, seqs, starts, rows: int, *, dtype=None, layer: int = 0):
         """The last starts[b + 1] - starts[b] tokens of seqs[b] as they are
         held: (k, v), rows x kv_heads x head_dim of dtype (bfloat16)."""
-        import torch
-
-        dtype, dev, n = dtype or torch.bfloat16, self.device, seqs.shape[0]
-        k = torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype, device=dev)
+        i, n = self._index, seqs.shape[0]
+        k = torch.empty((rows, self.kv_heads, self.head_dim), dtype=dtype or torch.bfloat16,
+                        device=self.device)
         v = torch.empty_like(k)
-        check(lib().uv_kv_read(
-            self._p, layer, _ints(seqs, None, dev, "seqs"),
-            None if starts is None else _ints(starts, n + 1, dev, "starts"), n, rows, _dtype(k),
-            k.data_ptr(), v.data_ptr(), _stream(self.pool)))
+        check(self._lib.uv_kv_read(
+            self._p, layer, _ints(seqs, None, i, "seqs"),
+            None if starts is None else _ints(starts, n + 1, i, "starts"), n, rows, _dtype(k),
+            k.data_ptr(), v.data_ptr(), _raw_stream(i)))
         return k, v
 
     # -- attention --
@@ -245,29 +254,28 @@ class KvCache:
         """Attention of q (rows x q_heads x head_dim, packed like append's
         rows) over the cache; row i of n sees the tokens up to its own.  most:
         the longest entry's rows.  Returns out, or (out, lse) with lse=True."""
-        import torch
-
-        dtype, dev, n = _dtype(q), self.device, seqs.shape[0]
-        q, qr, qh = _operand(q, None, self.head_dim, dev, "q")
+        i, n, dim, dtype = self._index, seqs.shape[0], self.head_dim, _dtype(q)
+        q, qr, qh = _operand(q, None, dim, i, "q")
         rows, heads = q.shape[0], q.shape[1]
         key = (n, rows, most if starts is not None else 1, heads)
         size = self._scratch_bytes.get(key)
         if size is None:
             b = C.c_int64()
-            check(lib().uv_kv_attend_bytes(self._p, *key, C.byref(b)))
+            check(self._lib.uv_kv_attend_bytes(self._p, *key, C.byref(b)))
             if len(self._scratch_bytes) > 1000:
                 self._scratch_bytes.clear()
-            size = self._scratch_bytes[key] = b.value
-        out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=dev)
-        sums = torch.empty((rows, heads), dtype=torch.float32, device=dev) if lse else None
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-        check(lib().uv_kv_attend(
-            self._p, layer, _ints(seqs, None, dev, "seqs"),
-            None if starts is None else _ints(starts, n + 1, dev, "starts"), n, rows, key[2],
-            dtype, q.data_ptr(), qr, qh, heads,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(),
-            None if sums is None else sums.data_ptr(), scratch.data_ptr(), size,
-            _stream(self.pool)))
+            size = self._scratch_bytes[key] = -(-b.value // 4)  # int32 words
+        out = (torch.empty_like(q) if qh == dim and qr == heads * dim else
+               torch.empty((rows, heads, dim), dtype=q.dtype, device=self.device))
+        sums = (torch.empty((rows, heads), dtype=torch.float32, device=self.device) if lse
+                else None)
+        scratch = self.work.new_empty(size)
+        check(self._lib.uv_kv_attend(
+            self._p, layer, _ints(seqs, None, i, "seqs"),
+            None if starts is None else _ints(starts, n + 1, i, "starts"), n, rows, key[2], dtype,
+            q.data_ptr(), qr, qh, heads, self._scale if scale is None else scale, out.data_ptr(),
+            None if sums is None else sums.data_ptr(), scratch.data_ptr(), 4 * size,
+            _raw_stream(i)))
         return (out, sums) if lse else out
 
 
@@ -277,24 +285,24 @@ def prompt_attention(q, k, v, starts, starts_k=None, *, causal: bool = True,
     x kv_heads x head_dim; sequence b has query rows [starts[b], starts[b + 1])
     and key rows [starts_k[b], starts_k[b + 1]) (the same by default), its
     queries being the last of its keys.  Returns out, or (out, lse)."""
-    import torch
-
-    dtype, dev, dim = _dtype(q, k, v), q.device, q.shape[-1]
-    if not q.is_cuda:
+    L = _load()
+    i, dim, dtype = q.get_device(), q.shape[-1], _dtype(q)
+    if i < 0:
         raise ValueError("q must be a CUDA tensor")
-    q, qr, qh = _operand(q, None, dim, dev, "q")
-    k, kr, kh = _operand(k, None, dim, dev, "k")
-    v, vr, vh = _operand(v, k.shape[1], dim, dev, "v")
-    if k.shape[0] != v.shape[0]:
-        raise ValueError("k and v must have the same number of rows")
+    if k.dtype is not q.dtype or v.dtype is not q.dtype or v.shape != k.shape:
+        raise ValueError("q, k and v must have one type, k and v one shape")
+    q, qr, qh = _operand(q, None, dim, i, "q")
+    k, kr, kh = _operand(k, None, dim, i, "k")
+    v, vr, vh = _operand(v, None, dim, i, "v")
+    rows, heads = q.shape[0], q.shape[1]
     n = starts.shape[0] - 1
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    sums = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if lse else None
-    check(lib().uv_prompt_attention(
-        dev.index or 0, _ints(starts, None, dev, "starts"),
-        None if starts_k is None else _ints(starts_k, n + 1, dev, "starts_k"), n, q.shape[0],
-        k.shape[0], q.shape[1], k.shape[1], dim, int(causal),
-        1.0 / math.sqrt(dim) if scale is None else scale, dtype, q.data_ptr(), qr, qh,
-        k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, out.data_ptr(),
-        None if sums is None else sums.data_ptr(), _stream(q)))
+    out = (torch.empty_like(q) if qh == dim and qr == heads * dim else
+           torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device))
+    sums = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if lse else None
+    check(L.uv_prompt_attention(
+        i, _ints(starts, None, i, "starts"),
+        None if starts_k is None else _ints(starts_k, n + 1, i, "starts_k"), n, rows, k.shape[0],
+        heads, k.shape[1], dim, int(causal), 1.0 / math.sqrt(dim) if scale is None else scale,
+        dtype, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh, v.data_ptr(), vr, vh, out.data_ptr(),
+        None if sums is None else sums.data_ptr(), _raw_stream(i)))
     return (out, sums) if lse else out
