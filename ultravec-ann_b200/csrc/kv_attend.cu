@@ -98,6 +98,12 @@ __device__ __forceinline__ Job load_entry(const Cache &c, const Rows &r, int b, 
   return j;
 }
 
+// a / b of numbers that are not negative: few are longer than 32 bits, whose
+// division takes a fifth of the time
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -151,7 +157,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ int64_t sums[2][kWarps];
-  __shared__ int64_t begin[3];  // first entry of the piece, its first tile, its first job
+  __shared__ int64_t begin[3];  // first entry of the piece, its first unit, its first job
+  __shared__ Job first_job;
   __shared__ float join_m[kWarps][kCols], join_l[kWarps][kCols];
   __shared__ bool complete;
 
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     if (w < warp) before_t += sums[0][w], before_j += sums[1][w];
   }
   // at least one tile for every warp of a block
-  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kWarps);
+  const int64_t per = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)kWarps);
   const int64_t T0 = per * blockIdx.x, T1 = min(T0 + per, total);
   // rows of sequences without a token
   for (int b = blockIdx.x; b < rows.n; b += gridDim.x) {
@@ -209,6 +216,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         begin[0] = b;
         begin[1] = bt;
         begin[2] = bj;
+        first_job = j;
         break;
       }
       bt += jobs * j.units();
@@ -218,10 +226,11 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   __syncthreads();
   int entry = (int)begin[0];
   int64_t base_t = begin[1], base_j = begin[2];
-  Job job = load_entry(c, rows, entry, group, kCols);
+  Job job = first_job;
 
   uint8_t *ring = smem + warp * kStages * kTileBytes;
-  uint32_t issued = 0, taken = 0;  // tiles of this warp's ring
+  int to_fill = 0, slot = 0;  // the ring's next slot to load, and to read
+  uint32_t phase = 0;
   bool dead = false;
 
   // A segment: the part of a job that lies in this block's piece.
@@ -240,8 +249,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         entry++;
         job = load_entry(c, rows, entry, group, kCols);
       }
-      const int64_t local = T - base_t, units = job.units(), jl = local / units;
-      const int off = (int)(local % units);
+      const int64_t local = T - base_t, units = job.units(), jl = quotient(local, units);
+      const int off = (int)(local - jl * units);
       const int take = (int)min(units - off, T1 - T);
       T += take;
       const int j0 = max(0, off - kJobCost), j1 = max(0, off + take - kJobCost);
@@ -250,8 +259,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       seg->job = job;
       const int64_t start = base_t + jl * units;
       seg->number = base_j + jl;
-      seg->first_block = (int)((start + kJobCost) / per);
-      seg->blocks = (int)((start + units - 1) / per) - seg->first_block + 1;
+      seg->first_block = (int)quotient(start + kJobCost, per);
+      seg->blocks = (int)quotient(start + units - 1, per) - seg->first_block + 1;
       seg->head = (int)(jl % c.heads);
       seg->c0 = ct * kCols;
       seg->j0 = j0;
@@ -275,20 +284,45 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
   auto issue = [&](int i) {
     const uint8_t *p = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)src, i & 31);
     if (lane == 0 && !dead) {
-      const int slot = issued % kStages;
-      tc::mbar_arrive_expect_tx(&full[warp][slot], kTileBytes);
-      bulk_load(ring + slot * kTileBytes, p, kTileBytes, &full[warp][slot]);
+      tc::mbar_arrive_expect_tx(&full[warp][to_fill], kTileBytes);
+      bulk_load(ring + to_fill * kTileBytes, p, kTileBytes, &full[warp][to_fill]);
     }
-    issued++;
+    if (++to_fill == kStages) to_fill = 0;
+  };
+  // Rows g and g + 8 of 16 of a segment's query columns, as they lie.
+  auto load_queries = [&](const Segment &seg, int half, uint32_t (&raw)[2][D / 8]) {
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int col = seg.c0 + 16 * half + 8 * r + g;
+      const bool live = 2 * half + r < NT && col < seg.job.n * group;
+      const int row = seg.job.first + (live ? col / group : 0);
+      const int hq = seg.head * group + (live ? col % group : 0);
+      const uint4 *q = (const uint4 *)((const uint16_t *)a.q.p + (int64_t)row * a.q.row +
+                                       (int64_t)hq * a.q.head + t * (D / 4));
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const uint4 v = live ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+        raw[r][4 * i] = v.x;
+        raw[r][4 * i + 1] = v.y;
+        raw[r][4 * i + 2] = v.z;
+        raw[r][4 * i + 3] = v.w;
+      }
+    }
   };
   auto start = [&](const Segment &seg) {
     lookup(seg, 0);
     for (int i = 0; i < min(seg.mine, kStages); i++) issue(i);
   };
 
+  // The first queries are asked for ahead of the tiles: behind a ring's worth
+  // from every warp of the card they would wait for 3 us.
+  uint32_t raw[2][D / 8];
   Segment seg, after;
   bool more = next(&seg);
-  if (more) start(seg);
+  if (more) {
+    load_queries(seg, 0, raw);
+    start(seg);
+  }
   while (more) {
     const Job &at = seg.job;
     const int ncol = at.n * group, c0 = seg.c0, head = seg.head, mine = seg.mine;
@@ -302,25 +336,9 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     int lim[NT][2];
 #pragma unroll
     for (int half = 0; half < (NT + 1) / 2; half++) {
-      uint32_t raw[2][D / 8];
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const int col = c0 + 16 * half + 8 * r + g;
-        const bool live = (2 * half + r < NT) && col < ncol;
-        const int row = at.first + (live ? col / group : 0), hq = head * group + (live ? col % group : 0);
-        const uint4 *q = (const uint4 *)((const uint16_t *)a.q.p + (int64_t)row * a.q.row +
-                                         (int64_t)hq * a.q.head + t * (D / 4));
-#pragma unroll
-        for (int i = 0; i < D / 32; i++) {
-          const uint4 v = live ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
-          raw[r][4 * i] = v.x;
-          raw[r][4 * i + 1] = v.y;
-          raw[r][4 * i + 2] = v.z;
-          raw[r][4 * i + 3] = v.w;
-        }
-      }
+      if (half > 0) load_queries(seg, half, raw);
       float y[2][D / 4];
-      rotate_rows<D, BF16>(c, raw, y);
+      rotate_rows<D, BF16, NT == 1 ? 1 : 2>(c, raw, y);
 #pragma unroll
       for (int r = 0; r < 2; r++) {
         if (2 * half + r >= NT) break;
@@ -405,34 +423,40 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     };
     // ---- one pass over the warp's tiles ----
     for (int i = 0; i < mine; i++) {
-      const int slot = taken % kStages;
-      if (!dead && !__all_sync(0xffffffffu, tc::mbar_wait(&full[warp][slot], (taken / kStages) & 1,
-                                                          kWaitLimit))) {
+      uint64_t *bar = &full[warp][slot];
+      if (!__all_sync(0xffffffffu, tc::mbar_try_wait(bar, phase)) &&
+          !__all_sync(0xffffffffu, tc::mbar_wait(bar, phase, kWaitLimit))) {
         // give up: note it, let the copies in flight land, load no more
         if (lane == 0) atomicOr(&c.work[kStatus], kTimeout);
-        for (; taken < issued; taken++)
-          tc::mbar_wait(&full[warp][taken % kStages], (taken / kStages) & 1, kWaitLimit);
+        for (int k = 0; k < min(kStages, mine - i); k++) {
+          tc::mbar_wait(&full[warp][slot], phase, kWaitLimit);
+          if (++slot == kStages) slot = 0, phase ^= 1;
+        }
         dead = true;
       }
       if (dead) break;
-      taken++;
       const uint8_t *tile = ring + slot * kTileBytes;
       const int key0 = (seg.j0 + warp + i * kWarps) * kTile;
 
       float s[2][NT][4];
+      Words<D> kw[2][2];
 #pragma unroll
       for (int sb = 0; sb < 2; sb++) {
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+          kw[sb][r] = load_words<D>(tile + (16 * sb + 8 * r + g) * (D / 2) + t * (D / 8));
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int k = 0; k < 4; k++) s[sb][nt][k] = hs[nt][k & 1];
-        const uint8_t *rowp = tile + (16 * sb + g) * (D / 2) + t * (D / 8);
-        const Words<D> ka = load_words<D>(rowp), kb = load_words<D>(rowp + 8 * (D / 2));
+      }
 #pragma unroll
-        for (int w = 0; w < D / 32; w++) {
+      for (int w = 0; w < D / 32; w++)
+#pragma unroll
+        for (int sb = 0; sb < 2; sb++) {
           uint32_t xa[4], xb[4];
-          unpack8(ka.w[w], xa);
-          unpack8(kb.w[w], xb);
+          unpack8(kw[sb][0].w[w], xa);
+          unpack8(kw[sb][1].w[w], xb);
 #pragma unroll
           for (int k = 0; k < 4; k += 2)
 #pragma unroll
@@ -442,11 +466,11 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
                 mma16816<false>(s[sb][nt], xa[k], xb[k], xa[k + 1], xb[k + 1],
                                 qf[part][nt][w][k], qf[part][nt][w][k + 1]);
         }
-      }
       float ks[2][2], vs[2][2];
       const float *kscale = (const float *)(tile + kTile * (D / 2));
       const float *vscale = (const float *)(tile + kTile * (D + 4));
-      const bool whole = key0 + kTile <= lim_first;  // every column sees every token
+      // every column sees every token
+      const bool whole = __all_sync(0xffffffffu, key0 + kTile <= lim_first);
 #pragma unroll
       for (int sb = 0; sb < 2; sb++)
 #pragma unroll
@@ -584,12 +608,16 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         if ((ahead & 31) == 0) lookup(seg, ahead);
         issue(ahead);
       }
+      if (++slot == kStages) slot = 0, phase ^= 1;
     }
 
     recentre();
     // the next segment's tiles are on their way while this one's parts join
     more = next(&after);
-    if (more) start(after);
+    if (more) {
+      load_queries(after, 0, raw);
+      start(after);
+    }
 
     // ---- join the warps' parts: 2 and 3 leave theirs, 0 and 1 add to them ----
 #pragma unroll
@@ -635,7 +663,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     }
     // ---- the job's result, or this block's part of it ----
     // (starts that do not rise give more jobs than rows allow: no slot, no part)
-    const int64_t slot = seg.number + blockIdx.x;
+    const int64_t part = seg.number + blockIdx.x;
     const bool fits = seg.number + seg.first_block + seg.blocks <= slots;
     bool final = seg.blocks == 1 && fits;
     auto total_of = [&](int col, float *top) {
@@ -671,17 +699,17 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         const int col = i / (D / 4), d4 = i % (D / 4);
         const float4 u = *(const float4 *)(out + col * kRow + 4 * d4);
         const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4);
-        __stcg((float4 *)(sc.o + (slot * kCols + col) * D) + d4,
+        __stcg((float4 *)(sc.o + (part * kCols + col) * D) + d4,
                make_float4(__fadd_rn(u.x, v.x), __fadd_rn(u.y, v.y), __fadd_rn(u.z, v.z),
                            __fadd_rn(u.w, v.w)));
       }
       if (tid < kCols) {
         float top;
         const float sum = total_of(tid, &top);
-        __stcg(&sc.ml[slot * kCols + tid], make_float2(top, sum));
+        __stcg(&sc.ml[part * kCols + tid], make_float2(top, sum));
       }
       __syncthreads();
-      if (tid == 0) set_flag(&sc.flag[slot], a.call);
+      if (tid == 0) set_flag(&sc.flag[part], a.call);
       // Whoever finds every part written joins them, in their order.  The block
       // that finishes last does; two that finish together may both, and write
       // the same bytes.  Nothing waits, and no counter has to start at zero.

@@ -110,15 +110,14 @@ __device__ __forceinline__ void pdl_launch() {
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  // (not volatile: independent products may be reordered between dependent ones)
   if (BF16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -206,8 +205,8 @@ __device__ __forceinline__ void hadamard_mma(float (&y)[2][D / 4], const uint32_
   }
 }
 
-// The remaining index bits, then 1 / sqrt(D) if asked.
-template <int D>
+// The remaining index bits, of both rows or of row g alone.
+template <int D, int ROWS = 2>
 __device__ __forceinline__ void hadamard_rest(float (&y)[2][D / 4]) {
 #pragma unroll
   for (int h = 4; h < D / 4; h *= 2)
@@ -215,7 +214,7 @@ __device__ __forceinline__ void hadamard_rest(float (&y)[2][D / 4]) {
     for (int j = 0; j < D / 4; j++)
       if ((j & h) == 0)
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
+        for (int r = 0; r < ROWS; r++) {
           const float u = y[r][j], v = y[r][j + h];
           y[r][j] = __fadd_rn(u, v);
           y[r][j + h] = __fsub_rn(u, v);
@@ -279,10 +278,10 @@ __device__ __forceinline__ void apply_signs(const Cache &c, int round, float (&y
   }
 }
 
-// y = R x for 16 rows of packed halves or bfloats (a is consumed).  The
-// products are exact and add up in f32; later rounds take f32 rows as three
-// bfloats.
-template <int D, bool BF16>
+// y = R x for 16 rows of packed halves or bfloats (a is consumed), or for rows
+// g alone (ROWS = 1: the others are zero).  The products are exact and add up
+// in f32; later rounds take f32 rows as three bfloats.
+template <int D, bool BF16, int ROWS = 2>
 __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D / 8],
                                             float (&y)[2][D / 4]) {
 #pragma unroll
@@ -291,14 +290,14 @@ __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D /
 #pragma unroll
     for (int j = 0; j < (D == 64 ? 8 : 16); j++) {
       const uint32_t flip = (s << (15 - j)) & 0x80008000u;
-      a[0][16 * w + j] ^= flip;
-      a[1][16 * w + j] ^= flip;
+#pragma unroll
+      for (int r = 0; r < ROWS; r++) a[r][16 * w + j] ^= flip;
     }
   }
 #pragma unroll
   for (int j = 0; j < D / 4; j++) y[0][j] = y[1][j] = 0.0f;
   hadamard_mma<D, BF16>(y, a, Hadamard::make<BF16>());
-  hadamard_rest<D>(y);
+  hadamard_rest<D, ROWS>(y);
   float scale = inv_sqrt_d<D>();
   for (int r = 1; r < c.rounds; r++) {
     apply_signs<D>(c, r, y);
@@ -306,10 +305,9 @@ __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D /
     scale = __fmul_rn(scale, inv_sqrt_d<D>());
   }
 #pragma unroll
-  for (int j = 0; j < D / 4; j++) {
-    y[0][j] = __fmul_rn(y[0][j], scale);
-    y[1][j] = __fmul_rn(y[1][j], scale);
-  }
+  for (int j = 0; j < D / 4; j++)
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) y[r][j] = __fmul_rn(y[r][j], scale);
 }
 
 // x = R^T y in place, for 16 f32 rows; the first transform takes PARTS
