@@ -776,6 +776,12 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
             y[r][j] = col < kCols ? out[(col < kCols ? col : 0) * kRow + t * (D / 4) + j] : 0.0f;
           }
         rotate_back<D, 2>(c, y, true);
+        const float f = rotation_scale<D>(c);
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) {
+          y[0][j] = __fmul_rn(y[0][j], f);
+          y[1][j] = __fmul_rn(y[1][j], f);
+        }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
           const int col = 16 * half + 8 * r + g, x = c0 + col;

@@ -63,119 +63,136 @@ __device__ __forceinline__ uint32_t pack_codes(const float *t) {
   return w - 0x4b400000u * 0x11111111u;
 }
 
+// A warp takes `each` of a block's 2 * heads parts (keys and values of a head),
+// which share what finding the block took: four dependent loads.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer, Rows rows,
-                                                             Strided kin, Strided vin,
-                                                             int64_t blocks) {
+                                                             Strided kin, Strided vin, int64_t blocks,
+                                                             int each) {
   if (c.work[kStatus] != 0) return;  // an extend failed: these rows have no place
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-  const int parts = 2 * c.heads;
-  if (item >= blocks * parts) return;
-  const int part = (int)(item % parts), head = part >> 1;
-  const bool value = part & 1;
-  const Block at = find_block(rows, c, item / parts);
+  const int parts = 2 * c.heads, groups = (parts + each - 1) / each;
+  if (item >= blocks * groups) return;
+  const Block at = find_block(rows, c, item / groups);
   const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
   if (s < 0 && lane == 0) atomicOr(&c.work[kStatus], kBadSeq);
   if (pos0 >= len) return;
-  const Strided &in = value ? vin : kin;
-  const uint16_t *src = (const uint16_t *)in.p + (int64_t)head * in.head + t * (D / 4);
-
-  uint32_t a[2][D / 8];
-  bool live[2];
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    const int p = pos0 + g + 8 * r;
-    live[r] = p >= begin && p < len;
-    const uint4 *q = (const uint4 *)(src + (int64_t)(first + p) * in.row);
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      const uint4 w = live[r] ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
-      a[r][4 * i] = w.x;
-      a[r][4 * i + 1] = w.y;
-      a[r][4 * i + 2] = w.z;
-      a[r][4 * i + 3] = w.w;
-    }
-  }
   const int page = c.page_at(s, pos0 / c.page_tokens);
   if (c.refs[page] != 1) {  // others hold it: extend has not made room
     if (lane == 0) atomicOr(&c.work[kStatus], kShared);
     return;
   }
-  float y[2][D / 4];
-  rotate_rows<D, BF16>(c, a, y);
+  const bool live[2] = {pos0 + g >= begin && pos0 + g < len, pos0 + g + 8 >= begin && pos0 + g + 8 < len};
+  const int from = (int)(item % groups) * each, to_part = min(from + each, parts);
+  for (int part = from; part < to_part; part++) {
+    const int head = part >> 1;
+    const bool value = part & 1;
+    const Strided &in = value ? vin : kin;
+    const uint16_t *src = (const uint16_t *)in.p + (int64_t)head * in.head + t * (D / 4);
+    uint32_t a[2][D / 8];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const uint4 *q = (const uint4 *)(src + (int64_t)(first + pos0 + g + 8 * r) * in.row);
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const uint4 w = live[r] ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+        a[r][4 * i] = w.x;
+        a[r][4 * i + 1] = w.y;
+        a[r][4 * i + 2] = w.z;
+        a[r][4 * i + 3] = w.w;
+      }
+    }
+    float y[2][D / 4];
+    rotate_rows<D, BF16, 2, false>(c, a, y);
 
-  uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
-                  (value ? kTile * (D / 2 + 4) : 0);
-  const int row0 = pos0 % kTile;
+    uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
+                    (value ? kTile * (D / 2 + 4) : 0);
+    const int row0 = pos0 % kTile;
+    const float shrink = rotation_scale<D>(c);
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    // a power of two takes the row's size out, so that squares neither
-    // overflow nor vanish
-    float m = 0.0f;
+    for (int r = 0; r < 2; r++) {
+      float square = 0.0f, grow = 1.0f;
+      auto squares = [&] {
+        float more = 0.0f;
+        square = 0.0f;
 #pragma unroll
-    for (int j = 0; j < D / 4; j++) m = fmaxf(m, fabsf(y[r][j]));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const int e = max(-100, min(log2i(m), 126));
-    const float down = exp2i(-e);
-    float square = 0.0f;
-#pragma unroll
-    for (int j = 0; j < D / 4; j++) {
-      y[r][j] = __fmul_rn(y[r][j], down);
-      square = __fmaf_rn(y[r][j], y[r][j], square);
-    }
-    square += __shfl_xor_sync(0xffffffffu, square, 1);
-    square += __shfl_xor_sync(0xffffffffu, square, 2);
-    const float inv = square > 0.0f
-                          ? __fdiv_rn(1.0f, __fmul_rn(kStep, __fsqrt_rn(__fmul_rn(square, 1.0f / D))))
-                          : 0.0f;
-    float ly = 0.0f;
-    uint32_t w[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      float n[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float z = fminf(fmaxf(__fmul_rn(y[r][8 * i + j], inv), -8.0f), 7.0f);
-        n[j] = __fadd_rd(z, 12582920.0f);  // 1.5 * 2^23 + 8, rounded down: floor(z) + 8
-        ly = __fmaf_rn(__fadd_rn(__fsub_rn(n[j], 12582920.0f), 0.5f), y[r][8 * i + j], ly);
-      }
-      w[i] = pack_codes(n);
-    }
-    ly += __shfl_xor_sync(0xffffffffu, ly, 1);
-    ly += __shfl_xor_sync(0xffffffffu, ly, 2);
-    // |y| finite and not zero: ly > 0, since every level has its value's sign
-    // (a row of zeros has the scale zero; one with an infinity or a NaN gets NaN)
-    const float scale = square == 0.0f ? 0.0f : __fmul_rn(__fdiv_rn(square, ly), exp2i(e));
-    const int row = row0 + g + 8 * r;
-    if (live[r] && t == 0) ((float *)(tile + kTile * (D / 2)))[row] = scale;
-    if (!value) {
-      if (live[r]) {
-        uint32_t *to = (uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
-        if (D == 128) {
-          *(uint4 *)to = make_uint4(w[0], w[1], w[2], w[D / 32 - 1]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 32; i++) to[i] = w[i];
+        for (int j = 0; j < D / 4; j += 2) {
+          square = __fmaf_rn(y[r][j], y[r][j], square);
+          more = __fmaf_rn(y[r][j + 1], y[r][j + 1], more);
         }
-      }
-      continue;
-    }
-    // Tokens 2p and 2p + 1 are lanes g and g ^ 1: the even one takes the
-    // granules of dimensions 0..3 of each word, the odd one those of 4..7.
-    const bool odd = g & 1;
-    const bool other = __shfl_xor_sync(0xffffffffu, (int)live[r], 4);
-    uint16_t *pair = (uint16_t *)(tile + (row >> 1) * D) + t * (D / 8);
+        square = __fadd_rn(square, more);
+        square += __shfl_xor_sync(0xffffffffu, square, 1);
+        square += __shfl_xor_sync(0xffffffffu, square, 2);
+      };
+      squares();
+      if (__any_sync(0xffffffffu, !(square > 0x1p-80f && square < 0x1p80f))) {
+        // A power of two takes the row's size out, so that squares neither
+        // overflow nor vanish (for the rows that need it: 1 for the others).
+        float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      const uint32_t x = __shfl_xor_sync(0xffffffffu, w[i], 4);
-      if (live[r] && other) {
-        ((uint32_t *)pair)[2 * i + odd] =
-            odd ? (x >> 16) | (w[i] & 0xffff0000u) : (w[i] & 0xffffu) | (x << 16);
-      } else if (live[r]) {
-        pair[4 * i + odd] = (uint16_t)w[i];
-        pair[4 * i + 2 + odd] = (uint16_t)(w[i] >> 16);
+        for (int j = 0; j < D / 4; j++) m = fmaxf(m, fabsf(y[r][j]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = square > 0x1p-80f && square < 0x1p80f ? 0 : max(-100, min(log2i(m), 126));
+        grow = exp2i(e);
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) y[r][j] = __fmul_rn(y[r][j], exp2i(-e));
+        squares();
+      }
+      const float inv =
+          square > 0.0f ? __fdiv_rn(1.0f, __fmul_rn(kStep, __fsqrt_rn(__fmul_rn(square, 1.0f / D))))
+                        : 0.0f;
+      float ly = 0.0f, more = 0.0f;
+      uint32_t w[D / 32];
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        float n[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float z = fminf(fmaxf(__fmul_rn(y[r][8 * i + j], inv), -8.0f), 7.0f);
+          n[j] = __fadd_rd(z, 12582920.0f);  // 1.5 * 2^23 + 8, rounded down: floor(z) + 8
+          float &sum = j % 2 ? more : ly;
+          sum = __fmaf_rn(__fadd_rn(__fsub_rn(n[j], 12582920.0f), 0.5f), y[r][8 * i + j], sum);
+        }
+        w[i] = pack_codes(n);
+      }
+      ly = __fadd_rn(ly, more);
+      ly += __shfl_xor_sync(0xffffffffu, ly, 1);
+      ly += __shfl_xor_sync(0xffffffffu, ly, 2);
+      // |y| finite and not zero: ly > 0, since every level has its value's sign
+      // (a row of zeros has the scale zero; one with an infinity or a NaN gets NaN)
+      const float scale =
+          square == 0.0f ? 0.0f : __fmul_rn(__fmul_rn(__fdiv_rn(square, ly), shrink), grow);
+      const int row = row0 + g + 8 * r;
+      if (live[r] && t == 0) ((float *)(tile + kTile * (D / 2)))[row] = scale;
+      if (!value) {
+        if (live[r]) {
+          uint32_t *to = (uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
+          if (D == 128) {
+            *(uint4 *)to = make_uint4(w[0], w[1], w[2], w[D / 32 - 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) to[i] = w[i];
+          }
+        }
+        continue;
+      }
+      // Tokens 2p and 2p + 1 are lanes g and g ^ 1: the even one takes the
+      // granules of dimensions 0..3 of each word, the odd one those of 4..7.
+      const bool odd = g & 1;
+      const bool other = __shfl_xor_sync(0xffffffffu, (int)live[r], 4);
+      uint16_t *pair = (uint16_t *)(tile + (row >> 1) * D) + t * (D / 8);
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {
+        const uint32_t x = __shfl_xor_sync(0xffffffffu, w[i], 4);
+        if (live[r] && other) {
+          ((uint32_t *)pair)[2 * i + odd] =
+              odd ? (x >> 16) | (w[i] & 0xffff0000u) : (w[i] & 0xffffu) | (x << 16);
+        } else if (live[r]) {
+          pair[4 * i + odd] = (uint16_t)w[i];
+          pair[4 * i + 2 + odd] = (uint16_t)(w[i] >> 16);
+        }
       }
     }
   }
@@ -184,87 +201,102 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) read_kernel(Cache c, int layer, Rows rows,
                                                            uint16_t *kout, uint16_t *vout,
-                                                           int64_t blocks) {
+                                                           int64_t blocks, int each) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-  const int parts = 2 * c.heads;
-  if (item >= blocks * parts) return;
-  const int part = (int)(item % parts), head = part >> 1;
-  const bool value = part & 1;
-  const Block at = find_block(rows, c, item / parts);
+  const int parts = 2 * c.heads, groups = (parts + each - 1) / each;
+  if (item >= blocks * groups) return;
+  const Block at = find_block(rows, c, item / groups);
   const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
-  uint16_t *out = (value ? vout : kout) + head * D;
-  for (int i = lane; i < at.blank * (D / 8); i += 32)  // rows without a token read as zeros
-    ((uint4 *)(out + (int64_t)(at.row0 + i / (D / 8)) * c.heads * D))[i % (D / 8)] =
-        make_uint4(0, 0, 0, 0);
+  const int from = (int)(item % groups) * each, to_part = min(from + each, parts);
+  if (at.blank > 0)  // rows without a token read as zeros
+    for (int part = from; part < to_part; part++)
+      for (int i = lane; i < at.blank * (D / 8); i += 32)
+        ((uint4 *)((part & 1 ? vout : kout) + ((int64_t)(at.row0 + i / (D / 8)) * c.heads + (part >> 1)) * D))
+            [i % (D / 8)] = make_uint4(0, 0, 0, 0);
   if (pos0 >= len) return;
   const int page = c.page_at(s, pos0 / c.page_tokens);
-  const uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
-                        (value ? kTile * (D / 2 + 4) : 0);
   const int row0 = pos0 % kTile;
-  bool live[2];
-  float scale[2];
-  uint32_t w[2][D / 32];
+  const float shrink = rotation_scale<D>(c);
+  for (int part = from; part < to_part; part++) {
+    const int head = part >> 1;
+    const bool value = part & 1;
+    uint16_t *out = (value ? vout : kout) + head * D;
+    const uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
+                          (value ? kTile * (D / 2 + 4) : 0);
+    bool live[2];
+    float scale[2];
+    uint32_t w[2][D / 32];
 #pragma unroll
-  for (int r = 0; r < 2; r++) {
-    const int row = row0 + g + 8 * r, p = pos0 + g + 8 * r;
-    live[r] = p >= begin && p < len;
-    scale[r] = live[r] ? ((const float *)(tile + kTile * (D / 2)))[row] : 0.0f;
-    if (!value) {
-      const uint32_t *from = (const uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
+    for (int r = 0; r < 2; r++) {
+      const int row = row0 + g + 8 * r, p = pos0 + g + 8 * r;
+      live[r] = p >= begin && p < len;
+      scale[r] = live[r] ? __fmul_rn(((const float *)(tile + kTile * (D / 2)))[row], shrink) : 0.0f;
+      if (!value) {
+        const uint32_t *from_row = (const uint32_t *)(tile + row * (D / 2)) + t * (D / 32);
+        if (D == 128) {
+          const uint4 v = *(const uint4 *)from_row;
+          w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][D / 32 - 1] = v.w;
+        } else {
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) w[r][i] = from[i];
-    } else {
-      const bool odd = g & 1;
-      const uint32_t *pair = (const uint32_t *)(tile + (row >> 1) * D) + t * (D / 16);
+          for (int i = 0; i < D / 32; i++) w[r][i] = from_row[i];
+        }
+      } else {
+        const bool odd = g & 1;
+        const uint2 *pair = (const uint2 *)((const uint32_t *)(tile + (row >> 1) * D) + t * (D / 16));
 #pragma unroll
-      for (int i = 0; i < D / 32; i++) {
-        const uint32_t x = pair[2 * i], y = pair[2 * i + 1];
-        w[r][i] = __byte_perm(x, y, odd ? 0x7632 : 0x5410);
+        for (int i = 0; i < D / 32; i++) {
+          const uint2 v = pair[i];
+          w[r][i] = __byte_perm(v.x, v.y, odd ? 0x7632 : 0x5410);
+        }
       }
     }
-  }
-  // The levels are exact halves, so the first transform needs one product.
-  // A half2 holds the nibbles i and i + 4 of a word: with the element's bits
-  // renamed (2, 0, 1 for 0, 1, 2) the owner of every output stays the same.
-  float y[2][D / 4];
+    // The levels are exact halves, so the first transform needs one product.
+    // A half2 holds the nibbles i and i + 4 of a word: with the element's bits
+    // renamed (2, 0, 1 for 0, 1, 2) the owner of every output stays the same.
+    float y[2][D / 4];
 #pragma unroll
-  for (int j = 0; j < D / 4; j++) y[0][j] = y[1][j] = 0.0f;
-  uint32_t a[2][D / 8];
+    for (int j = 0; j < D / 4; j++) y[0][j] = y[1][j] = 0.0f;
+    uint32_t a[2][D / 8];
 #pragma unroll
-  for (int r = 0; r < 2; r++)
+    for (int r = 0; r < 2; r++)
 #pragma unroll
-    for (int i = 0; i < D / 32; i++) {
-      uint32_t o[4];
-      unpack8_levels(w[r][i], o);
+      for (int i = 0; i < D / 32; i++) {
+        uint32_t o[4];
+        unpack8_levels(w[r][i], o);
 #pragma unroll
-      for (int k = 0; k < 4; k++) a[r][4 * i + k] = o[k];
+        for (int k = 0; k < 4; k++) a[r][4 * i + k] = o[k];
+      }
+    hadamard_mma<D, false>(y, a, Hadamard::make<false>());
+    hadamard_rest<D>(y);
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int i = 0; i < D / 32; i++) {  // element 2 k + h of a word -> k + 4 h
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) o[(k >> 1) + 4 * (k & 1)] = y[r][8 * i + k];
+#pragma unroll
+        for (int k = 0; k < 8; k++) y[r][8 * i + k] = __fmul_rn(o[k], scale[r]);
+      }
+    rotate_back<D, 3>(c, y, false);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      if (!live[r]) continue;
+      uint4 *to = (uint4 *)(out + (int64_t)(first + pos0 + g + 8 * r) * c.heads * D + t * (D / 4));
+#pragma unroll
+      for (int i = 0; i < D / 32; i++)
+        __stcs(to + i, make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
+                                  pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
+                                  pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
+                                  pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7])));
     }
-  hadamard_mma<D, false>(y, a, Hadamard::make<false>());
-  hadamard_rest<D>(y);
-#pragma unroll
-  for (int r = 0; r < 2; r++)
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) {  // element 2 k + h of a word -> k + 4 h
-      float o[8];
-#pragma unroll
-      for (int k = 0; k < 8; k++) o[(k >> 1) + 4 * (k & 1)] = y[r][8 * i + k];
-#pragma unroll
-      for (int k = 0; k < 8; k++) y[r][8 * i + k] = __fmul_rn(o[k], scale[r]);
-    }
-  rotate_back<D, 3>(c, y, false);
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    if (!live[r]) continue;
-    uint4 *to = (uint4 *)(out + (int64_t)(first + pos0 + g + 8 * r) * c.heads * D + t * (D / 4));
-#pragma unroll
-    for (int i = 0; i < D / 32; i++)
-      __stcs(to + i, make_uint4(pack2<BF16>(y[r][8 * i], y[r][8 * i + 1]),
-                                pack2<BF16>(y[r][8 * i + 2], y[r][8 * i + 3]),
-                                pack2<BF16>(y[r][8 * i + 4], y[r][8 * i + 5]),
-                                pack2<BF16>(y[r][8 * i + 6], y[r][8 * i + 7])));
   }
 }
+
+// Parts a warp takes: one while that leaves the card room (a token each), four
+// where there are many blocks.
+static int parts_each(int64_t blocks, int heads) { return blocks * 2 * heads > 148 * 16 ? 4 : 1; }
 
 static int64_t block_bound(const Rows &r) {
   return r.starts == nullptr ? r.n : r.rows / 16 + 2 * (int64_t)r.n;
@@ -273,18 +305,22 @@ static int64_t block_bound(const Rows &r) {
 template <int D, bool BF16>
 static cudaError_t append_d(const Cache &c, int layer, const Rows &rows, const Strided &k,
                             const Strided &v, cudaStream_t st) {
-  const int64_t blocks = block_bound(rows), warps = blocks * 2 * c.heads;
+  const int64_t blocks = block_bound(rows);
+  const int each = parts_each(blocks, c.heads);
+  const int64_t warps = blocks * ((2 * c.heads + each - 1) / each);
   const int64_t grid = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
-  append_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, k, v, blocks);
+  append_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, k, v, blocks, each);
   return cudaGetLastError();
 }
 template <int D, bool BF16>
 static cudaError_t read_d(const Cache &c, int layer, const Rows &rows, void *k, void *v,
                           cudaStream_t st) {
-  const int64_t blocks = block_bound(rows), warps = blocks * 2 * c.heads;
+  const int64_t blocks = block_bound(rows);
+  const int each = parts_each(blocks, c.heads);
+  const int64_t warps = blocks * ((2 * c.heads + each - 1) / each);
   const int64_t grid = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
   read_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, (uint16_t *)k,
-                                                               (uint16_t *)v, blocks);
+                                                               (uint16_t *)v, blocks, each);
   return cudaGetLastError();
 }
 

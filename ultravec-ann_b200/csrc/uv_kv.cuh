@@ -280,8 +280,9 @@ __device__ __forceinline__ void apply_signs(const Cache &c, int round, float (&y
 
 // y = R x for 16 rows of packed halves or bfloats (a is consumed), or for rows
 // g alone (ROWS = 1: the others are zero).  The products are exact and add up
-// in f32; later rounds take f32 rows as three bfloats.
-template <int D, bool BF16, int ROWS = 2>
+// in f32; later rounds take f32 rows as three bfloats.  With SCALE = false the
+// result is sqrt(D)^rounds times too large.
+template <int D, bool BF16, int ROWS = 2, bool SCALE = true>
 __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D / 8],
                                             float (&y)[2][D / 4]) {
 #pragma unroll
@@ -304,26 +305,28 @@ __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D /
     hadamard_f32<D, 3>(y, Hadamard::make<true>());
     scale = __fmul_rn(scale, inv_sqrt_d<D>());
   }
+  if (!SCALE) return;
 #pragma unroll
   for (int j = 0; j < D / 4; j++)
 #pragma unroll
     for (int r = 0; r < ROWS; r++) y[r][j] = __fmul_rn(y[r][j], scale);
 }
 
-// x = R^T y in place, for 16 f32 rows; the first transform takes PARTS
-// bfloats a value, and may have been done already (first = false).
+// sqrt(D)^-rounds
+template <int D>
+__device__ __forceinline__ float rotation_scale(const Cache &c) {
+  float scale = inv_sqrt_d<D>();
+  for (int r = 1; r < c.rounds; r++) scale = __fmul_rn(scale, inv_sqrt_d<D>());
+  return scale;
+}
+
+// x = sqrt(D)^rounds R^T y in place, for 16 f32 rows; the first transform takes
+// PARTS bfloats a value, and may have been done already (first = false).
 template <int D, int PARTS>
 __device__ __forceinline__ void rotate_back(const Cache &c, float (&y)[2][D / 4], bool first) {
-  float scale = 1.0f;
   for (int r = c.rounds - 1; r >= 0; r--) {
     if (first || r != c.rounds - 1) hadamard_f32<D, PARTS>(y, Hadamard::make<true>());
     apply_signs<D>(c, r, y);
-    scale = __fmul_rn(scale, inv_sqrt_d<D>());
-  }
-#pragma unroll
-  for (int j = 0; j < D / 4; j++) {
-    y[0][j] = __fmul_rn(y[0][j], scale);
-    y[1][j] = __fmul_rn(y[1][j], scale);
   }
 }
 
