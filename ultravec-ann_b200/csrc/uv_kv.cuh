@@ -305,11 +305,12 @@ __device__ __forceinline__ void rotate_rows(const Cache &c, uint32_t (&a)[2][D /
     hadamard_f32<D, 3>(y, Hadamard::make<true>());
     scale = __fmul_rn(scale, inv_sqrt_d<D>());
   }
-  if (!SCALE) return;
+  if constexpr (SCALE) {
 #pragma unroll
   for (int j = 0; j < D / 4; j++)
 #pragma unroll
     for (int r = 0; r < ROWS; r++) y[r][j] = __fmul_rn(y[r][j], scale);
+  }
 }
 
 // sqrt(D)^-rounds
