@@ -5,20 +5,28 @@
 // j <= i + (keys - queries).  out = softmax(scale q k^T) v, a row that sees
 // nothing is zero.
 //
-// A block holds two tiles of 128 query rows that share their keys: two heads of
-// a group, or 256 consecutive rows where the group is odd.  Per 128 keys and
-// tile: S = Q K^T into TMEM (tcgen05, M = N = 128), a warpgroup with one row a
-// thread takes S into registers (maximum, exponentials and sum without any
-// shuffle), writes P back over S, and O += P V takes P from TMEM.  While one
-// tile is in its softmax the tensor core works for the other.
+// A tile is 128 query rows of one head.  Per 128 keys: S = Q K^T into TMEM
+// (tcgen05, M = N = 128), a warpgroup with one row a thread takes S into
+// registers (exponentials and sums without any shuffle), writes P back over S, and
+// O += P V takes P from TMEM, its first 64 keys while the exponentials of the
+// others still run.  Two tiles share an SM: while one is in its softmax the tensor
+// core works for the other.  At D = 128 they are one block's, with the same keys
+// (two heads of a group, or 256 consecutive rows where the group is odd); at
+// D = 64 two blocks', each of which starts and writes out while the other works.
+// One long prompt of D = 128 (8192 tokens, 32 heads) takes 562 us in the first form
+// and 640 in the second, which has room for one tile of keys and one of values;
+// 48 short texts of D = 64 take 66 and 49 us.
 //
-//   warps 0-3, 4-7   softmax and output of the two tiles
-//   warp 8           issues the products (one lane), owns the TMEM
-//   warp 9           loads Q, K, V by TMA (one lane)
-//   warps 10, 11     mend the values of blocks with masked keys (below)
+//   warps 0-3 (, 4-7)  softmax and output of a tile
+//   the next one       issues the products, owns the TMEM
+//   the next one       loads Q, K, V by TMA (one lane)
+//   the next two       mend the values of blocks with masked keys (below)
 //
-// Blocks of keys go from the last, masked ones to the first.  O is rescaled
-// only when a row's maximum grows by more than 2^8, in TMEM by its own warp.
+// Blocks of keys go from the last, masked ones to the first.  A row's weights
+// stand against a reference, the maximum of the first keys that it sees, and no
+// maximum is taken after that: as long as the sums of its weights stay below
+// 2^14 the reference serves as well.  Where one does not, the row takes a new
+// reference and its warp rescales O in TMEM.
 //
 // What a row does not see must not reach it, but a weight of zero times a value
 // of infinity or NaN is a NaN.  So in blocks with a masked key such values are
@@ -39,8 +47,7 @@
 namespace uvb {
 namespace prompt {
 
-constexpr int kRows = 128, kKeys = 128, kSlots = 5;
-constexpr int kSoftmaxWarps = 8, kThreads = 32 * (kSoftmaxWarps + 4);
+constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // 2^f on [-1/2, 1/2], relative error below 2.7e-6: a least-squares fit of the relative
 // error with weights that drive it to its minimax, made for this file
@@ -207,11 +214,18 @@ __device__ __forceinline__ constexpr uint32_t idesc(int M, int N, bool bf16, boo
 
 template <int D>
 struct Shape {
-  static constexpr int kTile = 128 * D * 2;  // bytes of 128 rows
-  static constexpr int kQ = 0, kRing = 2 * kTile, kOdd = kRing + kSlots * kTile;
+  static constexpr int kTiles = D == 128 ? 2 : 1, kBlocks = 3 - kTiles;  // blocks an SM
+  static constexpr int kSoftmaxWarps = 4 * kTiles, kThreads = 32 * (kSoftmaxWarps + 4);
+  static constexpr int kSlots = kTiles == 2 ? 5 : 4;  // tiles of keys and values in turn
+  static constexpr int kTile = 128 * D * 2;           // bytes of 128 rows
+  static constexpr int kQ = 0, kRing = kTiles * kTile, kOdd = kRing + kSlots * kTile;
   static constexpr int kBars = kOdd + 3 * D * 4;
   static constexpr int kBytes = kBars + 256;
-  static constexpr int kO = 256;  // TMEM: S of both tiles, then O of both
+  // TMEM: S (then P) of the tiles, then their O
+  static constexpr int kO = 128 * kTiles, kColumns = 256 * kTiles;
+  // Registers of the softmax warps and of the others: they add up to what the
+  // block was launched with (8 x 232 + 4 x 40 = 12 x 168, 4 x 208 + 4 x 48 = 8 x 128).
+  static constexpr int kMore = kTiles == 2 ? 232 : 208, kLess = kTiles == 2 ? 40 : 48;
 };
 
 // What a block works on.
@@ -226,10 +240,16 @@ __device__ __forceinline__ int limit(const Args &a, const Item &it, int row) {
   return a.causal ? max(0, min(it.nk, row + it.nk - it.nq + 1)) : it.nk;
 }
 
+// A block's tiles are two heads of a group, or consecutive rows of one head.
+template <int TILES>
+__host__ __device__ __forceinline__ bool pairs_heads(const Args &a) {
+  return TILES == 2 && a.q_heads / a.heads % 2 == 0;
+}
+
+template <int TILES>
 __device__ __forceinline__ bool find_item(const Args &a, Item *it) {
-  const int group = a.q_heads / a.heads;
-  const bool twins = group % 2 == 0;  // two heads of a group, or two tiles of rows
-  const int rows = twins ? kRows : 2 * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
+  const bool twins = pairs_heads<TILES>(a);
+  const int rows = twins ? kRows : TILES * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
   const int64_t tiles = a.rows_q / rows + a.n;
   // the last tiles, which see the most keys, start first
   const int64_t u = tiles - 1 - blockIdx.x / heads;
@@ -249,7 +269,7 @@ __device__ __forceinline__ bool find_item(const Args &a, Item *it) {
   it->nk = max(0, bounded(a.starts_k[lo + 1], a.rows_k) - it->k0);
   int first = INT_MAX;
   it->n = 0;
-  for (int t = 0; t < 2; t++) {
+  for (int t = 0; t < TILES; t++) {
     it->head[t] = twins ? 2 * h + t : h;
     it->i0[t] = (int)i0 + (twins ? 0 : t * kRows);
     it->blocks[t] = 0;
@@ -265,11 +285,12 @@ __device__ __forceinline__ bool find_item(const Args &a, Item *it) {
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     prompt_kernel(const Args a, const __grid_constant__ CUtensorMap qmap,
                   const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap) {
   using L = Shape<D>;
+  constexpr int kTiles = L::kTiles, kSlots = L::kSlots, kSoftmaxWarps = L::kSoftmaxWarps;
   extern __shared__ __align__(1024) uint8_t sm[];
   int(*odd)[D] = (int(*)[D])(sm + L::kOdd);  // the first key whose value is NaN, +inf, -inf
   uint64_t *bars = (uint64_t *)(sm + L::kBars);
@@ -280,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
 
   Item it;
-  if (!find_item(a, &it)) return;
+  if (!find_item<kTiles>(a, &it)) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kv_head = it.head[0] / (a.q_heads / a.heads);
 
@@ -295,25 +316,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&kv_full[i], 1);
       tc::mbar_init(&kv_empty[i], 1);
     }
-    for (int i = 0; i < 4; i++) tc::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
+    for (int i = 0; i < 4; i++) tc::mbar_init(&p_ready[i], 4);
     tc::mbar_init(mended, 64);
     tc::mbar_init(drained, 1);
     *abort_s = 0;
     tc::mbar_fence_init();
   }
-  for (int i = tid; i < 3 * D; i += kThreads) odd[i / D][i % D] = INT_MAX;
-  if (warp == kSoftmaxWarps) tc::tmem_alloc(tmem_s, 512);
+  for (int i = tid; i < 3 * D; i += L::kThreads) odd[i / D][i % D] = INT_MAX;
+  if (warp == kSoftmaxWarps) {
+    tc::tmem_alloc(tmem_s, L::kColumns);
+    tc::tmem_relinquish();
+  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_s;
   const int n = it.n, flagged = max(0, n - it.whole);
 
-  // Registers: 8 warps x 32 x 232 + 4 x 32 x 40 = 64512 = 384 x 168, what the
-  // block was launched with.
   if (warp < kSoftmaxWarps) {
     // ================= softmax: thread = row =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kMore));
     const int t = warp >> 2, row = it.i0[t] + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
@@ -479,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
     tc::tc_fence_before();
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLess));
   }
   if (warp == kSoftmaxWarps) {
     // ================= products =================
@@ -493,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t q_desc = tc::sw128_desc(q_base), k_desc = tc::sw128_desc(q_base + L::kRing);
     const uint64_t v_desc = sw128_desc_n(q_base + L::kRing, 128 * 128);
     const int nu = uniform(n), whole = uniform(it.whole);
-    const int nb[2] = {(int)uniform(it.blocks[0]), (int)uniform(it.blocks[1])};
+    const int nb[2] = {(int)uniform(it.blocks[0]), kTiles == 2 ? (int)uniform(it.blocks[1]) : 0};
     bool ok = true;
     auto wait = [&](uint64_t *bar, int phase) {
       if (ok) ok = __all_sync(0xffffffffu, wait_for(bar, phase));
@@ -508,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       bool have_k = false;
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
+      for (int t = 0; t < kTiles; t++) {
         if (j < nb[t]) {
           const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
 #pragma unroll
@@ -558,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kSoftmaxWarps + 1) {
     if (lane == 0) {
       // ================= loads =================
-      for (int t = 0; t < 2; t++) {
+      for (int t = 0; t < kTiles; t++) {
         if (it.blocks[t] == 0) continue;
         tc::mbar_arrive_expect_tx(&q_full[t], L::kTile);
         for (int x = 0; x < D; x += 64)
@@ -580,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*abort_s) {  // no copy may land after the block is gone
         for (int64_t k = issued > kSlots ? issued - kSlots : 0; k < issued; k++)
           wait_for(&kv_full[k % kSlots], (int)(k / kSlots));
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < kTiles; t++)
           if (it.blocks[t] > 0) wait_for(&q_full[t], 0);
       }
     }
@@ -630,8 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == kSoftmaxWarps) {
     tc::tc_fence_after();
-    tc::tmem_relinquish();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(tmem, L::kColumns);
   }
 }
 
@@ -675,14 +696,15 @@ static cudaError_t launch_d(const Args &a, cudaStream_t st) {
              !tile_map(&v, a.v, a.rows_k, a.heads, D, BF16)) {
     return cudaErrorInvalidValue;
   }
-  const bool twins = (a.q_heads / a.heads) % 2 == 0;
-  const int64_t grid = twins ? ((int64_t)a.rows_q / kRows + a.n) * (a.q_heads / 2)
-                             : ((int64_t)a.rows_q / (2 * kRows) + a.n) * a.q_heads;
+  using L = Shape<D>;
+  const int64_t grid = pairs_heads<L::kTiles>(a)
+                           ? ((int64_t)a.rows_q / kRows + a.n) * (a.q_heads / 2)
+                           : ((int64_t)a.rows_q / (L::kTiles * kRows) + a.n) * a.q_heads;
   if (grid > INT_MAX) return cudaErrorInvalidValue;
   const cudaError_t e = cudaFuncSetAttribute(
-      prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kBytes);
+      prompt_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return e;
-  prompt_kernel<D, BF16><<<(unsigned)grid, kThreads, Shape<D>::kBytes, st>>>(a, q, k, v);
+  prompt_kernel<D, BF16><<<(unsigned)grid, L::kThreads, L::kBytes, st>>>(a, q, k, v);
   return cudaGetLastError();
 }
 
