@@ -2,6 +2,8 @@
 // the attention over prompts: argument checks and launches.  Every buffer is
 // the caller's device memory; nothing here waits for the device except
 // uv_kv_check.
+#include <cfloat>
+
 #include "capi_internal.h"
 #include "uv_prompt.h"
 
@@ -295,6 +297,7 @@ int uv_kv_attend(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int3
   UV_TRY(typed(dtype));
   if (most < 1 || q_heads < 1 || q_heads % kv->kv_heads != 0)
     return fail(UV_EINVAL, "q_heads must be a multiple of kv_heads, most at least 1");
+  if (!(scale > 0.0f) || scale > FLT_MAX) return fail(UV_EINVAL, "scale must be positive");
   if (n == 0 || rows == 0) return UV_OK;
   UV_TRY(operand(q, q_row, q_head, kv->device, "q", &a.q));
   UV_TRY(dense(out, kv->device, "out"));
@@ -339,6 +342,7 @@ int uv_prompt_attention(int32_t device, const int32_t *starts_q, const int32_t *
   if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 || q_heads > 65535)
     return fail(UV_EINVAL, "q_heads must be a multiple of kv_heads");
   UV_TRY(typed(dtype));
+  if (!(scale > 0.0f) || scale > FLT_MAX) return fail(UV_EINVAL, "scale must be positive");
   if (n == 0 || rows_q == 0) return UV_OK;
   prompt::Args a;
   UV_TRY(on_device(starts_q, device, "starts_q"));
