@@ -83,6 +83,31 @@ def test_random_calls(uv, page, n_pages, seed):
     c.check()
 
 
+def test_more_entries_than_threads(uv):
+    """Over 1024 sequences in a call: shared last pages, long and short growth."""
+    c, m = make(uv, 9000, 2600, 300, 1, 32, heads=1)
+    pool = c.pool.cpu().numpy().copy()
+    rng = np.random.default_rng(1)
+    a, b = np.arange(1300), np.arange(1300, 2600)
+    for step, most in enumerate((50, 2, 180)):
+        n = rng.integers(0, most, 1300)
+        c.extend(ints(a), ints(n))
+        assert m.extend(a, n)
+        same(c, m, pool)
+        if step == 0:
+            c.fork(ints(a), ints(b))
+            m.fork(a, b)
+    both = rng.permutation(2600)
+    n = rng.integers(0, 3, 2600)
+    c.extend(ints(both), ints(n))
+    assert m.extend(both, n)
+    same(c, m, pool)
+    c.truncate(ints(both), ints(m.lens[both] // 2))
+    m.truncate(both, m.lens[both] // 2)
+    same(c, m, pool)
+    c.check()
+
+
 def test_beams_copy_a_shared_last_page_and_nothing_else(uv):
     c, m = make(uv)
     pool = c.pool.cpu().numpy().copy()

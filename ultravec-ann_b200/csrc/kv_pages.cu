@@ -76,38 +76,32 @@ __global__ void __launch_bounds__(kThreads) alloc_kernel(Cache c, const int32_t 
   const int per = (n + kThreads - 1) / kThreads;
   const int lo = min((int)threadIdx.x * per, n), hi = min(lo + per, n);
   // what every entry needs: pages in the low half, copies in the high half
+  auto wants = [&](int i, int *bad) -> int64_t {
+    const int s = seqs[i], m = more[i];
+    if (s < 0 || s >= c.max_seqs || m < 0 || (COPY && m >= c.max_seqs)) {
+      *bad |= kBadSeq;
+      return 0;
+    }
+    const int len = c.length(s);
+    if (COPY) {
+      if (len != 0) *bad |= kNotEmpty;
+      const int64_t pages = pages_for(c.length(m), page);
+      return pages << 32 | pages;
+    }
+    if ((int64_t)len + m > (int64_t)c.max_pages * page) {
+      *bad |= kTooLong;
+      return 0;
+    }
+    const int have = pages_for(len, page);
+    const int cow = m > 0 && len % page != 0 && c.refs[c.page_at(s, have - 1)] > 1;
+    return pages_for((int64_t)len + m, page) - have + cow + ((int64_t)cow << 32);
+  };
   int64_t need = 0;
   int bad = 0;
   for (int i = lo; i < hi; i++) {
     const int s = seqs[i];
-    if (s < 0 || s >= c.max_seqs) {
-      bad |= kBadSeq;
-      continue;
-    }
-    if (atomicExch(&c.mark()[s], 1) != 0) bad |= kBadSeq;
-    const int len = c.length(s), have = pages_for(len, page);
-    if (COPY) {
-      const int from = more[i];
-      if (from < 0 || from >= c.max_seqs) {
-        bad |= kBadSeq;
-        continue;
-      }
-      if (len != 0) bad |= kNotEmpty;
-      const int64_t pages = pages_for(c.length(from), page);
-      need += pages << 32 | pages;
-    } else {
-      const int count = more[i];
-      if (count < 0) {
-        bad |= kBadSeq;
-        continue;
-      }
-      if ((int64_t)len + count > (int64_t)c.max_pages * page) {
-        bad |= kTooLong;
-        continue;
-      }
-      const int cow = count > 0 && len % page != 0 && c.refs[c.page_at(s, have - 1)] > 1;
-      need += pages_for((int64_t)len + count, page) - have + cow + ((int64_t)cow << 32);
-    }
+    if (s >= 0 && s < c.max_seqs && atomicExch(&c.mark()[s], 1) != 0) bad |= kBadSeq;
+    need += wants(i, &bad);
   }
   if (bad) atomicOr(&errors, bad);
   int64_t total2;
@@ -159,49 +153,27 @@ __global__ void __launch_bounds__(kThreads) alloc_kernel(Cache c, const int32_t 
     return;
   }
   // Each entry's place among the fresh pages and the moves (the counts are
-  // still those of the check, so it is the same sum again); the pages go out
-  // by warps, so that one long prompt does not keep one thread busy.
+  // still those of the check, so it is the same sum again).  A thread serves its
+  // entries itself where they take a page or so each; long ones go out by warps,
+  // so that one prompt does not keep one thread busy.
+  const bool short_ones = per == 1 && total <= 4 * (int64_t)n;
   int released = 0;
-  for (int i = lo; i < hi; i++) {
+  auto serve = [&](int i, int64_t at, int64_t want, int first, int step) {
     const int s = seqs[i], len = c.length(s), have = pages_for(len, page);
-    c.offset()[i] = (int)(off2 & 0xffffffffll);
-    if (COPY) {
-      const int64_t pages = pages_for(c.length(more[i]), page);
-      off2 += pages << 32 | pages;
-    } else {
-      int cow = 0;
-      if (more[i] > 0 && len % page != 0) cow = c.refs[c.page_at(s, have - 1)] > 1;
-      c.mark()[i] = cow | (int)((off2 >> 32) << 1);
-      off2 += pages_for((int64_t)len + more[i], page) - have + cow + ((int64_t)cow << 32);
-    }
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = warp; i < n; i += kThreads / 32) {
-    const int s = seqs[i], len = c.length(s), have = pages_for(len, page);
-    const int off = c.offset()[i];
+    const int off = (int)(at & 0xffffffffll), take = (int)(want & 0xffffffffll);
+    const int cow = COPY ? 0 : (int)(want >> 32);
     int32_t *row = c.table + (int64_t)s * c.max_pages;
-    int take, column, cow = 0;
-    if (COPY) {
-      take = pages_for(c.length(more[i]), page);
-      column = 0;
-    } else {
-      const int m = c.mark()[i];
-      cow = m & 1;
-      take = pages_for((int64_t)len + more[i], page) - have + cow;
-      column = have - cow;
-      if (cow && lane == 0) {
-        const int old = c.page_at(s, have - 1);
-        c.move_src()[m >> 1] = old;
-        c.move_dst()[m >> 1] = fresh[off];
-        if (atomicSub(&c.refs[old], 1) == 1) {
-          released++;
-          atomicMin(&next_hint, old);
-        }
+    const int column = COPY ? 0 : have - cow;
+    if (cow && first == 0) {
+      const int old = c.page_at(s, column), move = (int)(at >> 32);
+      c.move_src()[move] = old;
+      c.move_dst()[move] = fresh[off];
+      if (atomicSub(&c.refs[old], 1) == 1) {
+        released++;
+        atomicMin(&next_hint, old);
       }
-      __syncwarp();
     }
-    for (int j = lane; j < take; j += 32) {
+    for (int j = first; j < take; j += step) {
       const int p = fresh[off + j];
       if (COPY) {
         c.move_src()[off + j] = c.page_at(more[i], j);
@@ -210,12 +182,35 @@ __global__ void __launch_bounds__(kThreads) alloc_kernel(Cache c, const int32_t 
       row[column + j] = p;
       c.refs[p] = 1;
     }
-    __syncwarp();
-    if (lane == 0) c.lens[s] = COPY ? c.length(more[i]) : len + more[i];
+    return COPY ? c.length(more[i]) : len + more[i];
+  };
+  if (short_ones) {
+    if (lo < hi) c.lens[seqs[lo]] = serve(lo, off2, need, 0, 1);
+  } else {
+    int ignore = 0;
+    for (int i = lo; i < hi; i++) {
+      const int64_t want = per == 1 ? need : wants(i, &ignore);
+      c.offset()[i] = (int)(off2 & 0xffffffffll);
+      c.mark()[i] = (int)(off2 >> 32) << 1 | (COPY ? 0 : (int)(want >> 32));
+      off2 += want;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = warp; i < n; i += kThreads / 32) {
+      const int s = seqs[i], len = c.length(s), have = pages_for(len, page), m = c.mark()[i];
+      const int cow = m & 1;
+      const int take = COPY ? pages_for(c.length(more[i]), page)
+                            : pages_for((int64_t)len + more[i], page) - have + cow;
+      const int now = serve(i, (int64_t)(m >> 1) << 32 | (uint32_t)c.offset()[i],
+                            (int64_t)cow << 32 | take, lane, 32);
+      __syncwarp();
+      if (lane == 0) c.lens[s] = now;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) c.mark()[i] = 0;
   }
   if (released) atomicSub(&c.work[kUsed], released);
   __syncthreads();
-  for (int i = threadIdx.x; i < c.max_seqs && i < n; i += kThreads) c.mark()[i] = 0;
   if (threadIdx.x == 0) {
     c.work[kUsed] += (int)total;
     if (total > 0) {
@@ -276,9 +271,9 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(Cache c, int fix) {
 // ---- fork and truncate ----
 // One cluster: block 0 checks the entries, the others read its verdict
 // through shared memory, then all warps share the entries' table columns in
-// groups of 32.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
-    fork_kernel(Cache c, const int32_t *src, const int32_t *dst, const int32_t *lens, int n) {
+// groups of 32.  One block does where each of its warps has one group at most
+// (128 groups take 9.4 us in one block, 7.2 in a cluster of eight).
+__global__ void __launch_bounds__(kThreads) fork_kernel(Cache c, const int32_t *src, const int32_t *dst, const int32_t *lens, int n) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ int errors;
@@ -312,7 +307,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 31;
   const int warp = cluster.block_rank() * (kThreads / 32) + (threadIdx.x >> 5);
   const int groups = (c.max_pages + 31) / 32;
-  for (int64_t u = warp; u < (int64_t)n * groups; u += kCluster * (kThreads / 32)) {
+  for (int64_t u = warp; u < (int64_t)n * groups; u += (int64_t)cluster.num_blocks() * (kThreads / 32)) {
     const int i = (int)(u % n), col = (int)(u / n) * 32 + lane;
     const int s = src[i], d = dst[i];
     int len = c.length(s);
@@ -326,8 +321,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
   }
 }
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
-    truncate_kernel(Cache c, const int32_t *seqs, const int32_t *lens, int n) {
+__global__ void __launch_bounds__(kThreads) truncate_kernel(Cache c, const int32_t *seqs, const int32_t *lens, int n) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ int errors, released, low;
@@ -358,7 +352,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
   const int warp = cluster.block_rank() * (kThreads / 32) + (threadIdx.x >> 5);
   const int groups = (c.max_pages + 31) / 32;
   int freed = 0, least = c.n_pages;
-  for (int64_t u = warp; u < (int64_t)n * groups; u += kCluster * (kThreads / 32)) {
+  for (int64_t u = warp; u < (int64_t)n * groups; u += (int64_t)cluster.num_blocks() * (kThreads / 32)) {
     const int s = seqs[u % n], i = (int)(u % n), col = (int)(u / n) * 32 + lane;
     const int len = c.length(s), keep = lens != nullptr ? min(lens[i], len) : 0;
     if (col >= pages_for(keep, c.page_tokens) && col < pages_for(len, c.page_tokens)) {
@@ -377,7 +371,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
   // The lengths change after every warp of the cluster has read them.
   cluster.sync();
   for (int64_t i = (int64_t)cluster.block_rank() * kThreads + threadIdx.x; i < n;
-       i += kCluster * kThreads) {
+       i += (int64_t)cluster.num_blocks() * kThreads) {
     const int s = seqs[i], len = c.length(s);
     c.lens[s] = lens != nullptr ? min(lens[i], len) : 0;
   }
@@ -465,15 +459,29 @@ cudaError_t copy_launch(const Cache &c, const int32_t *src, const int32_t *dst, 
   const cudaError_t e = cudaGetLastError();
   return e != cudaSuccess ? e : move_launch(c, 0, sms, st);
 }
+template <class... P, class... A>
+static cudaError_t cluster_launch(void (*kernel)(P...), const Cache &c, int n, cudaStream_t st,
+                                  A... args) {
+  const int blocks = (int64_t)n * ((c.max_pages + 31) / 32) <= kThreads / 32 ? 1 : kCluster;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = blocks;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, c, args..., n);
+}
 cudaError_t fork_launch(const Cache &c, const int32_t *src, const int32_t *dst,
                         const int32_t *lens, int n, cudaStream_t st) {
-  fork_kernel<<<kCluster, kThreads, 0, st>>>(c, src, dst, lens, n);
-  return cudaGetLastError();
+  return cluster_launch(fork_kernel, c, n, st, src, dst, lens);
 }
 cudaError_t truncate_launch(const Cache &c, const int32_t *seqs, const int32_t *lens, int n,
                             cudaStream_t st) {
-  truncate_kernel<<<kCluster, kThreads, 0, st>>>(c, seqs, lens, n);
-  return cudaGetLastError();
+  return cluster_launch(truncate_kernel, c, n, st, seqs, lens);
 }
 cudaError_t compact_launch(const Cache &c, int sms, cudaStream_t st) {
   compact_kernel<<<1, kThreads, 0, st>>>(c);

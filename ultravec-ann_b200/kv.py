@@ -130,16 +130,18 @@ class KvCache:
         if tiles * TILE != page_tokens or width != TILE * (head_dim + 8):
             raise ValueError(f"the pool's pages do not have the shape of {page_tokens} tokens of "
                              f"{head_dim} dimensions")
-        s = signs.tolist()
-        if not 1 <= len(s) <= 3 or any(len(r) != head_dim for r in s):
+        import numpy as np
+
+        s = signs.cpu().numpy() if hasattr(signs, "cpu") else np.asarray(signs)
+        if s.ndim != 2 or not 1 <= s.shape[0] <= 3 or s.shape[1] != head_dim:
             raise ValueError("signs must be 1 to 3 rounds of head_dim values")
+        if not (np.abs(s) == 1).all():
+            raise ValueError("signs must be +1 or -1")
         desc = uv_kv(pool.device.index or 0, head_dim, heads, layers, page_tokens, pages,
-                     table.shape[0], table.shape[1], len(s))
-        for r, row in enumerate(s):
-            for i, x in enumerate(row):
-                if x not in (1, -1):
-                    raise ValueError("signs must be +1 or -1")
-                desc.signs[r][i // 32] |= (x < 0) << (i % 32)
+                     table.shape[0], table.shape[1], s.shape[0])
+        bits = np.packbits(s < 0, axis=1, bitorder="little").view(np.uint32)
+        for r, row in enumerate(bits):
+            desc.signs[r][:len(row)] = row.tolist()
         self = cls.__new__(cls)
         self._attach(desc, pool, table, lens, refs)
         check(self._lib.uv_kv_recount(self._p, _raw_stream(self._index)))
