@@ -35,8 +35,13 @@
 // output.
 //
 // Bound: per 128 x 128 tile and D = 128 the two products take 1024 cycles of
-// the tensor core and the exponentials 1024 of the MUFU (16 a cycle), so part of
-// the exponentials is computed by a polynomial in the FMA pipe instead.
+// the tensor core, the exponentials 1024 of the MUFU (16 a cycle) if it computes
+// them all (a quarter goes to a polynomial in the FMA pipe), and their arguments,
+// sums and packing about as many issue cycles.  A tile's chain (scores, 128
+// exponentials a thread at about 7 cycles, product) takes 2300 cycles with the
+// other tile beside it, so 3500 pass for two tiles, of which the tensor core
+// works 2048: 980 TFLOP/s for 8192 tokens and 32 heads (0.56 ms), at the 1.4 GHz
+// that the power limit then leaves.
 #include <cfloat>
 #include <climits>
 #include <cuda.h>
@@ -246,27 +251,14 @@ __host__ __device__ __forceinline__ bool pairs_heads(const Args &a) {
   return TILES == 2 && a.q_heads / a.heads % 2 == 0;
 }
 
+// Fills in the tiles of rows i0 .. of entry b.
 template <int TILES>
-__device__ __forceinline__ bool find_item(const Args &a, Item *it) {
+__device__ __forceinline__ void describe(const Args &a, int b, int64_t i0, int h, Item *it) {
   const bool twins = pairs_heads<TILES>(a);
-  const int rows = twins ? kRows : TILES * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
-  const int64_t tiles = a.rows_q / rows + a.n;
-  // the last tiles, which see the most keys, start first
-  const int64_t u = tiles - 1 - blockIdx.x / heads;
-  const int h = blockIdx.x % heads;
-  // entry b has starts_q[b + 1] / rows - starts_q[b] / rows + 1 tiles
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (bounded(a.starts_q[mid], a.rows_q) / rows + mid <= u) lo = mid;
-    else hi = mid - 1;
-  }
-  it->q0 = bounded(a.starts_q[lo], a.rows_q);
-  it->nq = bounded(a.starts_q[lo + 1], a.rows_q) - it->q0;
-  const int64_t i0 = (u - (it->q0 / rows + lo)) * rows;
-  if (i0 < 0 || i0 >= it->nq) return false;
-  it->k0 = bounded(a.starts_k[lo], a.rows_k);
-  it->nk = max(0, bounded(a.starts_k[lo + 1], a.rows_k) - it->k0);
+  it->q0 = bounded(a.starts_q[b], a.rows_q);
+  it->nq = bounded(a.starts_q[b + 1], a.rows_q) - it->q0;
+  it->k0 = bounded(a.starts_k[b], a.rows_k);
+  it->nk = max(0, bounded(a.starts_k[b + 1], a.rows_k) - it->k0);
   int first = INT_MAX;
   it->n = 0;
   for (int t = 0; t < TILES; t++) {
@@ -281,6 +273,84 @@ __device__ __forceinline__ bool find_item(const Args &a, Item *it) {
     it->n = max(it->n, it->blocks[t]);
   }
   it->whole = first / kKeys;
+}
+
+// One warp's search for the block's work.  Tiles go in the order of their key
+// blocks, most first, so that no long one is left for the end: how many tiles of
+// an entry have c blocks or more is a division, so the u-th tile is a binary
+// search over c, with the entries over the lanes.  (One sequence of 6000 tokens
+// ahead of 90 of 300, 8 heads of 128: 211 us in the order of the pack, from its
+// end, 200 so.)  Past 128 entries the order is the pack's.
+template <int TILES>
+__device__ __forceinline__ bool find_item(const Args &a, Item *it) {
+  constexpr int kEach = 4;
+  const bool twins = pairs_heads<TILES>(a);
+  const int rows = twins ? kRows : TILES * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
+  const int64_t u = blockIdx.x / heads;
+  const int h = blockIdx.x % heads, lane = threadIdx.x & 31;
+  if (a.n > 32 * kEach) {
+    // entry b has starts_q[b + 1] / rows - starts_q[b] / rows + 1 tiles
+    const int64_t w = (int64_t)a.rows_q / rows + a.n - 1 - u;
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (bounded(a.starts_q[mid], a.rows_q) / rows + mid <= w) lo = mid;
+      else hi = mid - 1;
+    }
+    const int q0 = bounded(a.starts_q[lo], a.rows_q);
+    const int64_t i0 = (w - (q0 / rows + lo)) * rows;
+    if (i0 < 0 || i0 >= bounded(a.starts_q[lo + 1], a.rows_q) - q0) return false;
+    if (lane == 0) describe<TILES>(a, lo, i0, h, it);
+    return true;
+  }
+  int nq[kEach], nk[kEach], most = 0;
+#pragma unroll
+  for (int s = 0; s < kEach; s++) {
+    const int b = 32 * s + lane;
+    nq[s] = nk[s] = 0;
+    if (b < a.n) {
+      nq[s] = max(0, bounded(a.starts_q[b + 1], a.rows_q) - bounded(a.starts_q[b], a.rows_q));
+      nk[s] = max(0, bounded(a.starts_k[b + 1], a.rows_k) - bounded(a.starts_k[b], a.rows_k));
+    }
+    most = max(most, (nk[s] + kKeys - 1) / kKeys);
+  }
+  // an entry's first tile whose last row sees something of key block c - 1
+  auto begin = [&](int s, int c) {
+    const int tiles = (nq[s] + rows - 1) / rows;
+    if (c == 0) return 0;
+    const int64_t x = (int64_t)(c - 1) * kKeys + (a.causal ? nq[s] - nk[s] : 0);
+    if (!a.causal) return x < nk[s] ? 0 : tiles;
+    return x >= nq[s] ? tiles : x < 0 ? 0 : (int)(x / rows);
+  };
+  auto at_least = [&](int c) {  // tiles with c blocks or more, of all entries
+    int sum = 0;
+#pragma unroll
+    for (int s = 0; s < kEach; s++) sum += (nq[s] + rows - 1) / rows - begin(s, c);
+    return (int64_t)__reduce_add_sync(0xffffffffu, sum);
+  };
+  if (u >= at_least(0)) return false;
+  int lo = 0, hi = __reduce_max_sync(0xffffffffu, most);
+  while (lo < hi) {  // the largest c with more than u tiles
+    const int mid = (lo + hi + 1) >> 1;
+    if (at_least(mid) > u) lo = mid;
+    else hi = mid - 1;
+  }
+  int v = (int)(u - at_least(lo + 1));  // among the tiles with exactly c blocks
+#pragma unroll
+  for (int s = 0; s < kEach; s++) {
+    const int from = begin(s, lo), count = begin(s, lo + 1) - from;
+    int before = count;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    const int sum = __shfl_sync(0xffffffffu, before, 31);
+    before -= count;
+    if (v >= before && v < before + count)
+      describe<TILES>(a, 32 * s + lane, (int64_t)(from + v - before) * rows, h, it);
+    v -= sum;
+    if (v < 0) break;
+  }
   return true;
 }
 
@@ -300,9 +370,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
   uint32_t *tmem_s = (uint32_t *)(drained + 1);
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
 
-  Item it;
-  if (!find_item<kTiles>(a, &it)) return;
+  __shared__ Item item;
+  __shared__ bool found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == 0) {
+    const bool some = find_item<kTiles>(a, &item);
+    if (lane == 0) found = some;
+  }
+  __syncthreads();
+  if (!found) return;
+  const Item it = item;
   const int kv_head = it.head[0] / (a.q_heads / a.heads);
 
   if (tid == 0) {

@@ -13,7 +13,7 @@
 // a row of the A operand whose K order is free, so a lane takes a quarter of a
 // row as it lies; for the values A is transposed (rows are dimensions, K is
 // the token), a half2 holds two tokens, and the interleaved granules give a
-// lane one 32-bit word with 4 dimensions of both, so the same three
+// lane one 32-bit word with 4 dimensions of both, so the same
 // instructions unpack both.  A token never shares a byte pair with another:
 // rows are written without reading their neighbours.
 //
