@@ -625,7 +625,8 @@ int uv_kv_compact(const uv_kv *kv, void *stream);
 /* The last rows of sequences, packed: seqs[b] owns rows [starts[b],
  * starts[b + 1]) (one each when starts is NULL), its last tokens in order.
  * Element [row][head][i] of an input is at row * row_stride + head *
- * head_stride + i; strides are multiples of 8, bases 16-byte aligned.
+ * head_stride + i; strides are multiples of 8, bases 16-byte aligned.  The
+ * starts rise from 0 to rows.
  * append writes them (extend has made the room); read returns them as they are
  * held, dense (rows without a token as zeros). */
 int uv_kv_append(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int32_t *starts,

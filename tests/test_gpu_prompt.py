@@ -148,6 +148,44 @@ def test_strides_streams_and_repeats(uv):
     assert torch.equal(want, got)
 
 
+def test_one_row_one_head_and_broadcast_heads(uv):
+    import torch
+
+    rng = np.random.default_rng(9)
+    q, k, v = (rows(rng, n, 1, 64, "float16") for n in (1, 300, 300))
+    out, lse = uv.prompt_attention(q, k, v, starts([1]), starts([300]), lse=True)
+    compare(out, lse, q, k, v, [1], [300], True, "float16", 0.125)
+    q = rows(rng, 40, 4, 64, "float16")
+    k, v = (rows(rng, 40, 1, 64, "float16") for _ in range(2))
+    wide = uv.prompt_attention(q, k.expand(-1, 2, -1), v.expand(-1, 2, -1), starts([40]))
+    assert torch.equal(wide, uv.prompt_attention(q, k, v, starts([40])))
+    st = torch.cuda.current_stream().cuda_stream
+    n = starts([40]).data_ptr()
+    out = torch.empty_like(q)
+    for strides in ((0, 64), (256, 0), (3, 64), (-256, 64)):
+        rc = uv.lib().uv_prompt_attention(0, n, None, 1, 40, 40, 4, 4, 64, 1, 0.125, 0, q.data_ptr(), *strides,
+                                          q.data_ptr(), 256, 64, q.data_ptr(), 256, 64, out.data_ptr(), None, st)
+        assert rc == 1, strides
+
+
+@pytest.mark.parametrize("n", [1, 33, 150])
+def test_many_sequences_of_every_length(uv, n):
+    """Entries over all lanes, and more than the ordered search takes."""
+    rng = np.random.default_rng(n)
+    nq = [int(x) for x in rng.integers(0, 200, n)]
+    nk = [x + int(y) for x, y in zip(nq, rng.integers(0, 150, n))]
+    nq[0], nk[0] = 130, 400
+    q, k, v = rows(rng, sum(nq), 2, 64, "bfloat16"), rows(rng, sum(nk), 1, 64, "bfloat16"), rows(rng, sum(nk), 1, 64, "bfloat16")
+    for causal in (True, False):
+        out, lse = uv.prompt_attention(q, k, v, starts(nq), starts(nk), causal=causal, lse=True)
+        a = np.concatenate([[0], np.cumsum(nq)])
+        b = np.concatenate([[0], np.cumsum(nk)])
+        for i in list(range(min(n, 4))) + [n // 2, n - 1]:
+            x, y = slice(a[i], a[i + 1]), slice(b[i], b[i + 1])
+            compare(out[x], lse[x], q[x], k[y], v[y], [nq[i]], [nk[i]], causal, "bfloat16", 0.125)
+        assert np.isfinite(f64(out)).all()
+
+
 def test_refused_arguments(uv):
     import torch
 

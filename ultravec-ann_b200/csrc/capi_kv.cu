@@ -104,6 +104,15 @@ int operand(const void *p, int64_t row, int64_t head, int device, const char *wh
   return UV_OK;
 }
 
+// For a tensor map: a stride over one element is not read, but has to be one.
+int mapped(kv::Strided *x, int rows, int heads, int dim, const char *what) {
+  if (heads == 1) x->head = dim;
+  if (rows == 1) x->row = (int64_t)heads * x->head;
+  if (x->row == 0 || x->head == 0)
+    return fail(UV_EINVAL, std::string(what) + ": strides must be positive");
+  return UV_OK;
+}
+
 int dense(const void *p, int device, const char *what) {
   UV_TRY(on_device(p, device, what));
   if ((uintptr_t)p % 16) return fail(UV_EINVAL, std::string(what) + " must be 16-byte aligned");
@@ -353,9 +362,12 @@ int uv_prompt_attention(int32_t device, const int32_t *starts_q, const int32_t *
     UV_TRY(on_device(starts_k, device, "starts_k"));
   }
   UV_TRY(operand(q, q_row, q_head, device, "q", &a.q));
+  UV_TRY(mapped(&a.q, rows_q, q_heads, head_dim, "q"));
   if (rows_k > 0) {
     UV_TRY(operand(k, k_row, k_head, device, "k", &a.k));
     UV_TRY(operand(v, v_row, v_head, device, "v", &a.v));
+    UV_TRY(mapped(&a.k, rows_k, kv_heads, head_dim, "k"));
+    UV_TRY(mapped(&a.v, rows_k, kv_heads, head_dim, "v"));
   } else {
     a.k = a.v = {q, 0, 0};  // never read
   }
