@@ -316,6 +316,38 @@ def test_one_long_sequence_and_many_ragged_ones_split_alike(uv):
         assert (np.abs(f64(alone) - want) <= attend_tolerance(want, size, reach, "bfloat16")).all()
 
 
+@pytest.mark.parametrize("typ", ["float16", "bfloat16"])
+def test_a_long_flat_sequence(uv, typ):
+    """150,001 tokens of nearly equal weight: the outputs are 1 / 80 of a value,
+    so what the sums lose of codes that all are positive would show."""
+    import torch
+
+    n, d = 150_001, 128
+    c = uv.KvCache(d, 1, 2400, 2, n, page_tokens=64)
+    c.extend(ints([1]), ints([n]))
+    c.check()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tiles = c.pool[0]
+    half = 32 * d // 2
+    for at, size in ((0, 0.05), (half + 128, 1.0)):
+        code = (torch.randn(*tiles.shape[:-1], 32 * d, generator=g, device="cuda") / 0.3352).floor().add(8)
+        code = code.clamp(0, 15).to(torch.uint8)
+        tiles[..., at:at + half] = code[..., 0::2] | (code[..., 1::2] << 4)
+        scale = size * 0.3352 * torch.exp(0.2 * torch.randn(*tiles.shape[:-1], 32, generator=g, device="cuda"))
+        tiles[..., at + half:at + half + 128] = scale.view(torch.uint8)
+    signs = np.array([[-1.0 if c._desc.signs[0][i // 32] >> (i % 32) & 1 else 1.0 for i in range(d)]])
+    q = rows_of(np.random.default_rng(0), 2, 4, d, typ, False)
+    out = c.attend(ints([1]), q, starts([2]), 2)
+    want, _, size, reach = M.attend(f64(q), M.held(tiles.cpu().numpy(), c.table[1].cpu().numpy(), n, d),
+                                    M.rotation(signs), 1 / math.sqrt(d))
+    err = np.abs(f64(out) - want)
+    assert (err <= attend_tolerance(want, size, reach, typ)).all()
+    # the roundings of 150,000 weights are independent, so their sum is far below
+    # the bound: a tenth of the output's size would be a lost sum
+    assert np.linalg.norm(err) < 0.1 * np.linalg.norm(want)
+    c.check()
+
+
 def test_pools_beyond_32_bits_of_bytes_and_other_layers(uv):
     import torch
 

@@ -168,6 +168,20 @@ def test_one_row_one_head_and_broadcast_heads(uv):
         assert rc == 1, strides
 
 
+@pytest.mark.parametrize("d,causal", [(64, True), (128, True), (128, False)])
+def test_a_few_rows_behind_many_keys(uv, d, causal):
+    """The last rows of 70,001 tokens, whose scores climb along the sequence, so
+    that the references move again and again from the last keys to the first."""
+    import torch
+
+    rng = np.random.default_rng(d)
+    q, k, v = rows(rng, 3, 2, d, "bfloat16"), rows(rng, 70_001, 1, d, "bfloat16"), rows(rng, 70_001, 1, d, "bfloat16")
+    slope = torch.linspace(60, 0, 70_001, device="cuda")[:, None, None]
+    k = (k.float() + slope * q.float().mean(1, keepdim=True)[:1] / d).bfloat16()
+    out, lse = uv.prompt_attention(q, k, v, starts([3]), starts([70_001]), causal=causal, lse=True)
+    compare(out, lse, q, k, v, [3], [70_001], causal, "bfloat16", 1 / math.sqrt(d))
+
+
 @pytest.mark.parametrize("n", [1, 33, 150])
 def test_many_sequences_of_every_length(uv, n):
     """Entries over all lanes, and more than the ordered search takes."""
