@@ -40,7 +40,7 @@
 // sums and packing about as many issue cycles.  A tile's chain (scores, 128
 // exponentials a thread at about 7 cycles, product) takes 2300 cycles with the
 // other tile beside it, so 3500 pass for two tiles, of which the tensor core
-// works 2048: 980 TFLOP/s for 8192 tokens and 32 heads (0.56 ms), at the 1.4 GHz
+// works 2048: 980 TFLOP/s for 8192 tokens and 32 heads (0.56 ms), at the 1.69 GHz
 // that the power limit then leaves.
 #include <cfloat>
 #include <climits>
@@ -58,7 +58,12 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // error with weights that drive it to its minimax, made for this file
 constexpr float kC0 = 0.9999992847442627f, kC1 = 0.6931217908859253f, kC2 = 0.240247443318367f,
                 kC3 = 0.05591785907745361f, kC4 = 0.009570101276040077f;
-constexpr int kPoly = 2, kPolyOf = 8;  // of kPolyOf columns, kPoly take the polynomial
+// Of kPolyOf columns, kPoly take the polynomial: packed prompts take 177 us with 0,
+// 172 with 1, 170 with 2; one long prompt 522, 533 and 522, texts of D = 64 48 with any.
+constexpr int kPoly = 2, kPolyOf = 8;
+// Barriers of mended values, in turn: the ring holds at most three blocks of values whose
+// product is still to be issued, so none completes a second time before it was waited for.
+constexpr int kMends = 4;
 constexpr float kGrow = 16384.0f;  // weights (sums of 32 of them) up to this stay unanswered
 
 __device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
   uint64_t *bars = (uint64_t *)(sm + L::kBars);
   uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + kSlots;
   uint64_t *s_full = kv_empty + kSlots, *p_ready = s_full + 2, *o_done = p_ready + 4;
-  uint64_t *h_done = o_done + 2, *mended = h_done + 2, *drained = mended + 1;
+  uint64_t *h_done = o_done + 2, *mended = h_done + 2, *drained = mended + kMends;
   uint32_t *tmem_s = (uint32_t *)(drained + 1);
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
 
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       tc::mbar_init(&kv_empty[i], 1);
     }
     for (int i = 0; i < 4; i++) tc::mbar_init(&p_ready[i], 4);
-    tc::mbar_init(mended, 64);
+    for (int i = 0; i < kMends; i++) tc::mbar_init(&mended[i], 64);
     tc::mbar_init(drained, 1);
     *abort_s = 0;
     tc::mbar_fence_init();
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     const float2 ll = split(l);
     const float sum = __fadd_rn(ll.x, ll.y);
     if (blocks > 0 && ok) settle(wait_for(&o_done[t], 0));
-    if (flagged > 0 && ok) settle(wait_for(mended, flagged - 1));
+    if (flagged > 0 && ok) settle(wait_for(&mended[(flagged - 1) % kMends], (flagged - 1) / kMends));
     settle(!*abort_s);
     if (!ok) *abort_s = 1;
     tc::tc_fence_after();
@@ -603,7 +608,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     for (int j = nu; j >= 0 && ok; j--) {
       if (j < nu) {
         if (!wait(&kv_full[v_slot], v_phase)) break;
-        if (j >= whole && !wait(mended, nu - 1 - j)) break;
+        const int f = nu - 1 - j;
+        if (j >= whole && !wait(&mended[f % kMends], f / kMends)) break;
       }
       bool have_k = false;
 #pragma unroll
@@ -723,7 +729,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         }
       }
       tc::fence_async_smem();
-      tc::mbar_arrive(mended);
+      tc::mbar_arrive(&mended[f % kMends]);
     }
   }
   __syncthreads();
