@@ -79,6 +79,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Half of a transpose over lanes: a of the lane without `bit` stays, b of the one with it.
+__device__ __forceinline__ void trade(uint4 &a, uint4 &b, int bit) {
+  const bool hi = threadIdx.x & bit;
+  auto word = [&](uint32_t &x, uint32_t &y) {
+    const uint32_t z = __shfl_xor_sync(0xffffffffu, hi ? x : y, bit);
+    if (hi) x = z;
+    else y = z;
+  };
+  word(a.x, b.x);
+  word(a.y, b.y);
+  word(a.z, b.z);
+  word(a.w, b.w);
+}
+
 // ---- pairs of floats ----
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 pair(float a, float b) {
@@ -140,6 +154,47 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, int phase) {
     if (done) return true;
   }
   return false;
+}
+// A wait for another role of the block, which may itself run into the limit first.
+__device__ __forceinline__ bool wait_long(uint64_t *bar, int64_t phase) {
+  bool done = false;
+  for (int i = 0; i < 4 && !done; i++) done = wait_for(bar, phase);
+  return done;
+}
+// Asks for the index of a block that has not started, to do its work here: the
+// answer (16 bytes) arrives on `bar`.
+__device__ __forceinline__ void ask_next(void *answer, uint64_t *bar) {
+  tc::mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
+          "r"(tc::smem_u32(answer)),
+      "r"(tc::smem_u32(bar))
+      : "memory");
+}
+// The index, or -1 where none was left.
+__device__ __forceinline__ int answer_of(const void *answer) {
+  int block;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 a, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=r"(block)
+      : "r"(tc::smem_u32(answer))
+      : "memory");
+  return block;
+}
+// Whether any of the 64 threads that mend says so.
+__device__ __forceinline__ bool any_of_64(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "barrier.red.or.pred q, 1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r;
 }
 __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z,
                                             uint64_t *bar) {
@@ -230,7 +285,7 @@ struct Shape {
   static constexpr int kTile = 128 * D * 2;           // bytes of 128 rows
   static constexpr int kQ = 0, kRing = kTiles * kTile, kOdd = kRing + kSlots * kTile;
   static constexpr int kBars = kOdd + 3 * D * 4;
-  static constexpr int kBytes = kBars + 256;
+  static constexpr int kBytes = kBars + 320;
   // TMEM: S (then P) of the tiles, then their O
   static constexpr int kO = 128 * kTiles, kColumns = 256 * kTiles;
   // Registers of the softmax warps and of the others: they add up to what the
@@ -287,12 +342,12 @@ __device__ __forceinline__ void describe(const Args &a, int b, int64_t i0, int h
 // ahead of 90 of 300, 8 heads of 128: 211 us in the order of the pack, from its
 // end, 200 so.)  Past 128 entries the order is the pack's.
 template <int TILES>
-__device__ __forceinline__ bool find_item(const Args &a, Item *it) {
+__device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   constexpr int kEach = 4;
   const bool twins = pairs_heads<TILES>(a);
-  const int rows = twins ? kRows : TILES * kRows, heads = twins ? a.q_heads / 2 : a.q_heads;
-  const int64_t u = blockIdx.x / heads;
-  const int h = blockIdx.x % heads, lane = threadIdx.x & 31;
+  const int shift = !twins && TILES == 2 ? 8 : 7, rows = 1 << shift, heads = twins ? a.q_heads / 2 : a.q_heads;
+  const int64_t u = block / heads;
+  const int h = block % heads, lane = threadIdx.x & 31;
   if (a.n > 32 * kEach) {
     // entry b has starts_q[b + 1] / rows - starts_q[b] / rows + 1 tiles
     const int64_t w = (int64_t)a.rows_q / rows + a.n - 1 - u;
@@ -321,16 +376,17 @@ __device__ __forceinline__ bool find_item(const Args &a, Item *it) {
   }
   // an entry's first tile whose last row sees something of key block c - 1
   auto begin = [&](int s, int c) {
-    const int tiles = (nq[s] + rows - 1) / rows;
+    const int tiles = (nq[s] + rows - 1) >> shift;
     if (c == 0) return 0;
     const int64_t x = (int64_t)(c - 1) * kKeys + (a.causal ? nq[s] - nk[s] : 0);
     if (!a.causal) return x < nk[s] ? 0 : tiles;
-    return x >= nq[s] ? tiles : x < 0 ? 0 : (int)(x / rows);
+    return x >= nq[s] ? tiles : x < 0 ? 0 : (int)(x >> shift);
   };
   auto at_least = [&](int c) {  // tiles with c blocks or more, of all entries
     int sum = 0;
 #pragma unroll
-    for (int s = 0; s < kEach; s++) sum += (nq[s] + rows - 1) / rows - begin(s, c);
+    for (int s = 0; s < kEach; s++)
+      if (32 * s < a.n) sum += ((nq[s] + rows - 1) >> shift) - begin(s, c);
     return (int64_t)__reduce_add_sync(0xffffffffu, sum);
   };
   if (u >= at_least(0)) return false;
@@ -372,27 +428,26 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
   uint64_t *q_full = bars, *kv_full = bars + 2, *kv_empty = kv_full + kSlots;
   uint64_t *s_full = kv_empty + kSlots, *p_ready = s_full + 2, *o_done = p_ready + 4;
   uint64_t *h_done = o_done + 2, *mended = h_done + 2, *drained = mended + kMends;
-  uint32_t *tmem_s = (uint32_t *)(drained + 1);
+  uint64_t *q_empty = drained + 1, *item_full = q_empty + 2, *item_empty = item_full + 2;
+  uint64_t *out_done = item_empty + 2, *asked = out_done + 1;
+  uint32_t *tmem_s = (uint32_t *)(asked + 1);
   volatile int *abort_s = (volatile int *)(tmem_s + 1);
 
-  __shared__ Item item;
-  __shared__ bool found;
+  // Pieces of work in turn, as the loading warp finds them: a block does its own
+  // and then those of blocks that have not started.
+  __shared__ Item items[2];
+  __shared__ int last_item[2], any_odd[2];  // no work left; values that are no numbers were found
+  __shared__ __align__(16) uint4 answer;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (warp == 0) {
-    const bool some = find_item<kTiles>(a, &item);
-    if (lane == 0) found = some;
-  }
-  __syncthreads();
-  if (!found) return;
-  const Item it = item;
-  const int kv_head = it.head[0] / (a.q_heads / a.heads);
-
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&q_empty[i], 1);
       tc::mbar_init(&s_full[i], 1);
       tc::mbar_init(&o_done[i], 1);
       tc::mbar_init(&h_done[i], 1);
+      tc::mbar_init(&item_full[i], 1);
+      tc::mbar_init(&item_empty[i], kSoftmaxWarps + 3);
     }
     for (int i = 0; i < kSlots; i++) {
       tc::mbar_init(&kv_full[i], 1);
@@ -401,10 +456,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     for (int i = 0; i < 4; i++) tc::mbar_init(&p_ready[i], 4);
     for (int i = 0; i < kMends; i++) tc::mbar_init(&mended[i], 64);
     tc::mbar_init(drained, 1);
+    tc::mbar_init(out_done, kSoftmaxWarps);
+    tc::mbar_init(asked, 1);
     *abort_s = 0;
     tc::mbar_fence_init();
   }
-  for (int i = tid; i < 3 * D; i += L::kThreads) odd[i / D][i % D] = INT_MAX;
   if (warp == kSoftmaxWarps) {
     tc::tmem_alloc(tmem_s, L::kColumns);
     tc::tmem_relinquish();
@@ -413,26 +469,41 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_s;
-  const int n = it.n, flagged = max(0, n - it.whole);
+  // the k-th piece of work, once it is there
+  auto take = [&](int k) {
+    const bool there = __all_sync(0xffffffffu, wait_long(&item_full[k & 1], k >> 1));
+    if (!there) *abort_s = 1;
+    return there && !*(volatile int *)&last_item[k & 1];
+  };
+  auto release = [&](int k) {
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&item_empty[k & 1]);
+  };
 
   if (warp < kSoftmaxWarps) {
     // ================= softmax: thread = row =================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kMore));
-    const int t = warp >> 2, row = it.i0[t] + (warp & 3) * 32 + lane;
+    const int t = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
-    const int blocks = it.blocks[t], lim = limit(a, it, row);
-    const int first = limit(a, it, it.i0[t]);
     const float c = __fmul_rn(a.scale, kLog2e);
-    float m = -INFINITY;
-    f2 l = 0;
     bool ok = true;
     auto settle = [&](bool fine) {  // the warp goes on, or gives up as one
       ok = __all_sync(0xffffffffu, ok && fine);
       return ok;
     };
+    // key blocks, pieces with one and mended blocks before this piece
+    int past = 0, outs = 0, mends = 0;
+#pragma unroll 1
+    for (int k = 0; take(k); k++) {
+    const Item &it = items[k & 1];
+    const int row = it.i0[t] + (warp & 3) * 32 + lane;
+    const int blocks = it.blocks[t], lim = limit(a, it, row), flagged = max(0, it.n - it.whole);
+    const int first = limit(a, it, it.i0[t]);
+    float m = -INFINITY;
+    f2 l = 0;
     for (int j = blocks - 1, i = 0; j >= 0 && ok; j--, i++) {
-      if (!settle(wait_for(&s_full[t], i))) break;
+      if (!settle(wait_for(&s_full[t], past + i))) break;
       tc::tc_fence_after();
       uint32_t r[4][32];
 #pragma unroll
@@ -476,7 +547,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
               // O holds what the products before this half have added: those of
               // the block before are done (S came after them), those of this
               // block's first half say so
-              if (h > 0 && !settle(wait_for(&h_done[t], i))) break;
+              if (h > 0 && !settle(wait_for(&h_done[t], past + i))) break;
               tc::tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < D / 32; q++) {
@@ -539,14 +610,19 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     // ---- output ----
     const float2 ll = split(l);
     const float sum = __fadd_rn(ll.x, ll.y);
-    if (blocks > 0 && ok) settle(wait_for(&o_done[t], 0));
-    if (flagged > 0 && ok) settle(wait_for(&mended[(flagged - 1) % kMends], (flagged - 1) / kMends));
+    past += blocks;
+    mends += flagged;
+    if (blocks > 0 && ok) settle(wait_for(&o_done[t], outs));
+    if (flagged > 0 && ok) settle(wait_for(&mended[(mends - 1) % kMends], (mends - 1) / kMends));
+    outs += blocks > 0;
     settle(!*abort_s);
     if (!ok) *abort_s = 1;
     tc::tc_fence_after();
     const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
+    const bool odds = flagged > 0 && *(volatile int *)&any_odd[k & 1] != 0;
     const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
-    uint16_t *to = (uint16_t *)a.out + ((int64_t)(it.q0 + row) * a.q_heads + it.head[t]) * D;
+    uint16_t *to = (uint16_t *)a.out +
+                   ((int64_t)(it.q0 + row - (lane & 3)) * a.q_heads + it.head[t]) * D + 8 * (lane & 3);
 #pragma unroll 1
     for (int q = 0; q < D / 32; q++) {
       uint32_t o[32];
@@ -560,7 +636,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         v[e] = none ? 0.0f : __fmul_rn(__uint_as_float(o[e]), inv);
         if (!ok) v[e] = NAN;  // a wait gave up
       }
-      if (flagged > 0 && !none) {
+      if (odds && !none) {
 #pragma unroll
         for (int e = 0; e < 32; e++) {
           const int d = 32 * q + e;
@@ -569,19 +645,30 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
           if (odd[0][d] < lim) v[e] = NAN;
         }
       }
-      if (live) {
+      // four lanes trade their rows' 16-byte pieces, so that a store's lanes lie side
+      // by side: row by row, 32 lanes' pieces are 32 lines
+      uint4 x[4];
 #pragma unroll
-        for (int e = 0; e < 32; e += 8)
-          *(uint4 *)(to + 32 * q + e) =
-              make_uint4(kv::pack2<BF16>(v[e], v[e + 1]), kv::pack2<BF16>(v[e + 2], v[e + 3]),
-                         kv::pack2<BF16>(v[e + 4], v[e + 5]), kv::pack2<BF16>(v[e + 6], v[e + 7]));
-      }
+      for (int e = 0; e < 4; e++)
+        x[e] = make_uint4(kv::pack2<BF16>(v[8 * e], v[8 * e + 1]), kv::pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
+                          kv::pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), kv::pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+      trade(x[0], x[2], 2);
+      trade(x[1], x[3], 2);
+      trade(x[0], x[1], 1);
+      trade(x[2], x[3], 1);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (row - (lane & 3) + e < it.nq)
+          *(uint4 *)(to + (int64_t)e * a.q_heads * D + 32 * q) = x[e];
     }
     if (live && a.lse != nullptr)
       a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
           none ? -INFINITY
                : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
     tc::tc_fence_before();
+    release(k);
+    if (lane == 0) tc::mbar_arrive(out_done);
+    }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLess));
   }
@@ -596,8 +683,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     const uint32_t tm = uniform(tmem), q_base = uniform(tc::smem_u32(sm + L::kQ));
     const uint64_t q_desc = tc::sw128_desc(q_base), k_desc = tc::sw128_desc(q_base + L::kRing);
     const uint64_t v_desc = sw128_desc_n(q_base + L::kRing, 128 * 128);
-    const int nu = uniform(n), whole = uniform(it.whole);
-    const int nb[2] = {(int)uniform(it.blocks[0]), kTiles == 2 ? (int)uniform(it.blocks[1]) : 0};
     bool ok = true;
     auto wait = [&](uint64_t *bar, int phase) {
       if (ok) ok = __all_sync(0xffffffffu, wait_for(bar, phase));
@@ -605,10 +690,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     };
     // block j's values (none for j = n), then block j - 1's scores
     int v_slot = 1, v_phase = 0, k_slot = 0, k_phase = 0;
+    int past[2] = {0, 0}, queries[2] = {0, 0}, mends = 0;
+#pragma unroll 1
+    for (int k = 0; take(k); k++) {
+    const int nu = uniform(items[k & 1].n), whole = uniform(items[k & 1].whole);
+    const int nb[2] = {(int)uniform(items[k & 1].blocks[0]),
+                       kTiles == 2 ? (int)uniform(items[k & 1].blocks[1]) : 0};
+    release(k);
     for (int j = nu; j >= 0 && ok; j--) {
       if (j < nu) {
         if (!wait(&kv_full[v_slot], v_phase)) break;
-        const int f = nu - 1 - j;
+        const int f = mends + nu - 1 - j;
         if (j >= whole && !wait(&mended[f % kMends], f / kMends)) break;
       }
       bool have_k = false;
@@ -618,7 +710,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
           const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            if (!wait(&p_ready[2 * t + h], nb[t] - 1 - j)) break;
+            if (!wait(&p_ready[2 * t + h], past[t] + nb[t] - 1 - j)) break;
             tc::tc_fence_after();
 #pragma unroll
             for (int k = 4 * h; k < 4 * h + 4; k++)
@@ -632,7 +724,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         if (j > 0 && j <= nb[t]) {
           if (!have_k && !wait(&kv_full[k_slot], k_phase)) break;
           have_k = true;
-          if (j == nb[t] && !wait(&q_full[t], 0)) break;
+          if (j == nb[t] && !wait(&q_full[t], queries[t])) break;
           tc::tc_fence_after();
           const uint64_t kd = k_desc + (uint64_t)(k_slot * (L::kTile >> 4));
 #pragma unroll
@@ -641,6 +733,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
             mma_ss(tm + 128 * t, q_desc + t * (L::kTile >> 4) + off, kd + off, ds, k > 0, leader);
           }
           mma_commit(&s_full[t], leader);
+          if (j == 1) mma_commit(&q_empty[t], leader);
         }
       }
       if (!ok) break;
@@ -655,81 +748,144 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         if (k_slot >= kSlots) k_slot -= kSlots, k_phase ^= 1;
       }
     }
+    mends += max(0, nu - whole);
+#pragma unroll
+    for (int t = 0; t < kTiles; t++) {
+      past[t] += nb[t];
+      queries[t] += nb[t] > 0;
+    }
     if (!ok) *abort_s = 1;
+    }
     // every product done before the TMEM goes
     mma_commit(drained, leader);
     wait_for(drained, 0);
     __syncwarp();
   } else if (warp == kSoftmaxWarps + 1) {
-    if (lane == 0) {
-      // ================= loads =================
-      for (int t = 0; t < kTiles; t++) {
-        if (it.blocks[t] == 0) continue;
-        tc::mbar_arrive_expect_tx(&q_full[t], L::kTile);
-        for (int x = 0; x < D; x += 64)
-          tma_load_3d(sm + L::kQ + t * L::kTile + x * 256, &qmap, x, it.head[t], it.q0 + it.i0[t],
-                      &q_full[t]);
+    // ================= loads =================
+    int block = blockIdx.x, k = 0;
+    int answers = 0, queries[2] = {0, 0};
+    int64_t issued = 0;
+    bool waiting = true;
+    if (lane == 0) ask_next(&answer, asked);
+    for (;;) {
+      if (k >= 2 && !__all_sync(0xffffffffu, wait_long(&item_empty[k & 1], (k >> 1) - 1))) {
+        *abort_s = 1;
+        break;
       }
-      int64_t issued = 0;
-      for (int seq = 0; seq < 2 * n; seq++, issued++) {
-        const int s = seq % kSlots, j = n - 1 - seq / 2;
-        if (!wait_for(&kv_empty[s], (seq / kSlots & 1) ^ 1) || *abort_s) {
-          *abort_s = 1;
-          break;
+      Item &it = items[k & 1];
+      const bool some = block >= 0 && find_item<kTiles>(a, block, &it);
+      __syncwarp();
+      if (some || block < 0) {
+        if (lane == 0) {
+          last_item[k & 1] = block < 0;
+          tc::mbar_arrive(&item_full[k & 1]);
         }
-        tc::mbar_arrive_expect_tx(&kv_full[s], L::kTile);
-        for (int x = 0; x < D; x += 64)
-          tma_load_3d(sm + L::kRing + s * L::kTile + x * 256, seq & 1 ? &vmap : &kmap, x, kv_head,
-                      it.k0 + j * kKeys, &kv_full[s]);
+        k++;
       }
-      if (*abort_s) {  // no copy may land after the block is gone
-        for (int64_t k = issued > kSlots ? issued - kSlots : 0; k < issued; k++)
-          wait_for(&kv_full[k % kSlots], (int)(k / kSlots));
-        for (int t = 0; t < kTiles; t++)
-          if (it.blocks[t] > 0) wait_for(&q_full[t], 0);
+      if (block < 0) break;
+      if (some && lane == 0 && !*abort_s) {
+        const int n = it.n, kv_head = it.head[0] / (a.q_heads / a.heads);
+        for (int i = 0; i < 2 * n; i++, issued++) {
+          const int s = issued % kSlots, j = n - 1 - i / 2;
+          if (!wait_for(&kv_empty[s], (issued / kSlots & 1) ^ 1) || *abort_s) {
+            *abort_s = 1;
+            break;
+          }
+          tc::mbar_arrive_expect_tx(&kv_full[s], L::kTile);
+          for (int x = 0; x < D; x += 64)
+            tma_load_3d(sm + L::kRing + s * L::kTile + x * 256, i & 1 ? &vmap : &kmap, x, kv_head,
+                        it.k0 + j * kKeys, &kv_full[s]);
+          if (i > 0) continue;
+          // the first keys are there by the time that the last scores let go of the queries
+          for (int t = 0; t < kTiles; t++) {
+            if (it.blocks[t] == 0) continue;
+            if (queries[t] > 0 && !wait_for(&q_empty[t], queries[t] - 1)) {
+              *abort_s = 1;
+              continue;
+            }
+            queries[t]++;
+            tc::mbar_arrive_expect_tx(&q_full[t], L::kTile);
+            for (int x = 0; x < D; x += 64)
+              tma_load_3d(sm + L::kQ + t * L::kTile + x * 256, &qmap, x, it.head[t],
+                          it.q0 + it.i0[t], &q_full[t]);
+          }
+        }
       }
+      __syncwarp();
+      block = -1;
+      if (waiting && __all_sync(0xffffffffu, wait_for(asked, answers++))) block = answer_of(&answer);
+      // (what was asked for is this block's to do, if only to say that it gave up)
+      waiting = __all_sync(0xffffffffu, block >= 0 && !*abort_s);
+      if (waiting && lane == 0) {
+        tc::fence_async_smem();
+        ask_next(&answer, asked);
+      }
+    }
+    if (lane == 0 && *abort_s) {  // no copy may land after the block is gone
+      for (int64_t i = issued > kSlots ? issued - kSlots : 0; i < issued; i++)
+        wait_for(&kv_full[i % kSlots], (int)(i / kSlots));
+      for (int t = 0; t < kTiles; t++)
+        if (queries[t] > 0) wait_for(&q_full[t], queries[t] - 1);
     }
     __syncwarp();
   } else if (warp > kSoftmaxWarps + 1) {
     // ================= mending values =================
     const int id = tid - 32 * (kSoftmaxWarps + 2);
-    for (int f = 0; f < flagged; f++) {
-      const int seq = 2 * f + 1, j = n - 1 - f;
-      const bool ok = wait_for(&kv_full[seq % kSlots], seq / kSlots) && !*abort_s;
-      if (!__all_sync(0xffffffffu, ok)) {
-        *abort_s = 1;
-        break;
-      }
-      uint8_t *v = sm + L::kRing + (seq % kSlots) * L::kTile;
-      constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u;
-      for (int i = id; i < 128 * (D / 8); i += 64) {
-        const int r = i / (D / 8), ch = i % (D / 8), key = j * kKeys + r;
-        uint4 *at = (uint4 *)(v + tc::sw128_chunk_offset(r, ch, 128));
-        uint4 x = *at;
-        if (key >= it.nk) {
-          *at = make_uint4(0, 0, 0, 0);
-          continue;
+    int64_t tiles = 0;  // of keys and values before this piece
+    int mends = 0;
+#pragma unroll 1
+    for (int k = 0; !any_of_64(!take(k)); k++) {  // (both warps, or none)
+      const int n = items[k & 1].n, nk = items[k & 1].nk;
+      const int flagged = max(0, n - items[k & 1].whole);
+      bool marked = false;
+      if (id == 0) any_odd[k & 1] = 0;
+      for (int f = 0; f < flagged; f++, mends++) {
+        const int64_t seq = tiles + 2 * f + 1;
+        const int key0 = (n - 1 - f) * kKeys;
+        bool ok = wait_for(&kv_full[seq % kSlots], seq / kSlots) && !*abort_s;
+        if (any_of_64(!ok)) {
+          *abort_s = 1;
+          mends += flagged - f;
+          break;
         }
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t bad = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t e = ~w[k] & kExp;  // a half's exponent bits all set: none left here
-          bad |= (uint32_t)((e & 0xffffu) == 0) | (uint32_t)((e >> 16) == 0);
+        uint8_t *v = sm + L::kRing + (seq % kSlots) * L::kTile;
+        // rows of the next sequence or of none (each thread the chunks that it looks at)
+        for (int i = (nk - key0) * (D / 8) + ((id - (nk - key0) * (D / 8)) & 63); i < 128 * (D / 8);
+             i += 64)
+          *(uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128)) = make_uint4(0, 0, 0, 0);
+        uint32_t top = 0;  // the largest magnitudes, as integers
+#pragma unroll 8
+        for (int i = id; i < 128 * (D / 8); i += 64) {
+          const uint4 x = *(const uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128));
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
         }
-        if (bad) {
-          for (int k = 0; k < 8; k++) {
-            const uint32_t half = w[k / 2] >> (16 * (k & 1)) & 0xffffu;
-            if ((~half & (kExp & 0xffffu)) != 0) continue;
-            const int kind = (half & 0x7fffu) != (kExp & 0xffffu) ? 0 : half >> 15 ? 2 : 1;
-            atomicMin(&odd[kind][8 * ch + k], key);
-            w[k / 2] &= k & 1 ? 0x0000ffffu : 0xffff0000u;
+        constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;  // infinity; NaNs are above
+        const bool bad = (top & 0xffffu) >= kExp || top >> 16 >= kExp;
+        if (any_of_64(bad)) {
+          if (!marked) {  // the marks of the piece before have been read
+            marked = true;
+            if (any_of_64(k > 0 && !wait_long(out_done, k - 1))) *abort_s = 1;
+            for (int i = id; i < 3 * D; i += 64) odd[i / D][i % D] = INT_MAX;
+            if (id == 0) any_odd[k & 1] = 1;
+            any_of_64(false);
           }
-          *at = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int i = id; i < 128 * D; i += 64) {
+            const int r = i / D, d = i % D;
+            if (key0 + r >= nk) break;
+            uint16_t *at = (uint16_t *)(v + tc::sw128_chunk_offset(r, d / 8, 128)) + d % 8;
+            const uint32_t half = *at;
+            if ((half & kExp) != kExp) continue;
+            atomicMin(&odd[(half & 0x7fffu) != kExp ? 0 : half >> 15 ? 2 : 1][d],
+                      key0 + r);
+            *at = 0;
+          }
         }
+        tc::fence_async_smem();
+        tc::mbar_arrive(&mended[mends % kMends]);
       }
-      tc::fence_async_smem();
-      tc::mbar_arrive(&mended[f % kMends]);
+      tiles += 2 * n;
+      release(k);
     }
   }
   __syncthreads();
