@@ -289,8 +289,8 @@ struct Shape {
   // TMEM: S (then P) of the tiles, then their O
   static constexpr int kO = 128 * kTiles, kColumns = 256 * kTiles;
   // Registers of the softmax warps and of the others: they add up to what the
-  // block was launched with (8 x 232 + 4 x 40 = 12 x 168, 4 x 208 + 4 x 48 = 8 x 128).
-  static constexpr int kMore = kTiles == 2 ? 232 : 208, kLess = kTiles == 2 ? 40 : 48;
+  // block was launched with (8 x 224 + 4 x 56 = 12 x 168, 4 x 208 + 4 x 48 = 8 x 128).
+  static constexpr int kMore = kTiles == 2 ? 224 : 208, kLess = kTiles == 2 ? 56 : 48;
 };
 
 // What a block works on.
@@ -346,7 +346,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   constexpr int kEach = 4;
   const bool twins = pairs_heads<TILES>(a);
   const int shift = !twins && TILES == 2 ? 8 : 7, rows = 1 << shift, heads = twins ? a.q_heads / 2 : a.q_heads;
-  const int64_t u = block / heads;
+  const int u = block / heads;
   const int h = block % heads, lane = threadIdx.x & 31;
   if (a.n > 32 * kEach) {
     // entry b has starts_q[b + 1] / rows - starts_q[b] / rows + 1 tiles
@@ -378,16 +378,16 @@ __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   auto begin = [&](int s, int c) {
     const int tiles = (nq[s] + rows - 1) >> shift;
     if (c == 0) return 0;
-    const int64_t x = (int64_t)(c - 1) * kKeys + (a.causal ? nq[s] - nk[s] : 0);
+    const int x = (c - 1) * kKeys + (a.causal ? nq[s] - nk[s] : 0);
     if (!a.causal) return x < nk[s] ? 0 : tiles;
-    return x >= nq[s] ? tiles : x < 0 ? 0 : (int)(x >> shift);
+    return x >= nq[s] ? tiles : x < 0 ? 0 : x >> shift;
   };
   auto at_least = [&](int c) {  // tiles with c blocks or more, of all entries
     int sum = 0;
 #pragma unroll
     for (int s = 0; s < kEach; s++)
       if (32 * s < a.n) sum += ((nq[s] + rows - 1) >> shift) - begin(s, c);
-    return (int64_t)__reduce_add_sync(0xffffffffu, sum);
+    return __reduce_add_sync(0xffffffffu, sum);
   };
   if (u >= at_least(0)) return false;
   int lo = 0, hi = __reduce_max_sync(0xffffffffu, most);
@@ -396,7 +396,7 @@ __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
     if (at_least(mid) > u) lo = mid;
     else hi = mid - 1;
   }
-  int v = (int)(u - at_least(lo + 1));  // among the tiles with exactly c blocks
+  int v = u - at_least(lo + 1);  // among the tiles with exactly c blocks
 #pragma unroll
   for (int s = 0; s < kEach; s++) {
     const int from = begin(s, lo), count = begin(s, lo + 1) - from;
@@ -496,178 +496,179 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     int past = 0, outs = 0, mends = 0;
 #pragma unroll 1
     for (int k = 0; take(k); k++) {
-    const Item &it = items[k & 1];
-    const int row = it.i0[t] + (warp & 3) * 32 + lane;
-    const int blocks = it.blocks[t], lim = limit(a, it, row), flagged = max(0, it.n - it.whole);
-    const int first = limit(a, it, it.i0[t]);
-    float m = -INFINITY;
-    f2 l = 0;
-    for (int j = blocks - 1, i = 0; j >= 0 && ok; j--, i++) {
-      if (!settle(wait_for(&s_full[t], past + i))) break;
-      tc::tc_fence_after();
-      uint32_t r[4][32];
+      const Item &it = items[k & 1];
+      const int row = it.i0[t] + (warp & 3) * 32 + lane;
+      const int blocks = it.blocks[t], lim = limit(a, it, row), flagged = max(0, it.n - it.whole);
+      const int first = limit(a, it, it.i0[t]);
+      float m = -INFINITY;
+      f2 l = 0;
+      for (int j = blocks - 1, i = 0; j >= 0 && ok; j--, i++) {
+        if (!settle(wait_for(&s_full[t], past + i))) break;
+        tc::tc_fence_after();
+        uint32_t r[4][32];
 #pragma unroll
-      for (int q = 0; q < 4; q++) tc::tmem_ld32(s_at + 32 * q, r[q]);
-      tc::tmem_ld_wait();
-      const bool masked = (j + 1) * kKeys > first;
-      const int seen = lim - j * kKeys;  // columns of this block that the row sees
-      if (masked) {
-        asm volatile("");  // a branch, not 128 selects in every block
+        for (int q = 0; q < 4; q++) tc::tmem_ld32(s_at + 32 * q, r[q]);
+        tc::tmem_ld_wait();
+        const bool masked = (j + 1) * kKeys > first;
+        const int seen = lim - j * kKeys;  // columns of this block that the row sees
+        if (masked) {
+          asm volatile("");  // a branch, not 128 selects in every block
 #pragma unroll
-        for (int e = 0; e < 128; e++)
-          if (e >= seen) r[e / 32][e % 32] = 0xff800000u;
-      }
+          for (int e = 0; e < 128; e++)
+            if (e >= seen) r[e / 32][e % 32] = 0xff800000u;
+        }
 #pragma unroll
-      for (int h = 0; h < 2; h++) {  // 64 keys
-        f2 sum;
-        uint32_t p[2][16];
-        // a row without a reference needs its maximum first; a row that needs
-        // none keeps its own, whoever shares its warp
-        bool need = m == -INFINITY, again = __any_sync(0xffffffffu, need);
-        for (;;) {
-          if (again) {
-            // (opaque here, so that the maximum is not computed ahead of the branch)
+        for (int h = 0; h < 2; h++) {  // 64 keys
+          f2 sum;
+          uint32_t p[2][16];
+          // a row without a reference needs its maximum first; a row that needs
+          // none keeps its own, whoever shares its warp
+          bool need = m == -INFINITY, again = __any_sync(0xffffffffu, need);
+          for (;;) {
+            if (again) {
+              // (opaque here, so that the maximum is not computed ahead of the branch)
 #pragma unroll
-            for (int e = 0; e < 64; e++) asm volatile("" : "+r"(r[2 * h + e / 32][e % 32]));
-            float top[4];
+              for (int e = 0; e < 64; e++) asm volatile("" : "+r"(r[2 * h + e / 32][e % 32]));
+              float top[4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-              const uint32_t *x = &r[2 * h + q / 2][16 * (q % 2)];
-              top[q] = __uint_as_float(x[0]);
+              for (int q = 0; q < 4; q++) {
+                const uint32_t *x = &r[2 * h + q / 2][16 * (q % 2)];
+                top[q] = __uint_as_float(x[0]);
 #pragma unroll
-              for (int e = 1; e < 16; e++) top[q] = max_nan(top[q], __uint_as_float(x[e]));
-            }
-            const float nm =
-                max_nan(m, max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])));
-            const float f =
-                !need || nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
-            m = need ? nm : m;
-            l = fma2(l, pair(f, f), 0);
-            if (i > 0 || h > 0) {
-              // O holds what the products before this half have added: those of
-              // the block before are done (S came after them), those of this
-              // block's first half say so
-              if (h > 0 && !settle(wait_for(&h_done[t], past + i))) break;
-              tc::tc_fence_after();
+                for (int e = 1; e < 16; e++) top[q] = max_nan(top[q], __uint_as_float(x[e]));
+              }
+              const float nm =
+                  max_nan(m, max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])));
+              const float f =
+                  !need || nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
+              m = need ? nm : m;
+              l = fma2(l, pair(f, f), 0);
+              if (i > 0 || h > 0) {
+                // O holds what the products before this half have added: those of
+                // the block before are done (S came after them), those of this
+                // block's first half say so
+                if (h > 0 && !settle(wait_for(&h_done[t], past + i))) break;
+                tc::tc_fence_after();
 #pragma unroll 1
-              for (int q = 0; q < D / 32; q++) {
-                uint32_t o[32];
-                tc::tmem_ld32(o_at + 32 * q, o);
-                tc::tmem_ld_wait();
+                for (int q = 0; q < D / 32; q++) {
+                  uint32_t o[32];
+                  tc::tmem_ld32(o_at + 32 * q, o);
+                  tc::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; e++)
-                  o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
-                tmem_st32(o_at + 32 * q, o);
+                  for (int e = 0; e < 32; e++)
+                    o[e] = __float_as_uint(__fmul_rn(__uint_as_float(o[e]), f));
+                  tmem_st32(o_at + 32 * q, o);
+                }
               }
             }
-          }
-          // a row that sees a score of +inf or NaN is NaN
-          const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
-          const f2 cc = pair(c, c), bb = pair(base, base);
-          f2 b0 = 0, b1 = 0;
+            // a row that sees a score of +inf or NaN is NaN
+            const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
+            const f2 cc = pair(c, c), bb = pair(base, base);
+            f2 b0 = 0, b1 = 0;
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            const uint32_t *x = &r[2 * h + e / 32][e % 32];
-            const f2 z = fma2(pair(__uint_as_float(x[0]), __uint_as_float(x[1])), cc, bb);
-            float2 y;
-            if (e % kPolyOf < kPoly) {
-              y = exp2_poly(z);
-            } else {
-              const float2 v = split(z);
-              y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+            for (int e = 0; e < 64; e += 2) {
+              const uint32_t *x = &r[2 * h + e / 32][e % 32];
+              const f2 z = fma2(pair(__uint_as_float(x[0]), __uint_as_float(x[1])), cc, bb);
+              float2 y;
+              if (e % kPolyOf < kPoly) {
+                y = exp2_poly(z);
+              } else {
+                const float2 v = split(z);
+                y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+              }
+              if (e % 4) b1 = add2(b1, pair(y.x, y.y));
+              else b0 = add2(b0, pair(y.x, y.y));
+              p[e / 32][e % 32 / 2] = kv::pack2<BF16>(y.x, y.y);
             }
-            if (e % 4) b1 = add2(b1, pair(y.x, y.y));
-            else b0 = add2(b0, pair(y.x, y.y));
-            p[e / 32][e % 32 / 2] = kv::pack2<BF16>(y.x, y.y);
+            sum = add2(b0, b1);
+            if (again) break;
+            // weights beyond 2^14 (or NaN): take a new reference and start over
+            const float2 v = split(sum);
+            need = !(v.x <= kGrow) || !(v.y <= kGrow);
+            again = __any_sync(0xffffffffu, need);
+            if (!again) break;
           }
-          sum = add2(b0, b1);
-          if (again) break;
-          // weights beyond 2^14 (or NaN): take a new reference and start over
-          const float2 v = split(sum);
-          need = !(v.x <= kGrow) || !(v.y <= kGrow);
-          again = __any_sync(0xffffffffu, need);
-          if (!again) break;
-        }
-        if (!ok) break;
-        l = add2(l, sum);
-        if (masked) {
-          asm volatile("");
+          if (!ok) break;
+          l = add2(l, sum);
+          if (masked) {
+            asm volatile("");
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) {
-            if (64 * h + e >= seen) p[e / 32][e % 32 / 2] &= 0xffff0000u;
-            if (64 * h + e + 1 >= seen) p[e / 32][e % 32 / 2] &= 0x0000ffffu;
+            for (int e = 0; e < 64; e += 2) {
+              if (e % kPolyOf >= kPoly) continue;  // the MUFU's are zeros already
+              if (64 * h + e >= seen) p[e / 32][e % 32 / 2] &= 0xffff0000u;
+              if (64 * h + e + 1 >= seen) p[e / 32][e % 32 / 2] &= 0x0000ffffu;
+            }
           }
+          tmem_st16(s_at + 64 * h, p[0]);
+          tmem_st16(s_at + 64 * h + 16, p[1]);
+          tmem_st_wait();
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&p_ready[2 * t + h]);
         }
-        tmem_st16(s_at + 64 * h, p[0]);
-        tmem_st16(s_at + 64 * h + 16, p[1]);
-        tmem_st_wait();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&p_ready[2 * t + h]);
       }
-    }
-    if (!ok) *abort_s = 1;
-    // ---- output ----
-    const float2 ll = split(l);
-    const float sum = __fadd_rn(ll.x, ll.y);
-    past += blocks;
-    mends += flagged;
-    if (blocks > 0 && ok) settle(wait_for(&o_done[t], outs));
-    if (flagged > 0 && ok) settle(wait_for(&mended[(mends - 1) % kMends], (mends - 1) / kMends));
-    outs += blocks > 0;
-    settle(!*abort_s);
-    if (!ok) *abort_s = 1;
-    tc::tc_fence_after();
-    const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
-    const bool odds = flagged > 0 && *(volatile int *)&any_odd[k & 1] != 0;
-    const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
-    uint16_t *to = (uint16_t *)a.out +
-                   ((int64_t)(it.q0 + row - (lane & 3)) * a.q_heads + it.head[t]) * D + 8 * (lane & 3);
+      if (!ok) *abort_s = 1;
+      // ---- output ----
+      const float2 ll = split(l);
+      const float sum = __fadd_rn(ll.x, ll.y);
+      past += blocks;
+      mends += flagged;
+      if (blocks > 0 && ok) settle(wait_for(&o_done[t], outs));
+      if (flagged > 0 && ok) settle(wait_for(&mended[(mends - 1) % kMends], (mends - 1) / kMends));
+      outs += blocks > 0;
+      settle(!*abort_s);
+      if (!ok) *abort_s = 1;
+      tc::tc_fence_after();
+      const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
+      const bool odds = flagged > 0 && *(volatile int *)&any_odd[k & 1] != 0;
+      const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
+      uint16_t *to = (uint16_t *)a.out +
+                     ((int64_t)(it.q0 + row - (lane & 3)) * a.q_heads + it.head[t]) * D + 8 * (lane & 3);
 #pragma unroll 1
-    for (int q = 0; q < D / 32; q++) {
-      uint32_t o[32];
-      if (blocks > 0 && ok) {
-        tc::tmem_ld32(o_at + 32 * q, o);
-        tc::tmem_ld_wait();
-      }
-      float v[32];
-#pragma unroll
-      for (int e = 0; e < 32; e++) {
-        v[e] = none ? 0.0f : __fmul_rn(__uint_as_float(o[e]), inv);
-        if (!ok) v[e] = NAN;  // a wait gave up
-      }
-      if (odds && !none) {
+      for (int q = 0; q < D / 32; q++) {
+        uint32_t o[32];
+        if (blocks > 0 && ok) {
+          tc::tmem_ld32(o_at + 32 * q, o);
+          tc::tmem_ld_wait();
+        }
+        float v[32];
 #pragma unroll
         for (int e = 0; e < 32; e++) {
-          const int d = 32 * q + e;
-          if (odd[1][d] < lim) v[e] = __fadd_rn(v[e], INFINITY);
-          if (odd[2][d] < lim) v[e] = __fadd_rn(v[e], -INFINITY);
-          if (odd[0][d] < lim) v[e] = NAN;
+          v[e] = none ? 0.0f : __fmul_rn(__uint_as_float(o[e]), inv);
+          if (!ok) v[e] = NAN;  // a wait gave up
         }
+        if (odds && !none) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const int d = 32 * q + e;
+            if (odd[1][d] < lim) v[e] = __fadd_rn(v[e], INFINITY);
+            if (odd[2][d] < lim) v[e] = __fadd_rn(v[e], -INFINITY);
+            if (odd[0][d] < lim) v[e] = NAN;
+          }
+        }
+        // four lanes trade their rows' 16-byte pieces, so that a store's lanes lie side
+        // by side: row by row, 32 lanes' pieces are 32 lines
+        uint4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          x[e] = make_uint4(kv::pack2<BF16>(v[8 * e], v[8 * e + 1]), kv::pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
+                            kv::pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), kv::pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+        trade(x[0], x[2], 2);
+        trade(x[1], x[3], 2);
+        trade(x[0], x[1], 1);
+        trade(x[2], x[3], 1);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (row - (lane & 3) + e < it.nq)
+            *(uint4 *)(to + (int64_t)e * a.q_heads * D + 32 * q) = x[e];
       }
-      // four lanes trade their rows' 16-byte pieces, so that a store's lanes lie side
-      // by side: row by row, 32 lanes' pieces are 32 lines
-      uint4 x[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        x[e] = make_uint4(kv::pack2<BF16>(v[8 * e], v[8 * e + 1]), kv::pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
-                          kv::pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), kv::pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
-      trade(x[0], x[2], 2);
-      trade(x[1], x[3], 2);
-      trade(x[0], x[1], 1);
-      trade(x[2], x[3], 1);
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (row - (lane & 3) + e < it.nq)
-          *(uint4 *)(to + (int64_t)e * a.q_heads * D + 32 * q) = x[e];
-    }
-    if (live && a.lse != nullptr)
-      a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
-          none ? -INFINITY
-               : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
-    tc::tc_fence_before();
-    release(k);
-    if (lane == 0) tc::mbar_arrive(out_done);
+      if (live && a.lse != nullptr)
+        a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
+            none ? -INFINITY
+                 : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
+      tc::tc_fence_before();
+      release(k);
+      if (lane == 0) tc::mbar_arrive(out_done);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLess));
@@ -693,68 +694,68 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     int past[2] = {0, 0}, queries[2] = {0, 0}, mends = 0;
 #pragma unroll 1
     for (int k = 0; take(k); k++) {
-    const int nu = uniform(items[k & 1].n), whole = uniform(items[k & 1].whole);
-    const int nb[2] = {(int)uniform(items[k & 1].blocks[0]),
-                       kTiles == 2 ? (int)uniform(items[k & 1].blocks[1]) : 0};
-    release(k);
-    for (int j = nu; j >= 0 && ok; j--) {
-      if (j < nu) {
-        if (!wait(&kv_full[v_slot], v_phase)) break;
-        const int f = mends + nu - 1 - j;
-        if (j >= whole && !wait(&mended[f % kMends], f / kMends)) break;
+      const int nu = uniform(items[k & 1].n), whole = uniform(items[k & 1].whole);
+      const int nb[2] = {(int)uniform(items[k & 1].blocks[0]),
+                         kTiles == 2 ? (int)uniform(items[k & 1].blocks[1]) : 0};
+      release(k);
+      for (int j = nu; j >= 0 && ok; j--) {
+        if (j < nu) {
+          if (!wait(&kv_full[v_slot], v_phase)) break;
+          const int f = mends + nu - 1 - j;
+          if (j >= whole && !wait(&mended[f % kMends], f / kMends)) break;
+        }
+        bool have_k = false;
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) {
+          if (j < nb[t]) {
+            const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              if (!wait(&p_ready[2 * t + h], past[t] + nb[t] - 1 - j)) break;
+              tc::tc_fence_after();
+#pragma unroll
+              for (int k = 4 * h; k < 4 * h + 4; k++)
+                mma_ts(tm + L::kO + 128 * t, tm + 128 * t + 64 * h + 8 * (k & 3),
+                       vd + (k * 16 * 128 >> 4), dp, k > 0 || j < nb[t] - 1, leader);
+              if (h == 0) mma_commit(&h_done[t], leader);
+            }
+            if (!ok) break;
+            if (j == 0) mma_commit(&o_done[t], leader);
+          }
+          if (j > 0 && j <= nb[t]) {
+            if (!have_k && !wait(&kv_full[k_slot], k_phase)) break;
+            have_k = true;
+            if (j == nb[t] && !wait(&q_full[t], queries[t])) break;
+            tc::tc_fence_after();
+            const uint64_t kd = k_desc + (uint64_t)(k_slot * (L::kTile >> 4));
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) {
+              const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+              mma_ss(tm + 128 * t, q_desc + t * (L::kTile >> 4) + off, kd + off, ds, k > 0, leader);
+            }
+            mma_commit(&s_full[t], leader);
+            if (j == 1) mma_commit(&q_empty[t], leader);
+          }
+        }
+        if (!ok) break;
+        if (j < nu) {
+          mma_commit(&kv_empty[v_slot], leader);
+          v_slot += 2;
+          if (v_slot >= kSlots) v_slot -= kSlots, v_phase ^= 1;
+        }
+        if (j > 0) {
+          mma_commit(&kv_empty[k_slot], leader);
+          k_slot += 2;
+          if (k_slot >= kSlots) k_slot -= kSlots, k_phase ^= 1;
+        }
       }
-      bool have_k = false;
+      mends += max(0, nu - whole);
 #pragma unroll
       for (int t = 0; t < kTiles; t++) {
-        if (j < nb[t]) {
-          const uint64_t vd = v_desc + (uint64_t)(v_slot * (L::kTile >> 4));
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            if (!wait(&p_ready[2 * t + h], past[t] + nb[t] - 1 - j)) break;
-            tc::tc_fence_after();
-#pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; k++)
-              mma_ts(tm + L::kO + 128 * t, tm + 128 * t + 64 * h + 8 * (k & 3),
-                     vd + (k * 16 * 128 >> 4), dp, k > 0 || j < nb[t] - 1, leader);
-            if (h == 0) mma_commit(&h_done[t], leader);
-          }
-          if (!ok) break;
-          if (j == 0) mma_commit(&o_done[t], leader);
-        }
-        if (j > 0 && j <= nb[t]) {
-          if (!have_k && !wait(&kv_full[k_slot], k_phase)) break;
-          have_k = true;
-          if (j == nb[t] && !wait(&q_full[t], queries[t])) break;
-          tc::tc_fence_after();
-          const uint64_t kd = k_desc + (uint64_t)(k_slot * (L::kTile >> 4));
-#pragma unroll
-          for (int k = 0; k < D / 16; k++) {
-            const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-            mma_ss(tm + 128 * t, q_desc + t * (L::kTile >> 4) + off, kd + off, ds, k > 0, leader);
-          }
-          mma_commit(&s_full[t], leader);
-          if (j == 1) mma_commit(&q_empty[t], leader);
-        }
+        past[t] += nb[t];
+        queries[t] += nb[t] > 0;
       }
-      if (!ok) break;
-      if (j < nu) {
-        mma_commit(&kv_empty[v_slot], leader);
-        v_slot += 2;
-        if (v_slot >= kSlots) v_slot -= kSlots, v_phase ^= 1;
-      }
-      if (j > 0) {
-        mma_commit(&kv_empty[k_slot], leader);
-        k_slot += 2;
-        if (k_slot >= kSlots) k_slot -= kSlots, k_phase ^= 1;
-      }
-    }
-    mends += max(0, nu - whole);
-#pragma unroll
-    for (int t = 0; t < kTiles; t++) {
-      past[t] += nb[t];
-      queries[t] += nb[t] > 0;
-    }
-    if (!ok) *abort_s = 1;
+      if (!ok) *abort_s = 1;
     }
     // every product done before the TMEM goes
     mma_commit(drained, leader);
@@ -854,7 +855,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
              i += 64)
           *(uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128)) = make_uint4(0, 0, 0, 0);
         uint32_t top = 0;  // the largest magnitudes, as integers
-#pragma unroll 8
+#pragma unroll 4
         for (int i = id; i < 128 * (D / 8); i += 64) {
           const uint4 x = *(const uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128));
           top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
