@@ -200,6 +200,38 @@ def test_many_sequences_of_every_length(uv, n):
         assert np.isfinite(f64(out)).all()
 
 
+@pytest.mark.parametrize("d,hq,causal", [(64, 16, True), (128, 16, True), (128, 18, True), (128, 16, False)])
+def test_more_work_than_blocks(uv, d, hq, causal):
+    """Every block takes several pieces of work, some with values that are no
+    numbers: what one piece has met does not reach the next."""
+    import torch
+
+    rng = np.random.default_rng(d + hq)
+    nq = [int(x) for x in rng.integers(1, 300, 48)]
+    nk = [x + 70 * (i % 3) for i, x in enumerate(nq)]
+    q, k = rows(rng, sum(nq), hq, d, "bfloat16"), rows(rng, sum(nk), 2, d, "bfloat16")
+    v = rows(rng, sum(nk), 2, d, "bfloat16")
+    bad, clean = v.clone(), v.clone()
+    b = np.concatenate([[0], np.cumsum(nk)])
+    a = np.concatenate([[0], np.cumsum(nq)])
+    where = {}
+    for i in range(0, 48, 3):
+        key, head, col = int(rng.integers(0, nk[i])), int(rng.integers(0, 2)), int(rng.integers(0, d))
+        what = (math.inf, -math.inf, math.nan)[i // 3 % 3]
+        bad[b[i] + key, head, col] = what
+        clean[b[i] + key, head, col] = 0
+        where[i] = key, head, col, what
+    out, lse = uv.prompt_attention(q, k, bad, starts(nq), starts(nk), causal=causal, lse=True)
+    for i, (key, head, col, what) in where.items():
+        first = max(0, key - (nk[i] - nq[i])) if causal else 0  # row that sees the key
+        part = out[a[i] + first:a[i + 1], head * (hq // 2):(head + 1) * (hq // 2), col]
+        assert bool((part.isnan() if math.isnan(what) else part == what).all())
+        mine = f64(clean[b[i]:b[i + 1]])
+        want = M.prompt(f64(q[a[i]:a[i + 1]]), f64(k[b[i]:b[i + 1]]), mine, causal, 1 / math.sqrt(d))[0]
+        part.copy_(torch.tensor(want[first:, head * (hq // 2):(head + 1) * (hq // 2), col]))
+    compare(out, lse, q, k, clean, nq, nk, causal, "bfloat16", 1 / math.sqrt(d))
+
+
 def test_refused_arguments(uv):
     import torch
 

@@ -13,14 +13,22 @@
 // core works for the other.  At D = 128 they are one block's, with the same keys
 // (two heads of a group, or 256 consecutive rows where the group is odd); at
 // D = 64 two blocks', each of which starts and writes out while the other works.
-// One long prompt of D = 128 (8192 tokens, 32 heads) takes 562 us in the first form
-// and 640 in the second, which has room for one tile of keys and one of values;
-// 48 short texts of D = 64 take 66 and 49 us.
+// (With a block for every piece of work, one long prompt of D = 128, 8192 tokens and
+// 32 heads, took 562 us in the first form and 640 in the second, which has room for
+// one tile of keys and one of values; 48 short texts of D = 64 took 66 and 49 us.)
 //
 //   warps 0-3 (, 4-7)  softmax and output of a tile
 //   the next one       issues the products, owns the TMEM
-//   the next one       loads Q, K, V by TMA (one lane)
+//   the next one       finds the work, loads Q, K, V by TMA (one lane)
 //   the next two       mend the values of blocks with masked keys (below)
+//
+// The grid has a block for every piece of work (its one or two tiles), and a block
+// that has loaded its piece's last keys cancels one that has not started and does its
+// work (the hardware hands them out in order): that piece's queries and first keys
+// come, and its first scores are made, while this one's output goes out.  Beside a
+// start and an end for every piece this took 7 packed prompts from 154 to 149 us and
+// 48 texts from 45 to 43; what mattered more was code that runs once a piece, at some
+// 10 cycles an instruction: the look over the values, the search, the output.
 //
 // Blocks of keys go from the last, masked ones to the first.  A row's weights
 // stand against a reference, the maximum of the first keys that it sees, and no
@@ -32,7 +40,8 @@
 // of infinity or NaN is a NaN.  So in blocks with a masked key such values are
 // taken out (as are the next sequence's rows), and for every column the first
 // key that held one is kept: rows that see that key get it added to their
-// output.
+// output.  Two warps look for the largest magnitude of a block (16 bits a value, two
+// at a time) and go through it value by value only where there is one.
 //
 // Bound: per 128 x 128 tile and D = 128 the two products take 1024 cycles of
 // the tensor core, the exponentials 1024 of the MUFU (16 a cycle) if it computes
@@ -40,7 +49,7 @@
 // sums and packing about as many issue cycles.  A tile's chain (scores, 128
 // exponentials a thread at about 7 cycles, product) takes 2300 cycles with the
 // other tile beside it, so 3500 pass for two tiles, of which the tensor core
-// works 2048: 980 TFLOP/s for 8192 tokens and 32 heads (0.56 ms), at the 1.69 GHz
+// works 2048: 1000 TFLOP/s for 8192 tokens and 32 heads (0.55 ms), at the 1.69 GHz
 // that the power limit then leaves.
 #include <cfloat>
 #include <climits>
@@ -166,8 +175,8 @@ __device__ __forceinline__ bool wait_long(uint64_t *bar, int64_t phase) {
 __device__ __forceinline__ void ask_next(void *answer, uint64_t *bar) {
   tc::mbar_arrive_expect_tx(bar, 16);
   asm volatile(
-      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::
-          "r"(tc::smem_u32(answer)),
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+      " [%0], [%1];" ::"r"(tc::smem_u32(answer)),
       "r"(tc::smem_u32(bar))
       : "memory");
 }
@@ -335,7 +344,7 @@ __device__ __forceinline__ void describe(const Args &a, int b, int64_t i0, int h
   it->whole = first / kKeys;
 }
 
-// One warp's search for the block's work.  Tiles go in the order of their key
+// One warp's search for a block's work.  Tiles go in the order of their key
 // blocks, most first, so that no long one is left for the end: how many tiles of
 // an entry have c blocks or more is a division, so the u-th tile is a binary
 // search over c, with the entries over the lanes.  (One sequence of 6000 tokens
@@ -345,7 +354,8 @@ template <int TILES>
 __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   constexpr int kEach = 4;
   const bool twins = pairs_heads<TILES>(a);
-  const int shift = !twins && TILES == 2 ? 8 : 7, rows = 1 << shift, heads = twins ? a.q_heads / 2 : a.q_heads;
+  const int shift = !twins && TILES == 2 ? 8 : 7, rows = 1 << shift;
+  const int heads = twins ? a.q_heads / 2 : a.q_heads;
   const int u = block / heads;
   const int h = block % heads, lane = threadIdx.x & 31;
   if (a.n > 32 * kEach) {
@@ -539,11 +549,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
               }
               const float nm =
                   max_nan(m, max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])));
-              const float f =
-                  !need || nm == -INFINITY ? 1.0f : exp2_fast(__fmul_rn(__fsub_rn(m, nm), c));
+              // (what has seen nothing has sums of zero: any factor keeps them)
+              const float f = need && m != -INFINITY && nm != -INFINITY
+                                  ? exp2_fast(__fmul_rn(__fsub_rn(m, nm), c))
+                                  : 1.0f;
               m = need ? nm : m;
               l = fma2(l, pair(f, f), 0);
-              if (i > 0 || h > 0) {
+              if (__any_sync(0xffffffffu, f != 1.0f)) {
                 // O holds what the products before this half have added: those of
                 // the block before are done (S came after them), those of this
                 // block's first half say so
@@ -621,7 +633,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       tc::tc_fence_after();
       const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
       const bool odds = flagged > 0 && *(volatile int *)&any_odd[k & 1] != 0;
-      const float inv = none ? 0.0f : __fdiv_rn(1.0f, sum);
+      // (the sums of a row that sees nothing are zeros: its keys' values are mended)
+      const float inv = !ok ? NAN : none ? 0.0f : __fdiv_rn(1.0f, sum);  // NaN: a wait gave up
       uint16_t *to = (uint16_t *)a.out +
                      ((int64_t)(it.q0 + row - (lane & 3)) * a.q_heads + it.head[t]) * D + 8 * (lane & 3);
 #pragma unroll 1
@@ -630,13 +643,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         if (blocks > 0 && ok) {
           tc::tmem_ld32(o_at + 32 * q, o);
           tc::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = 0;
         }
         float v[32];
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          v[e] = none ? 0.0f : __fmul_rn(__uint_as_float(o[e]), inv);
-          if (!ok) v[e] = NAN;  // a wait gave up
-        }
+        for (int e = 0; e < 32; e++) v[e] = __fmul_rn(__uint_as_float(o[e]), inv);
         if (odds && !none) {
 #pragma unroll
           for (int e = 0; e < 32; e++) {
@@ -651,8 +664,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
         uint4 x[4];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          x[e] = make_uint4(kv::pack2<BF16>(v[8 * e], v[8 * e + 1]), kv::pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
-                            kv::pack2<BF16>(v[8 * e + 4], v[8 * e + 5]), kv::pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
+          x[e] = make_uint4(kv::pack2<BF16>(v[8 * e], v[8 * e + 1]),
+                            kv::pack2<BF16>(v[8 * e + 2], v[8 * e + 3]),
+                            kv::pack2<BF16>(v[8 * e + 4], v[8 * e + 5]),
+                            kv::pack2<BF16>(v[8 * e + 6], v[8 * e + 7]));
         trade(x[0], x[2], 2);
         trade(x[1], x[3], 2);
         trade(x[0], x[1], 1);
@@ -850,14 +865,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
           break;
         }
         uint8_t *v = sm + L::kRing + (seq % kSlots) * L::kTile;
-        // rows of the next sequence or of none (each thread the chunks that it looks at)
-        for (int i = (nk - key0) * (D / 8) + ((id - (nk - key0) * (D / 8)) & 63); i < 128 * (D / 8);
-             i += 64)
-          *(uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128)) = make_uint4(0, 0, 0, 0);
+        // 16-byte pieces as they lie, 8 of them 64 columns of a row; first zeros for the
+        // next sequence's rows (from each thread in the pieces that it looks at)
+        const int from = 8 * min(nk - key0, 128);
+        for (int x = 0; x < D; x += 64)
+          for (int i = from + ((id - from) & 63); i < 128 * 8; i += 64)
+            *(uint4 *)(v + x * 256 + i * 16) = make_uint4(0, 0, 0, 0);
         uint32_t top = 0;  // the largest magnitudes, as integers
 #pragma unroll 4
-        for (int i = id; i < 128 * (D / 8); i += 64) {
-          const uint4 x = *(const uint4 *)(v + tc::sw128_chunk_offset(i / (D / 8), i % (D / 8), 128));
+        for (int i = 0; i < 128 * D * 2; i += 64 * 16) {
+          const uint4 x = *(const uint4 *)(v + id * 16 + i);
           top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
                                        __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
         }
