@@ -72,6 +72,8 @@ constexpr float kC0 = 0.9999992847442627f, kC1 = 0.6931217908859253f, kC2 = 0.24
 constexpr int kPoly = 2, kPolyOf = 8;
 // Barriers of mended values, in turn: the ring holds at most three blocks of values whose
 // product is still to be issued, so none completes a second time before it was waited for.
+// (An output waits for its piece's last one; by then at most the next piece's are mended,
+// and 256 rows end within three blocks.)
 constexpr int kMends = 4;
 constexpr float kGrow = 16384.0f;  // weights (sums of 32 of them) up to this stay unanswered
 
