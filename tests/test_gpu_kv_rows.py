@@ -316,6 +316,34 @@ def test_one_long_sequence_and_many_ragged_ones_split_alike(uv):
         assert (np.abs(f64(alone) - want) <= attend_tolerance(want, size, reach, "bfloat16")).all()
 
 
+@pytest.mark.parametrize("lens", [[20_000], [9000, 40, 7000, 300], [2500] * 24])
+def test_every_split_job_is_joined_every_time(uv, lens):
+    """Outputs that hold NaN before the call have the same bits after each of many
+    calls: of the blocks that share a job (one to two hundred, finishing
+    together), some one joins it, every time."""
+    import torch
+
+    rng = np.random.default_rng(len(lens))
+    heads, d = 2, 128
+    c, _ = cache(uv, d, heads, lens)
+    fill(c, lens, d, heads, "bfloat16", rng)
+    n = len(lens)
+    q = rows_of(rng, n, 4 * heads, d, "bfloat16", False)
+    seqs, L, st = ints(range(n)), uv.lib(), torch.cuda.current_stream().cuda_stream
+    want, sums = c.attend(seqs, q, lse=True)
+    out, lse, missed = torch.empty_like(want), torch.empty_like(sums), torch.zeros((), device="cuda")
+    scratch = torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")
+    for _ in range(1500):
+        out.fill_(math.nan)
+        lse.fill_(math.nan)
+        assert L.uv_kv_attend(c._p, 0, seqs.data_ptr(), None, n, n, 1, 1, q.data_ptr(), 4 * heads * d, d, 4 * heads,
+                              1 / math.sqrt(d), out.data_ptr(), lse.data_ptr(), scratch.data_ptr(),
+                              scratch.numel(), st) == 0
+        missed += (out != want).any() | (lse != sums).any()
+    assert int(missed) == 0
+    c.check()
+
+
 @pytest.mark.parametrize("typ", ["float16", "bfloat16"])
 def test_a_long_flat_sequence(uv, typ):
     """150,001 tokens of nearly equal weight: the outputs are 1 / 80 of a value,

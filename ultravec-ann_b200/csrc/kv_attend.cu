@@ -79,6 +79,9 @@ __device__ __forceinline__ Parts carve(void *p, int64_t slots, int cols, int D) 
 __device__ __forceinline__ void set_flag(unsigned long long *p, unsigned long long v) {
   asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
+// Orders what comes before it against what comes after it, stores before loads
+// among them, with every other such fence of the device.
+__device__ __forceinline__ void fence_sc() { asm volatile("fence.sc.gpu;" ::: "memory"); }
 __device__ __forceinline__ unsigned long long get_flag(const unsigned long long *p) {
   unsigned long long v;
   asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
@@ -732,11 +735,16 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       }
       __syncthreads();
       if (tid == 0) set_flag(&sc.flag[part], a.call);
-      // Whoever finds every part written joins them, in their order.  The block
-      // that finishes last does; two that finish together may both, and write
-      // the same bytes.  Nothing waits, and no counter has to start at zero.
+      // Whoever finds every part written joins them, in their order.  Between a
+      // block's own flag and its look at the others' stands a fence.sc: those
+      // fences have one order, and the block whose fence is the last in it sees
+      // every flag (or zeros, from a block that saw them all and joins).  Release
+      // and acquire alone would let two blocks miss each other's.  Two that
+      // finish together may both join, and write the same bytes.  Nothing waits,
+      // and no counter has to start at zero.
       const int64_t first = seg.number + seg.first_block;
       if (warp == 0) {
+        fence_sc();
         __syncwarp();
         bool all = true;
         for (int i = lane; i < seg.blocks; i += 32) all = all && get_flag(&sc.flag[first + i]) == a.call;
