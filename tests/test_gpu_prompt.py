@@ -182,6 +182,22 @@ def test_a_few_rows_behind_many_keys(uv, d, causal):
     compare(out, lse, q, k, v, [3], [70_001], causal, "bfloat16", 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("typ", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,key", [(64, 290), (64, 7), (128, 290), (128, 7)])
+def test_small_weights_beside_a_large_one(uv, typ, d, key):
+    """A key that stands 16 nats above the others and has values of zero: what is
+    left is weights of 1e-7, in as many bits as any others."""
+    rng = np.random.default_rng(d + key)
+    n = 300
+    q, k, v = rows(rng, n, 2, d, typ, 0.3), rows(rng, n, 2, d, typ), rows(rng, n, 2, d, typ, 1000.0)
+    q[:, :, 0] = 4
+    k[:, :, 0] = 0
+    k[key, :, 0] = 16 * math.sqrt(d) / 4
+    v[key] = 0
+    out, lse = uv.prompt_attention(q, k, v, starts([n]), causal=False, lse=True)
+    compare(out, lse, q, k, v, [n], [n], False, typ, 1 / math.sqrt(d))
+
+
 @pytest.mark.parametrize("n", [1, 33, 150])
 def test_many_sequences_of_every_length(uv, n):
     """Entries over all lanes, and more than the ordered search takes."""

@@ -33,7 +33,7 @@
 // Blocks of keys go from the last, masked ones to the first.  A row's weights
 // stand against a reference, the maximum of the first keys that it sees, and no
 // maximum is taken after that: as long as the sums of its weights stay below
-// 2^14 the reference serves as well.  Where one does not, the row takes a new
+// 2^14 (2^15 of halves) the reference serves as well.  Where one does not, the row takes a new
 // reference and its warp rescales O in TMEM.
 //
 // What a row does not see must not reach it, but a weight of zero times a value
@@ -75,7 +75,14 @@ constexpr int kPoly = 2, kPolyOf = 8;
 // (An output waits for its piece's last one; by then at most the next piece's are mended,
 // and 256 rows end within three blocks.)
 constexpr int kMends = 4;
-constexpr float kGrow = 16384.0f;  // weights (sums of 32 of them) up to this stay unanswered
+// Weights (sums of 32 of them) up to kGrow stay unanswered; a row's reference weighs
+// 2^lift.  Halves are exact to 2^-25 at their small end: lifted by 8, a weight keeps 11
+// bits down to 2^-22 of its row's largest, and what the others may grow by, 2^7, is
+// still beyond what the maximum of a row's first keys is usually passed by.
+template <bool BF16>
+struct Weights {
+  static constexpr float kLift = BF16 ? 0.0f : 8.0f, kGrow = BF16 ? 16384.0f : 32768.0f;
+};
 
 __device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
 
@@ -499,6 +506,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + 128 * t, o_at = tmem + lanes + L::kO + 128 * t;
     const float c = __fmul_rn(a.scale, kLog2e);
+    constexpr float kLift = Weights<BF16>::kLift, kGrow = Weights<BF16>::kGrow;
     bool ok = true;
     auto settle = [&](bool fine) {  // the warp goes on, or gives up as one
       ok = __all_sync(0xffffffffu, ok && fine);
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
               }
             }
             // a row that sees a score of +inf or NaN is NaN
-            const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmul_rn(m, -c) : NAN;
+            const float base = m == -INFINITY ? 0.0f : m <= FLT_MAX ? __fmaf_rn(m, -c, kLift) : NAN;
             const f2 cc = pair(c, c), bb = pair(base, base);
             f2 b0 = 0, b1 = 0;
 #pragma unroll
@@ -596,7 +604,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
             }
             sum = add2(b0, b1);
             if (again) break;
-            // weights beyond 2^14 (or NaN): take a new reference and start over
+            // weights beyond kGrow (or NaN): take a new reference and start over
             const float2 v = split(sum);
             need = !(v.x <= kGrow) || !(v.y <= kGrow);
             again = __any_sync(0xffffffffu, need);
@@ -682,7 +690,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       if (live && a.lse != nullptr)
         a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
             none ? -INFINITY
-                 : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum)), kLn2) : NAN;
+                 : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum) - kLift), kLn2) : NAN;
       tc::tc_fence_before();
       release(k);
       if (lane == 0) tc::mbar_arrive(out_done);
