@@ -183,6 +183,26 @@ def test_a_few_rows_behind_many_keys(uv, d, causal):
 
 
 @pytest.mark.parametrize("typ", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,hq,hk", [(64, 2, 1), (128, 4, 2), (128, 3, 1)])
+@pytest.mark.parametrize("excess", [15, 100])
+def test_a_reference_of_few_keys_is_left_where_it_is_too_low(uv, typ, d, hq, hk, excess):
+    """Keys ahead of the queries by no multiple of 128: some rows of a warp see
+    their first keys in a block whose other rows have references already, of a
+    key or a few.  Keys of that block stand above those references by `excess`
+    nats."""
+    rng = np.random.default_rng(excess)
+    nq, nk = [200, 64, 40], [1200, 64, 90]
+    for at in (900, 960, 1023):
+        q, k, v = rows(rng, sum(nq), hq, d, typ, 0.3), rows(rng, sum(nk), hk, d, typ), rows(rng, sum(nk), hk, d, typ)
+        q[:, :, 0] = 4
+        k[:, :, 0] = 0
+        for key in (at, 1200 + 3, 1264 + 45):
+            k[key, :, 0] = excess * math.sqrt(d) / 4
+        out, lse = uv.prompt_attention(q, k, v, starts(nq), starts(nk), lse=True)
+        compare(out, lse, q, k, v, nq, nk, True, typ, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("typ", ["float16", "bfloat16"])
 @pytest.mark.parametrize("d,key", [(64, 290), (64, 7), (128, 290), (128, 7)])
 def test_small_weights_beside_a_large_one(uv, typ, d, key):
     """A key that stands 16 nats above the others and has values of zero: what is

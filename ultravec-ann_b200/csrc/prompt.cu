@@ -542,8 +542,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
           f2 sum;
           uint32_t p[2][16];
           // a row without a reference needs its maximum first; a row that needs
-          // none keeps its own, whoever shares its warp
-          bool need = m == -INFINITY, again = __any_sync(0xffffffffu, need);
+          // none keeps its own, whoever shares its warp; `fresh` has taken its
+          // reference from these keys, so that no weight is above the reference's
+          bool need = m == -INFINITY, again = __any_sync(0xffffffffu, need), fresh = false;
           for (;;) {
             if (again) {
               // (opaque here, so that the maximum is not computed ahead of the branch)
@@ -603,10 +604,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
               p[e / 32][e % 32 / 2] = kv::pack2<BF16>(y.x, y.y);
             }
             sum = add2(b0, b1);
-            if (again) break;
-            // weights beyond kGrow (or NaN): take a new reference and start over
+            // weights beyond kGrow (or NaN): take a new reference and start over, once
+            // at most for a row (also where the warp is here for another row's first keys)
             const float2 v = split(sum);
-            need = !(v.x <= kGrow) || !(v.y <= kGrow);
+            fresh = fresh || need;
+            need = !fresh && (!(v.x <= kGrow) || !(v.y <= kGrow));
             again = __any_sync(0xffffffffu, need);
             if (!again) break;
           }
