@@ -218,6 +218,38 @@ def test_small_weights_beside_a_large_one(uv, typ, d, key):
     compare(out, lse, q, k, v, [n], [n], False, typ, 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_one_score_that_is_no_number(uv, d, causal):
+    """One key that gives NaN or +inf makes every row that sees it NaN, wherever in
+    a block it lies; one that gives -inf weighs nothing."""
+    import torch
+
+    rng = np.random.default_rng(d)
+    n = 300
+    q, k, v = rows(rng, n, 2, d, "bfloat16"), rows(rng, n, 1, d, "bfloat16"), rows(rng, n, 1, d, "bfloat16")
+    q[:, :, 3] = 1
+    k[:, :, 3] = 0
+    want = uv.prompt_attention(q, k, v, starts([n]), causal=causal)
+    for key in (1, 2, 3, 4, 5, 6, 7, 8, 64, 127, 128, 129, 200, 299):
+        first = key if causal else 0
+        for bad in (math.nan, math.inf):
+            kk = k.clone()
+            kk[key, :, 3] = bad
+            got, lse = uv.prompt_attention(q, kk, v, starts([n]), causal=causal, lse=True)
+            assert bool(got[first:].isnan().all()), (key, bad)
+            assert bool(lse[first:].isnan().all()), (key, bad)
+            assert torch.equal(got[:first], want[:first])
+        kk[key, :, 3] = -math.inf
+        got, lse = uv.prompt_attention(q, kk, v, starts([n]), causal=causal, lse=True)
+        kk[key, :, 3] = -1e6  # a score of -88,000 at the least: a weight of zero
+        a, wl, size, reach = M.prompt(f64(q), f64(kk), f64(v), causal, 1 / math.sqrt(d))
+        kk[key] = 0
+        reach = M.prompt(f64(q), f64(kk), f64(v), causal, 1 / math.sqrt(d))[3]
+        assert (np.abs(f64(got) - a) <= tolerance(a, size, reach, "bfloat16")).all(), key
+        assert (np.abs(f64(lse) - wl) <= 2.0 ** -17 * reach + 2.0 ** -13).all()
+
+
 @pytest.mark.parametrize("n", [1, 33, 150])
 def test_many_sequences_of_every_length(uv, n):
     """Entries over all lanes, and more than the ordered search takes."""

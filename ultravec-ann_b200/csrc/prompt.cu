@@ -135,13 +135,12 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
 }
 
 // 2^x for two x in the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by the
-// polynomial of degree 4, n added to the exponent.  x above 127 gives 2^127 (the
-// caller takes a new reference then), below -126 2^-126
-// (the caller makes masked weights exact zeros) and so does NaN (the caller's
-// row has NaN from its other columns then).
+// polynomial of degree 4, n added to the exponent.  x above 127 gives 2^127, and so
+// does NaN (the caller takes a new reference then, which makes the row NaN where a
+// score was), below -126 2^-126 (the caller makes masked weights exact zeros).
 __device__ __forceinline__ float2 exp2_poly(f2 x) {
   const float2 v = split(x);
-  x = pair(fminf(fmaxf(v.x, -126.0f), 127.0f), fminf(fmaxf(v.y, -126.0f), 127.0f));
+  x = pair(fmaxf(fminf(v.x, 127.0f), -126.0f), fmaxf(fminf(v.y, 127.0f), -126.0f));
   const f2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
   const f2 n = add2(x, magic), whole = add2(n, minus);
   const f2 f = fma2(whole, pair(-1.0f, -1.0f), x);
