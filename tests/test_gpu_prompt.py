@@ -300,6 +300,32 @@ def test_more_work_than_blocks(uv, d, hq, causal):
     compare(out, lse, q, k, clean, nq, nk, causal, "bfloat16", 1 / math.sqrt(d))
 
 
+@pytest.mark.parametrize("d,causal", [(64, True), (128, True), (128, False)])
+def test_marks_of_every_piece(uv, d, causal):
+    """Infinities in nearly every piece of work, in columns of their own: each
+    piece's marks stay until its rows are out, call after call."""
+    import torch
+
+    rng = np.random.default_rng(d)
+    nq = [int(x) for x in rng.integers(1, 140, 150)]
+    q, k, v = (rows(rng, sum(nq), h, d, "bfloat16") for h in (8, 2, 2))
+    a = np.concatenate([[0], np.cumsum(nq)])
+    where = []
+    for i in range(150):
+        key, col = a[i] + int(rng.integers(0, nq[i])), int(rng.integers(0, d))
+        where.append((i, key, col))
+        v[key, :, col] = math.inf
+    want = uv.prompt_attention(q, k, v, starts(nq), causal=causal)
+    inf = torch.zeros_like(want, dtype=torch.bool)
+    for i, key, col in where:
+        inf[key if causal else a[i]:a[i + 1], :, col] = True
+    assert torch.equal(want == math.inf, inf) and not bool(want.isnan().any())
+    differ = torch.zeros((), device="cuda")
+    for _ in range(300):
+        differ += (uv.prompt_attention(q, k, v, starts(nq), causal=causal) != want).any()
+    assert int(differ) == 0
+
+
 def test_refused_arguments(uv):
     import torch
 

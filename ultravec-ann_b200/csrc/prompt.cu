@@ -693,8 +693,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
             none ? -INFINITY
                  : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum) - kLift), kLn2) : NAN;
       tc::tc_fence_before();
-      release(k);
+      // (in this order: who finds piece k + 2 finds out_done past piece k, so that a
+      // wait for piece k + 1 by its parity cannot take piece k's phase for it)
+      __syncwarp();
       if (lane == 0) tc::mbar_arrive(out_done);
+      release(k);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kLess));
