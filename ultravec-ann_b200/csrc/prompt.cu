@@ -433,6 +433,18 @@ __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   return true;
 }
 
+// A piece of work that nobody will do: NaN rows, by one warp.
+template <int TILES, int D>
+__device__ __noinline__ void void_rows(uint32_t *out, float *lse, int q_heads, const Item &it) {
+  const int lane = threadIdx.x & 31;
+  for (int t = 0; t < TILES; t++)
+    for (int row = it.i0[t]; row < min(it.i0[t] + kRows, it.nq); row++) {
+      const int64_t at = (int64_t)(it.q0 + row) * q_heads + it.head[t];
+      for (int i = lane; i < D / 2; i += 32) out[at * (D / 2) + i] = 0x7fff7fffu;
+      if (lane == 0 && lse != nullptr) lse[at] = NAN;
+    }
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     prompt_kernel(const Args a, const __grid_constant__ CUtensorMap qmap,
@@ -453,7 +465,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
 
   // Pieces of work in turn, as the loading warp finds them: a block does its own
   // and then those of blocks that have not started.
-  __shared__ Item items[2];
+  __shared__ Item items[2], lost;
   __shared__ int last_item[2], any_odd[2];  // no work left; values that are no numbers were found
   __shared__ __align__(16) uint4 answer;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -795,11 +807,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
     int block = blockIdx.x, k = 0;
     int answers = 0, queries[2] = {0, 0};
     int64_t issued = 0;
-    bool waiting = true;
+    bool waiting = true, stuck = false;
     if (lane == 0) ask_next(&answer, asked);
     for (;;) {
       if (k >= 2 && !__all_sync(0xffffffffu, wait_long(&item_empty[k & 1], (k >> 1) - 1))) {
         *abort_s = 1;
+        stuck = true;
         break;
       }
       Item &it = items[k & 1];
@@ -849,6 +862,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       if (waiting && lane == 0) {
         tc::fence_async_smem();
         ask_next(&answer, asked);
+      }
+    }
+    if (stuck) {
+      // The piece in hand and the one asked for, whose answer is still to land, are
+      // no other block's.
+      const int next = waiting && __all_sync(0xffffffffu, wait_for(asked, answers)) ? answer_of(&answer) : -1;
+      for (int i = 0; i < 2; i++) {
+        const bool some = (i ? next : block) >= 0 && find_item<kTiles>(a, i ? next : block, &lost);
+        __syncwarp();
+        if (some) void_rows<kTiles, D>((uint32_t *)a.out, a.lse, a.q_heads, lost);
+        __syncwarp();
       }
     }
     if (lane == 0 && *abort_s) {  // no copy may land after the block is gone
