@@ -316,6 +316,36 @@ def test_one_long_sequence_and_many_ragged_ones_split_alike(uv):
         assert (np.abs(f64(alone) - want) <= attend_tolerance(want, size, reach, "bfloat16")).all()
 
 
+@pytest.mark.parametrize("lens", [[1], [40], [6000], [20_000, 3]])
+def test_queries_and_keys_that_are_no_numbers(uv, lens):
+    """NaN in a query makes its own row NaN and no other, however its job is split;
+    so does a key of NaN for the rows that see it."""
+    import torch
+
+    rng = np.random.default_rng(27)
+    c, _ = cache(uv, 128, 1, lens)
+    fill(c, lens, 128, 1, "bfloat16", rng)
+    n, seqs = len(lens), ints(range(len(lens)))
+    q = rows_of(rng, n, 8, 128, "bfloat16", False)
+    want, sums = c.attend(seqs, q, lse=True)
+    for bad in (math.nan, math.inf):
+        x = q.clone()
+        x[0, 2, 5] = bad
+        got, lse = c.attend(seqs, x, lse=True)
+        assert bool(got[0, 2].isnan().all()) and bool(lse[0, 2].isnan())
+        for a, b in ((got, want), (lse, sums)):
+            a[0, 2] = b[0, 2]
+            assert torch.equal(a, b)
+    k = rows_of(rng, 1, 1, 128, "bfloat16")
+    for bad in (math.nan, math.inf):
+        k[0, 0, 9] = bad
+        c.append(ints([0]), k, torch.zeros_like(k))
+        got, lse = c.attend(seqs, q, lse=True)
+        assert bool(got[0].isnan().all()) and bool(lse[0].isnan().all())
+        assert torch.equal(got[1:], want[1:]) and torch.equal(lse[1:], sums[1:])
+    c.check()
+
+
 @pytest.mark.parametrize("lens", [[20_000], [9000, 40, 7000, 300], [2500] * 24])
 def test_every_split_job_is_joined_every_time(uv, lens):
     """Outputs that hold NaN before the call have the same bits after each of many

@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int k = 0; k < 2; k++) {
-            float top = fmaxf(fmaxf(s[0][nt][k], s[0][nt][2 + k]), fmaxf(s[1][nt][k], s[1][nt][2 + k]));
+            float top = max_nan(max_nan(s[0][nt][k], s[0][nt][2 + k]), max_nan(s[1][nt][k], s[1][nt][2 + k]));
             float vtop = 0.0f;
 #pragma unroll
             for (int sb = 0; sb < 2; sb++)
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
                 if ((whole || seen(nt, k, sb, r)) && vs[sb][r] <= FLT_MAX) vtop = fmaxf(vtop, vs[sb][r]);
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) {
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
               vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
             }
             const bool none = m[nt][k] == -INFINITY;
@@ -645,6 +645,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     }
 
     // ---- join the warps' parts: 2 and 3 leave theirs, 0 and 1 add to them ----
+    // (maxima of maxima keep NaN: a column that has met nothing but NaN is not one
+    // that has seen nothing)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
           for (int k = 0; k < 2; k++) {
             const int col = 8 * nt + 2 * t + k;
             float top = join_m[0][col];
-            for (int v = 1; v < kWarps; v++) top = fmaxf(top, join_m[v][col]);
+            for (int v = 1; v < kWarps; v++) top = max_nan(top, join_m[v][col]);
             // a warp without a visible token adds nothing, whatever its sums hold
             const bool none = m[nt][k] == -INFINITY;
             const float f = __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
@@ -694,7 +696,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     auto total_of = [&](int col, float *top) {
       float sum = 0.0f;
       *top = join_m[0][col];
-      for (int v = 1; v < kWarps; v++) *top = fmaxf(*top, join_m[v][col]);
+      for (int v = 1; v < kWarps; v++) *top = max_nan(*top, join_m[v][col]);
       for (int v = 0; v < kWarps; v++)
         if (join_m[v][col] != -INFINITY)
           sum = __fmaf_rn(join_l[v][col], exp2_fast(__fsub_rn(join_m[v][col], *top)), sum);
@@ -760,8 +762,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         for (int col = warp; col < kCols; col += kWarps) {
           float top = -INFINITY, sum = 0.0f, acc[V];
           for (int i = lane; i < seg.blocks; i += 32)
-            top = fmaxf(top, __ldcg(&sc.ml[(first + i) * kCols + col]).x);
-          for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            top = max_nan(top, __ldcg(&sc.ml[(first + i) * kCols + col]).x);
+          for (int x = 16; x; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
 #pragma unroll
           for (int v = 0; v < V; v++) acc[v] = 0.0f;
           for (int i0 = 0; i0 < seg.blocks; i0 += 32) {

@@ -331,6 +331,12 @@ __device__ __forceinline__ void rotate_back(const Cache &c, float (&y)[2][D / 4]
   }
 }
 
+// The larger one, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 // 2^e as a float, e in [-126, 127].
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }
 // floor(log2 |x|) of a normal x (-127 for zero and subnormals, 128 for inf and NaN).
