@@ -346,6 +346,98 @@ def test_queries_and_keys_that_are_no_numbers(uv, lens):
     c.check()
 
 
+def crowd(uv, d, n, many):
+    """A cache of one head whose first sequence has n tokens; `many` in all share its
+    pages, so that a warp goes through many tiles of a job."""
+    c = uv.KvCache(d, 1, -(-n // 64) + 2, many, n + 64, seed=7)
+    c.extend(ints([0]), ints([n]))
+    c.check()
+    signs = np.array([[-1.0 if c._desc.signs[0][i // 32] >> (i % 32) & 1 else 1.0 for i in range(d)]])
+    return Shared(c, many), signs
+
+
+class Shared:
+    """Appends while the first sequence is alone, attends with everyone."""
+
+    def __init__(self, c, many):
+        self.c, self.rest = c, ints(range(1, many))
+        self.pool, self.table = c.pool, c.table
+
+    def append(self, *a):
+        self.c.free(self.rest)
+        self.c.append(*a)
+        self.c.fork(ints([0] * len(self.rest)), self.rest)
+
+    def attend(self, *a):
+        return self.c.attend(*a)
+
+    def check(self):
+        self.c.check()
+
+
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 1), (128, 4), (256, 2)])
+@pytest.mark.parametrize("typ", ["float16", "bfloat16"])
+def test_values_beside_larger_ones_of_no_weight(uv, typ, d, group):
+    """A token of negligible weight whose values are 2^12 to 2^40 times the others'
+    takes nothing from them: the bound is that of the roundings, which is of the
+    weighted values' size."""
+    import torch
+
+    rng = np.random.default_rng(d + group)
+    n = 300
+    c, signs = crowd(uv, d, n, 400)
+    r = M.rotation(signs)
+    for at, size in ((0, 2.0 ** 12), (17, 2.0 ** 14), (40, 2.0 ** 15), (150, 2.0 ** 20), (290, 2.0 ** 24), (31, 2.0 ** 40)):
+        k, v = (rows_of(rng, n, 1, d, "bfloat16", False) * 0.3 for _ in range(2))
+        k[:, :, 0] = 0
+        k[at, :, 0] = -90 * math.sqrt(d) / 4
+        v[at] = v[at] * size
+        c.append(ints([0]), k, v, starts([n]))
+        q = rows_of(rng, 3, group, d, typ, False) * 0.3
+        q[:, :, 0] = 4
+        out = c.attend(ints(range(400)), q.repeat(400, 1, 1), starts([3] * 400), 3)
+        want, _, big, reach = M.attend(f64(q), M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d),
+                                       r, 1 / math.sqrt(d))
+        # the scores that count are those of keys that weigh: reach without the odd one
+        near = M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d)
+        near[0][1][:, at] = 0
+        reach = M.attend(f64(q), near, r, 1 / math.sqrt(d))[3]
+        err = np.abs(f64(out).reshape(400, *want.shape) - want)
+        assert (err <= attend_tolerance(want, big, reach, typ)).all(), (at, size)
+    c.check()
+
+
+@pytest.mark.parametrize("typ", ["float16", "bfloat16"])
+@pytest.mark.parametrize("up", [True, False])
+def test_weights_and_values_that_run_against_each_other(uv, typ, up):
+    """Scores rise by 40 nats along 500 tokens while the values shrink as much (or
+    the reverse), so that every token adds as much to the output."""
+    import torch
+
+    rng = np.random.default_rng(25)
+    n, d = 500, 64
+    c, signs = crowd(uv, d, n, 400)
+    r = M.rotation(signs)
+    climb = torch.linspace(-20, 20, n, device="cuda") * (1 if up else -1)
+    k, v = (rows_of(rng, n, 1, d, "float32", False) for _ in range(2))
+    q = rows_of(rng, 4, 2, d, "float32", False) * 0.1
+    q[:, :, 0] = 4
+    k *= 0.05
+    k[:, 0, 0] = climb * math.sqrt(d) / 4
+    q, k = q.to(getattr(torch, typ)), k.bfloat16()
+    c.append(ints([0]), k, k, starts([n]))
+    (kl, ks), _ = M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d)
+    e = (kl[0] * ks[0][:, None]) @ (f64(q)[0, 0] @ r.T) / math.sqrt(d)  # what the held keys score
+    v = ((1 + 0.3 * v.double()) * torch.tensor(1e7 * np.exp(-e), device="cuda")[:, None, None]).bfloat16()
+    c.append(ints([0]), k, v, starts([n]))
+    out = c.attend(ints(range(400)), q.repeat(400, 1, 1), starts([4] * 400), 4)
+    held = M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d)
+    want, _, size, reach = M.attend(f64(q), held, r, 1 / math.sqrt(d))
+    err = np.abs(f64(out).reshape(400, *want.shape) - want)
+    assert (err <= attend_tolerance(want, size, reach, typ)).all()
+    c.check()
+
+
 @pytest.mark.parametrize("lens", [[20_000], [9000, 40, 7000, 300], [2500] * 24])
 def test_every_split_job_is_joined_every_time(uv, lens):
     """Outputs that hold NaN before the call have the same bits after each of many

@@ -29,8 +29,9 @@
 // times the sum, is taken off: from the scores at once, from the outputs every
 // four tiles.  Scores, maxima and sums are f32.  The weights are rounded to halves
 // after the multiplication by their token's value scale, itself divided by a power
-// of two that follows the largest scale seen, so they neither overflow nor lose
-// more than 2^-11: beside bf16 rows an eighth of the output's own rounding, beside
+// of two that follows the largest scale seen, but stays within 2^6 of the largest
+// product of scale and weight (a large value that weighs nothing takes no bits from
+// the others), so they neither overflow nor lose more than 2^-11: beside bf16 rows an eighth of the output's own rounding, beside
 // halves as much again (0.00034 of the result's size off in all, where exact
 // weights are 0.00021 off), so there the remainder goes along too; that product
 // costs 8 rows over 4.5k tokens each 0.7 us of 23.  The running maximum moves only when a score exceeds it by
@@ -47,6 +48,7 @@ constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kJump = 8.0f;     // log2 of what a score may exceed its reference by
 constexpr float kSpread = 16.0f;  // what a value scale may exceed its reference by
+constexpr int kAbove = 6;         // log2 of what that may exceed a scale times its weight by
 
 // Blocks an SM: three where the sums and the query's fragments leave room in
 // 168 registers, else two with the longer rings that then fit.
@@ -537,23 +539,35 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             float top = max_nan(max_nan(s[0][nt][k], s[0][nt][2 + k]), max_nan(s[1][nt][k], s[1][nt][2 + k]));
-            float vtop = 0.0f;
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const bool none = m[nt][k] == -INFINITY;
+            const float up = none ? top : top > kJump ? top : 0.0f;  // what m grows by
+            // the largest value scale, and the largest of them times its weight
+            float vtop = 0.0f, wtop = 0.0f;
 #pragma unroll
             for (int sb = 0; sb < 2; sb++)
 #pragma unroll
               for (int r = 0; r < 2; r++)
-                if ((whole || seen(nt, k, sb, r)) && vs[sb][r] <= FLT_MAX) vtop = fmaxf(vtop, vs[sb][r]);
+                if ((whole || seen(nt, k, sb, r)) && vs[sb][r] <= FLT_MAX) {
+                  vtop = fmaxf(vtop, vs[sb][r]);
+                  wtop = fmaxf(wtop, __fmul_rn(exp2_fast(__fsub_rn(s[sb][nt][2 * r + k], up)),
+                                               __fmul_rn(vs[sb][r], 0x1p-16f)));
+                }
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) {
-              top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
               vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, x));
+              wtop = fmaxf(wtop, __shfl_xor_sync(0xffffffffu, wtop, x));
             }
-            const bool none = m[nt][k] == -INFINITY;
-            const float up = none ? top : top > kJump ? top : 0.0f;  // what m grows by
-            const int ne = __fmul_rn(vtop, down[nt][k]) > kSpread ? min(log2i(vtop), 126) : ve[nt][k];
+            // What the sums hold shrinks with m, and the reference of their values
+            // with it; it rises for values of weight, to 2^kAbove times them at most.
+            const float grown = none ? 0.0f : up;
+            const int kept = max(ve[nt][k] - (int)fminf(grown, 1000.0f), -100);
+            const int risen = min(min(log2i(vtop), log2i(wtop) + 16 + kAbove), 126);
+            const int ne = __fmul_rn(vtop, exp2i(-kept)) > kSpread ? max(kept, risen) : kept;
             // (a column that has seen nothing has sums of zero: any factor keeps them)
-            const float f = none ? 1.0f : exp2_fast(-up);
-            const float both = __fmul_rn(f, exp2_fast((float)(ve[nt][k] - ne)));
+            const float f = exp2_fast(-grown);
+            const float both = exp2_fast(__fsub_rn((float)(ve[nt][k] - ne), grown));
             if (none) m[nt][k] = top;
             else m[nt][k] = __fadd_rn(m[nt][k], up);
             ve[nt][k] = ne;
@@ -585,7 +599,7 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
             for (int r = 0; r < 2; r++) {
               const float e = exp2_fast(s[sb][nt][2 * r + k]);
               l[nt][k] = __fadd_rn(l[nt][k], e);
-              w[2 * r + k] = __fmul_rn(e, __fmul_rn(vs[sb][r], down[nt][k]));
+              w[2 * r + k] = __fmul_rn(__fmul_rn(e, down[nt][k]), vs[sb][r]);
             }
           if (!whole)  // a token that is not seen weighs nothing even if its scale is no number
 #pragma unroll
