@@ -153,6 +153,27 @@ def test_rows_of_zeros_extremes_and_numbers_that_are_none(uv):
     check_rows(c, (k[7:], k[7:]), r, 0, 7, 128)
 
 
+def test_entries_without_rows_in_an_append(uv):
+    """A forked sequence that idles in a step: its last page stays shared, and the
+    other entries' rows are written."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    for n in (69, 70, 79, 81):
+        c, signs = cache(uv, 64, 2, [n, 40], extra=9)
+        c.fork(ints([0]), ints([2]))
+        k, v = (rows_of(rng, 3, 2, 64, "float16") for _ in range(2))
+        for order, counts, at in (([1, 2], [3, 0], [0, 3, 3]), ([2, 1], [0, 3], [0, 0, 3])):
+            c.extend(ints(order), ints(counts))
+            c.append(ints(order), k, v, ints(at))
+            c.check()
+            check_rows(c, (k, v), M.rotation(signs), 1, int(c.lens[1]) - 3, 64)
+        before = c.pool.clone()
+        c.append(ints([0, 2]), k[:0], v[:0], ints([0, 0, 0]))
+        c.check()
+        assert torch.equal(before, c.pool)
+
+
 def test_strided_rows_and_other_orders(uv):
     """Heads before rows, rows of a wider tensor, a misaligned view."""
     import torch

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
   const Block at = find_block(rows, c, item / groups);
   const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
   if (s < 0 && lane == 0) atomicOr(&c.work[kStatus], kBadSeq);
-  if (pos0 >= len) return;
+  if (pos0 >= len || begin >= len) return;  // no position, or an entry of no rows
   const int page = c.page_at(s, pos0 / c.page_tokens);
   if (c.refs[page] != 1) {  // others hold it: extend has not made room
     if (lane == 0) atomicOr(&c.work[kStatus], kShared);
