@@ -554,10 +554,12 @@ int uv_coset_reconstruct(const uv_coset *coset, const float *rows, int64_t n, fl
  * attention and reads may overlap.  The calls hold nothing of their own:
  * attention takes scratch (or allocates it in stream order).
  *
- * What the device alone can see to be wrong (a sequence number out of range or
- * listed twice, no free page) does not change the cache: the call sets bits of
- * a status word, and every later call that would change the cache does nothing
- * until uv_kv_check has read it. */
+ * What the device alone can see to be wrong in a call that changes the cache (a
+ * sequence number out of range or listed twice, no free page, rows for a shared
+ * page) does not change it at all: the call sets bits of a status word, and
+ * every later call that would change the cache does nothing until uv_kv_check
+ * has read it.  To a read or an attention a sequence out of range is an empty
+ * one, and a sequence may be listed more than once. */
 #define UV_F16 0
 #define UV_BF16 1
 
@@ -627,7 +629,7 @@ int uv_kv_compact(const uv_kv *kv, void *stream);
  * Element [row][head][i] of an input is at row * row_stride + head *
  * head_stride + i; strides are multiples of 8, bases 16-byte aligned.  The
  * starts rise from 0 to rows.
- * append writes them (extend has made the room); read returns them as they are
+ * append writes them, all or none (extend has made the room); read returns them as they are
  * held, dense (rows without a token as zeros). */
 int uv_kv_append(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int32_t *starts,
                  int32_t n, int32_t rows, int32_t dtype, const void *k, int64_t k_row_stride,

@@ -174,6 +174,60 @@ def test_entries_without_rows_in_an_append(uv):
         assert torch.equal(before, c.pool)
 
 
+@pytest.mark.parametrize("bad,counts,status", [
+    ([0, 9, 1], [40, 5, 70], 2),       # out of range
+    ([0, -1, 1], [40, 5, 70], 2),
+    ([0, 1, 0], [40, 70, 40], 2),      # listed twice
+    ([1, 0, 1], [70, 1, 0], 2),
+    ([0, 2, 1], [40, 6, 70], 16),      # its last page is shared
+    ([0, 3, 1], [40, 1, 70], 16),
+    ([2, 9, 2], [6, 5, 6], 2 | 16),
+    ([0, 1, 2], [40, 70, 100], 16),    # a page before the last
+])
+def test_an_append_with_a_bad_entry_writes_nothing(uv, bad, counts, status):
+    import torch
+
+    rng = np.random.default_rng(22)
+    c, signs = cache(uv, 128, 2, [40, 70, 100, 0, 0], extra=9)
+    c.fork(ints([2]), ints([3]))
+    k, v = (rows_of(rng, sum(counts), 2, 128, "bfloat16") for _ in range(2))
+    before = c.pool.clone()
+    for _ in range(3):
+        c.append(ints(bad), k, v, starts(counts))
+        c.append(ints([0]), k[:1], v[:1])  # stopped by the status
+    assert torch.equal(before, c.pool)
+    with pytest.raises(uv.KvError) as e:
+        c.check()
+    assert e.value.status == status
+    k, v = (rows_of(rng, 74, 2, 128, "bfloat16") for _ in range(2))
+    c.append(ints([1, 0]), k, v, starts([70, 4]))
+    c.check()
+    check_rows(c, (k[:70], v[:70]), M.rotation(signs), 1, 0, 128)
+
+
+def test_an_append_looks_over_more_entries_than_threads(uv):
+    import torch
+
+    rng = np.random.default_rng(23)
+    m = 2100
+    c = uv.KvCache(64, 1, 2 * m + 10, m + 1, 96, page_tokens=32)
+    n = [int(x) for x in rng.integers(0, 70, m)]
+    order = [int(x) for x in rng.permutation(m)]
+    c.extend(ints(order), ints([n[i] for i in order]))
+    some = [min(n[i], int(x)) for i, x in zip(order, rng.integers(0, 70, m))]
+    k, v = (rows_of(rng, sum(some), 1, 64, "float16") for _ in range(2))
+    c.append(ints(order), k, v, starts(some))
+    c.check()
+    kb, vb = c.read(ints(order), starts(some), sum(some))
+    for x, y in ((k, kb), (v, vb)):
+        assert float((x.double() - y.double()).norm() / x.double().norm()) < 0.13  # 4 bits: 0.107
+    before = c.pool.clone()
+    c.append(ints(order[:-1] + order[5:6]), k, v, starts(some))
+    with pytest.raises(uv.KvError) as e:
+        c.check()
+    assert e.value.status == 2 and torch.equal(before, c.pool)
+
+
 def test_strided_rows_and_other_orders(uv):
     """Heads before rows, rows of a wider tensor, a misaligned view."""
     import torch

@@ -65,26 +65,70 @@ __device__ __forceinline__ uint32_t pack_codes(const float *t) {
   return w - 0x4b400000u * 0x11111111u;
 }
 
+// What an append must find before its first byte is written: sequences in range,
+// none listed twice, and pages that nobody else holds (extend has made room).  One
+// block, as the page operations decide; a lane looks at one entry's page or two, and
+// where there are more (prompts) its warp shares them.  Beside the rows' own loads and
+// rotations it costs 2 us of 67 (8 prompts), and a launch of 3 us where the host bounds
+// the call.
+constexpr int kCheckThreads = 1024;
+__global__ void __launch_bounds__(kCheckThreads) append_check_kernel(Cache c, Rows rows) {
+  __shared__ int errors;
+  pdl_launch();
+  const int before = c.work[kStatus];  // (looked at in the end: it waits for nothing)
+  if (threadIdx.x == 0) errors = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int bad = 0;
+  for (int i0 = 0; i0 < rows.n; i0 += kCheckThreads) {
+    const int i = i0 + lane * (kCheckThreads / 32) + warp;  // a few long ones: a warp each
+    int s = -1, from = 0, to = -1;  // columns that the rows lie in
+    if (i < rows.n) {
+      s = rows.seq(i, c.max_seqs);
+      if (s < 0) {
+        bad |= kBadSeq;
+      } else {
+        const int len = c.length(s), n = min(rows.count(i), len);
+        if (n > 0) from = (len - n) / c.page_tokens, to = (len - 1) / c.page_tokens;
+        if (atomicExch(&c.mark()[s], 1) != 0) bad |= kBadSeq;
+      }
+    }
+    auto look = [&](int seq, int column) {
+      if (c.refs[c.page_at(seq, column)] != 1) bad |= kShared;
+    };
+    if (from <= to) look(s, from);
+    if (from < to) look(s, to);
+    for (uint32_t more = __ballot_sync(0xffffffffu, to - from > 1); more; more &= more - 1) {
+      const int who = __ffs(more) - 1;
+      const int seq = __shfl_sync(0xffffffffu, s, who), lo = __shfl_sync(0xffffffffu, from, who);
+      const int hi = __shfl_sync(0xffffffffu, to, who);
+      for (int column = lo + 1 + lane; column < hi; column += 32) look(seq, column);
+    }
+  }
+  if (bad) atomicOr(&errors, bad);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows.n; i += kCheckThreads) {
+    const int s = rows.seq(i, c.max_seqs);
+    if (s >= 0) c.mark()[s] = 0;
+  }
+  if (threadIdx.x == 0 && errors && before == 0) c.work[kStatus] = errors;
+}
+
 // A warp takes `each` of a block's 2 * heads parts (keys and values of a head),
 // which share what finding the block took: four dependent loads.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer, Rows rows,
                                                              Strided kin, Strided vin, int64_t blocks,
                                                              int each) {
-  if (c.work[kStatus] != 0) return;  // an extend failed: these rows have no place
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t item = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
   const int parts = 2 * c.heads, groups = (parts + each - 1) / each;
-  if (item >= blocks * groups) return;
+  if (item >= blocks * groups) return pdl_wait();
   const Block at = find_block(rows, c, item / groups);
   const int s = at.seq, len = at.len, pos0 = at.pos0, begin = at.begin, first = at.first;
-  if (s < 0 && lane == 0) atomicOr(&c.work[kStatus], kBadSeq);
-  if (pos0 >= len || begin >= len) return;  // no position, or an entry of no rows
+  // (every block waits for the check, also to end: what follows is ordered behind both)
+  if (pos0 >= len || begin >= len) return pdl_wait();  // no position, or an entry of no rows
   const int page = c.page_at(s, pos0 / c.page_tokens);
-  if (c.refs[page] != 1) {  // others hold it: extend has not made room
-    if (lane == 0) atomicOr(&c.work[kStatus], kShared);
-    return;
-  }
   const bool live[2] = {pos0 + g >= begin && pos0 + g < len, pos0 + g + 8 >= begin && pos0 + g + 8 < len};
   const int from = (int)(item % groups) * each, to_part = min(from + each, parts);
   for (int part = from; part < to_part; part++) {
@@ -107,6 +151,11 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
     }
     float y[2][D / 4];
     rotate_rows<D, BF16, 2, false>(c, a, y);
+    if (part == from) {
+      pdl_wait();
+      // an extend failed, so that these rows have no place, or the check found an entry bad
+      if (c.work[kStatus] != 0) return;
+    }
 
     uint8_t *tile = c.tile_at(layer, page, head, pos0 % c.page_tokens / kTile) +
                     (value ? kTile * (D / 2 + 4) : 0);
@@ -312,8 +361,20 @@ static cudaError_t append_d(const Cache &c, int layer, const Rows &rows, const S
   const int each = parts_each(blocks, c.heads);
   const int64_t warps = blocks * ((2 * c.heads + each - 1) / each);
   const int64_t grid = (warps + kRowThreads / 32 - 1) / (kRowThreads / 32);
-  append_kernel<D, BF16><<<(unsigned)grid, kRowThreads, 0, st>>>(c, layer, rows, k, v, blocks, each);
-  return cudaGetLastError();
+  append_check_kernel<<<1, kCheckThreads, 0, st>>>(c, rows);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // finds its places while the check runs, and waits for it before it writes
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, append_kernel<D, BF16>, c, layer, rows, k, v, blocks, each);
 }
 template <int D, bool BF16>
 static cudaError_t read_d(const Cache &c, int layer, const Rows &rows, void *k, void *v,
