@@ -228,6 +228,36 @@ def test_an_append_looks_over_more_entries_than_threads(uv):
     assert e.value.status == 2 and torch.equal(before, c.pool)
 
 
+@pytest.mark.parametrize("d,rounds", [(64, 1), (128, 1), (256, 1), (128, 2), (256, 3)])
+def test_rows_near_the_largest_number(uv, d, rounds):
+    """Rows whose transform would pass the largest float before it is scaled."""
+    import torch
+
+    rng = np.random.default_rng(24)
+    sizes = [1e30, 1e34, 1e36, 1e37, 3e38, 1.0, 1e-30, 1e37, 3.3e38]
+    c, signs = cache(uv, d, 1, [len(sizes)], rounds=rounds)
+    r = M.rotation(signs)
+    k = rows_of(rng, len(sizes), 1, d, "float32", False).double()
+    k = k / k.abs().amax(-1, keepdim=True) * torch.tensor(sizes, device="cuda", dtype=torch.float64)[:, None, None]
+    k[4] = 3e38  # as large in every dimension: one entry of the transform is sqrt(d) times that
+    k[7, 0, 1:] = 0
+    k = k.float().bfloat16()
+    v = k.flip(0).contiguous()
+    c.append(ints([0]), k, v, starts([len(sizes)]))
+    c.check()
+    check_rows(c, (k, v), r, 0, 0, d)
+    assert bool(torch.isfinite(held_scales(c, d)).all())
+
+
+def held_scales(c, d):
+    """The scales of a cache's first sequence, keys and values."""
+    import torch
+
+    n = int(c.lens[0])
+    (_, ks), (_, vs) = M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d)
+    return torch.tensor(np.stack([ks, vs]))
+
+
 def test_strided_rows_and_other_orders(uv):
     """Heads before rows, rows of a wider tensor, a misaligned view."""
     import torch

@@ -65,6 +65,19 @@ __device__ __forceinline__ uint32_t pack_codes(const float *t) {
   return w - 0x4b400000u * 0x11111111u;
 }
 
+// floor(log2) of the largest magnitude in a row of bfloats that four lanes hold (what
+// exp2i takes, both ways: 126 at most), 0 where the row has an infinity or a NaN (which then stays what it is).
+template <int D>
+__device__ __forceinline__ int bfloat_exponent(const uint32_t (&a)[D / 8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < D / 8; j++) top = __vmaxu2(top, a[j] & 0x7fff7fffu);
+  top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int e = (int)(max(top >> 16, top & 0xffffu) >> 7);
+  return e == 255 ? 0 : max(min(e, 253), 27) - 127;
+}
+
 // What an append must find before its first byte is written: sequences in range,
 // none listed twice, and pages that nobody else holds (extend has made room).  One
 // block, as the page operations decide; a lane looks at one entry's page or two, and
@@ -136,21 +149,57 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
     const bool value = part & 1;
     const Strided &in = value ? vin : kin;
     const uint16_t *src = (const uint16_t *)in.p + (int64_t)head * in.head + t * (D / 4);
-    uint32_t a[2][D / 8];
+    float y[2][D / 4], square[2], grow[2] = {1.0f, 1.0f};
+    auto squares = [&](int r) {
+      float some = 0.0f, more = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const uint4 *q = (const uint4 *)(src + (int64_t)(first + pos0 + g + 8 * r) * in.row);
-#pragma unroll
-      for (int i = 0; i < D / 32; i++) {
-        const uint4 w = live[r] ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
-        a[r][4 * i] = w.x;
-        a[r][4 * i + 1] = w.y;
-        a[r][4 * i + 2] = w.z;
-        a[r][4 * i + 3] = w.w;
+      for (int j = 0; j < D / 4; j += 2) {
+        some = __fmaf_rn(y[r][j], y[r][j], some);
+        more = __fmaf_rn(y[r][j + 1], y[r][j + 1], more);
       }
-    }
-    float y[2][D / 4];
+      some = __fadd_rn(some, more);
+      some += __shfl_xor_sync(0xffffffffu, some, 1);
+      some += __shfl_xor_sync(0xffffffffu, some, 2);
+      square[r] = some;
+    };
+    uint32_t a[2][D / 8];
+    auto load = [&] {
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const uint4 *q = (const uint4 *)(src + (int64_t)(first + pos0 + g + 8 * r) * in.row);
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+          const uint4 w = live[r] ? __ldg(q + i) : make_uint4(0, 0, 0, 0);
+          a[r][4 * i] = w.x;
+          a[r][4 * i + 1] = w.y;
+          a[r][4 * i + 2] = w.z;
+          a[r][4 * i + 3] = w.w;
+        }
+      }
+    };
+    load();
     rotate_rows<D, BF16, 2, false>(c, a, y);
+    squares(0);
+    squares(1);
+    if (BF16 && __any_sync(0xffffffffu, !(square[0] < 0x1p80f && square[1] < 0x1p80f))) {
+      // Bfloats may be so large that the transform passes the largest float: such
+      // rows are taken again, with a power of two out of them first.
+      load();
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int size = bfloat_exponent<D>(a[r]);  // (every lane: it shuffles)
+        const int e = square[r] < 0x1p80f ? 0 : size;
+        grow[r] = exp2i(e);
+#pragma unroll
+        for (int j = 0; j < D / 8; j++) {
+          const float2 v = unpack2<true>(a[r][j]);
+          a[r][j] = pack2<true>(__fmul_rn(v.x, exp2i(-e)), __fmul_rn(v.y, exp2i(-e)));
+        }
+      }
+      rotate_rows<D, BF16, 2, false>(c, a, y);
+      squares(0);
+      squares(1);
+    }
     if (part == from) {
       pdl_wait();
       // an extend failed, so that these rows have no place, or the check found an entry bad
@@ -163,21 +212,7 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
     const float shrink = rotation_scale<D>(c);
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-      float square = 0.0f, grow = 1.0f;
-      auto squares = [&] {
-        float more = 0.0f;
-        square = 0.0f;
-#pragma unroll
-        for (int j = 0; j < D / 4; j += 2) {
-          square = __fmaf_rn(y[r][j], y[r][j], square);
-          more = __fmaf_rn(y[r][j + 1], y[r][j + 1], more);
-        }
-        square = __fadd_rn(square, more);
-        square += __shfl_xor_sync(0xffffffffu, square, 1);
-        square += __shfl_xor_sync(0xffffffffu, square, 2);
-      };
-      squares();
-      if (__any_sync(0xffffffffu, !(square > 0x1p-80f && square < 0x1p80f))) {
+      if (__any_sync(0xffffffffu, !(square[r] > 0x1p-80f && square[r] < 0x1p80f))) {
         // A power of two takes the row's size out, so that squares neither
         // overflow nor vanish (for the rows that need it: 1 for the others).
         float m = 0.0f;
@@ -185,14 +220,14 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
         for (int j = 0; j < D / 4; j++) m = fmaxf(m, fabsf(y[r][j]));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int e = square > 0x1p-80f && square < 0x1p80f ? 0 : max(-100, min(log2i(m), 126));
-        grow = exp2i(e);
+        const int e = square[r] > 0x1p-80f && square[r] < 0x1p80f ? 0 : max(-100, min(log2i(m), 126));
+        grow[r] = __fmul_rn(grow[r], exp2i(e));
 #pragma unroll
         for (int j = 0; j < D / 4; j++) y[r][j] = __fmul_rn(y[r][j], exp2i(-e));
-        squares();
+        squares(r);
       }
       const float inv =
-          square > 0.0f ? __fdiv_rn(1.0f, __fmul_rn(kStep, __fsqrt_rn(__fmul_rn(square, 1.0f / D))))
+          square[r] > 0.0f ? __fdiv_rn(1.0f, __fmul_rn(kStep, __fsqrt_rn(__fmul_rn(square[r], 1.0f / D))))
                         : 0.0f;
       float ly = 0.0f, more = 0.0f;
       uint32_t w[D / 32];
@@ -214,7 +249,7 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(Cache c, int layer,
       // |y| finite and not zero: ly > 0, since every level has its value's sign
       // (a row of zeros has the scale zero; one with an infinity or a NaN gets NaN)
       const float scale =
-          square == 0.0f ? 0.0f : __fmul_rn(__fmul_rn(__fdiv_rn(square, ly), shrink), grow);
+          square[r] == 0.0f ? 0.0f : __fmul_rn(__fmul_rn(__fdiv_rn(square[r], ly), shrink), grow[r]);
       const int row = row0 + g + 8 * r;
       if (live[r] && t == 0) ((float *)(tile + kTile * (D / 2)))[row] = scale;
       if (!value) {
