@@ -421,6 +421,24 @@ def test_one_long_sequence_and_many_ragged_ones_split_alike(uv):
         assert (np.abs(f64(alone) - want) <= attend_tolerance(want, size, reach, "bfloat16")).all()
 
 
+@pytest.mark.parametrize("n,rounds", [(40, 1), (5000, 1), (5000, 3)])
+def test_values_near_the_largest_number(uv, n, rounds):
+    """Sums of thousands of them are beyond a float; their means are not."""
+    import torch
+
+    rng = np.random.default_rng(26)
+    d = 128
+    c, signs = cache(uv, d, 1, [n], rounds=rounds)
+    k, v = (rows_of(rng, n, 1, d, "float32", False) for _ in range(2))
+    v = (v.clamp(-3, 3) + 0.5) * 1e37
+    c.append(ints([0]), k.bfloat16(), v.bfloat16(), starts([n]))
+    q = rows_of(rng, 2, 4, d, "bfloat16", False) * 0.5
+    out = c.attend(ints([0]), q, starts([2]), 2)
+    want, _, size, reach = M.attend(f64(q), M.held(c.pool[0].cpu().numpy(), c.table[0].cpu().numpy(), n, d),
+                                    M.rotation(signs), 1 / math.sqrt(d))
+    assert (np.abs(f64(out) - want) <= attend_tolerance(want, size, reach, "bfloat16")).all()
+
+
 @pytest.mark.parametrize("lens", [[1], [40], [6000], [20_000, 3]])
 def test_queries_and_keys_that_are_no_numbers(uv, lens):
     """NaN in a query makes its own row NaN and no other, however its job is split;

@@ -18,7 +18,7 @@
 // one line, cut into equal pieces, one for each block of a single wave,
 // whatever the lengths are: the host need not know them.  A piece may hold the
 // end of a job, whole jobs and the start of another; each part leaves its
-// maximum, sum and unnormalised output in scratch, and the block that finds all
+// maximum, sum and output (divided by its sum) in scratch, and the block that finds all
 // of a job's parts written joins them in order, rotates back and rounds.
 //
 // Numbers: q is rotated in f32 and rounded to a half, after a power of two that
@@ -674,6 +674,17 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         }
       }
     __syncthreads();
+    auto total_of = [&](int col, float *top) {
+      float sum = 0.0f;
+      *top = join_m[0][col];
+      for (int v = 1; v < kWarps; v++) *top = max_nan(*top, join_m[v][col]);
+      for (int v = 0; v < kWarps; v++)
+        if (join_m[v][col] != -INFINITY)
+          sum = __fmaf_rn(join_l[v][col], exp2_fast(__fsub_rn(join_m[v][col], *top)), sum);
+      return sum;
+    };
+    // (divided by the block's sum at once: a mean of values is a float where their
+    // sum may not be one)
     constexpr int kRow = F::kRow;
     float *out = (float *)(smem + F::kRing), *mine_out = out + (warp & 1) * kCols * kRow;
 #pragma unroll
@@ -684,18 +695,19 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             const int col = 8 * nt + 2 * t + k;
-            float top = join_m[0][col];
-            for (int v = 1; v < kWarps; v++) top = max_nan(top, join_m[v][col]);
+            float top;
+            const float sum = total_of(col, &top);
             // a warp without a visible token adds nothing, whatever its sums hold
             const bool none = m[nt][k] == -INFINITY;
-            const float f = __fmul_rn(exp2_fast(__fsub_rn(m[nt][k], top)), exp2i(ve[nt][k]));
+            const float f = __fdiv_rn(exp2_fast(__fsub_rn(m[nt][k], top)), sum);
             const float flo = __fmul_rn(f, 0x1p24f), fhi = __fmul_rn(f, 0x1p20f);
+            const float unit = exp2i(ve[nt][k]);
 #pragma unroll
             for (int mt = 0; mt < D / 16; mt++) {
               float2 *to = (float2 *)(mine_out + col * kRow + g * (D / 8) + 2 * mt);
               const float2 was = step == 0 ? make_float2(0.0f, 0.0f) : *to;
-              const float u = none ? 0.0f : __fmul_rn(o[mt][nt][k], flo);
-              const float v = none ? 0.0f : __fmul_rn(o[mt][nt][2 + k], fhi);
+              const float u = none ? 0.0f : __fmul_rn(__fmul_rn(o[mt][nt][k], flo), unit);
+              const float v = none ? 0.0f : __fmul_rn(__fmul_rn(o[mt][nt][2 + k], fhi), unit);
               *to = make_float2(__fadd_rn(was.x, u), __fadd_rn(was.y, v));
             }
           }
@@ -707,15 +719,6 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     const int64_t part = seg.number + blockIdx.x;
     const bool fits = seg.number + seg.first_block + seg.blocks <= slots;
     bool final = seg.blocks == 1 && fits;
-    auto total_of = [&](int col, float *top) {
-      float sum = 0.0f;
-      *top = join_m[0][col];
-      for (int v = 1; v < kWarps; v++) *top = max_nan(*top, join_m[v][col]);
-      for (int v = 0; v < kWarps; v++)
-        if (join_m[v][col] != -INFINITY)
-          sum = __fmaf_rn(join_l[v][col], exp2_fast(__fsub_rn(join_m[v][col], *top)), sum);
-      return sum;
-    };
     auto write_lse = [&](int col, float top, float sum) {
       const int x = c0 + col;
       if (a.lse != nullptr && x < ncol)
@@ -727,12 +730,13 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         const int col = i / (D / 4), d4 = i % (D / 4);
         float4 *u = (float4 *)(out + col * kRow + 4 * d4);
         const float4 v = *(const float4 *)(out + (kCols + col) * kRow + 4 * d4), w = *u;
-        float top;
-        const float sum = total_of(col, &top);
-        const float inv = top == -INFINITY ? 0.0f : __fdiv_rn(1.0f, sum);
-        *u = make_float4(__fmul_rn(__fadd_rn(w.x, v.x), inv), __fmul_rn(__fadd_rn(w.y, v.y), inv),
-                         __fmul_rn(__fadd_rn(w.z, v.z), inv), __fmul_rn(__fadd_rn(w.w, v.w), inv));
-        if (d4 == 0 && fits) write_lse(col, top, sum);
+        *u = make_float4(__fadd_rn(w.x, v.x), __fadd_rn(w.y, v.y), __fadd_rn(w.z, v.z),
+                         __fadd_rn(w.w, v.w));
+        if (d4 == 0 && fits) {
+          float top;
+          const float sum = total_of(col, &top);
+          write_lse(col, top, sum);
+        }
       }
       __syncthreads();
     } else if (fits) {
@@ -774,19 +778,26 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
         for (int i = tid; i < seg.blocks; i += kAttendThreads) set_flag(&sc.flag[first + i], 0);
         constexpr int V = D / 32;
         for (int col = warp; col < kCols; col += kWarps) {
-          float top = -INFINITY, sum = 0.0f, acc[V];
-          for (int i = lane; i < seg.blocks; i += 32)
-            top = max_nan(top, __ldcg(&sc.ml[(first + i) * kCols + col]).x);
+          auto load = [&](int i) {
+            return i < seg.blocks ? __ldcg(&sc.ml[(first + i) * kCols + col])
+                                  : make_float2(-INFINITY, 0.0f);
+          };
+          const float2 ml0 = load(lane);
+          float top = ml0.x, sum = 0.0f, acc[V];
+          for (int i = lane + 32; i < seg.blocks; i += 32) top = max_nan(top, load(i).x);
           for (int x = 16; x; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
+          // a part's sum against the largest maximum
+          auto weight = [&](float2 ml) {
+            return ml.x == -INFINITY ? 0.0f : __fmul_rn(ml.y, exp2_fast(__fsub_rn(ml.x, top)));
+          };
+          for (int i = lane; i < seg.blocks; i += 32)
+            sum = __fadd_rn(sum, weight(i == lane ? ml0 : load(i)));
+          for (int x = 16; x; x >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, x));
+          const float inv = top == -INFINITY ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
           for (int v = 0; v < V; v++) acc[v] = 0.0f;
           for (int i0 = 0; i0 < seg.blocks; i0 += 32) {
-            float f = 0.0f;
-            if (i0 + lane < seg.blocks) {
-              const float2 ml = __ldcg(&sc.ml[(first + i0 + lane) * kCols + col]);
-              f = ml.x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(ml.x, top));
-              sum = __fmaf_rn(ml.y, f, sum);
-            }
+            const float f = __fmul_rn(weight(i0 == 0 ? ml0 : load(i0 + lane)), inv);
             const int n = min(32, seg.blocks - i0);
 #pragma unroll 4
             for (int i = 0; i < n; i++) {
@@ -801,11 +812,8 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
               }
             }
           }
-          for (int x = 16; x; x >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, x));
-          const float inv = top == -INFINITY ? 0.0f : __fdiv_rn(1.0f, sum);
 #pragma unroll
-          for (int v = 0; v < V; v++)
-            out[col * kRow + lane * V + v] = top == -INFINITY ? 0.0f : __fmul_rn(acc[v], inv);
+          for (int v = 0; v < V; v++) out[col * kRow + lane * V + v] = acc[v];
           if (lane == 0) write_lse(col, top, sum);
         }
         __syncthreads();
@@ -814,20 +822,15 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
     if (final) {
       for (int half = warp; half < (NT + 1) / 2; half += kWarps) {
         float y[2][D / 4];
+        const float f = rotation_scale<D>(c);  // ahead: the transform then passes no float
 #pragma unroll
         for (int r = 0; r < 2; r++)
 #pragma unroll
           for (int j = 0; j < D / 4; j++) {
             const int col = 16 * half + 8 * r + g;
-            y[r][j] = col < kCols ? out[(col < kCols ? col : 0) * kRow + t * (D / 4) + j] : 0.0f;
+            y[r][j] = col < kCols ? __fmul_rn(out[(col < kCols ? col : 0) * kRow + t * (D / 4) + j], f) : 0.0f;
           }
         rotate_back<D, 2>(c, y, true);
-        const float f = rotation_scale<D>(c);
-#pragma unroll
-        for (int j = 0; j < D / 4; j++) {
-          y[0][j] = __fmul_rn(y[0][j], f);
-          y[1][j] = __fmul_rn(y[1][j], f);
-        }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
           const int col = 16 * half + 8 * r + g, x = c0 + col;
