@@ -250,6 +250,20 @@ def test_one_score_that_is_no_number(uv, d, causal):
         assert (np.abs(f64(lse) - wl) <= 2.0 ** -17 * reach + 2.0 ** -13).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,size", [(300, 1e37), (3000, 1e38), (300, 1e-30)])
+def test_values_near_the_largest_number(uv, d, n, size):
+    """Sums of many of them are beyond a float; their means are not.  Small ones
+    keep their bits too."""
+    rng = np.random.default_rng(n)
+    q, k, v = rows(rng, 200, 2, d, "bfloat16", 0.5), rows(rng, n, 1, d, "bfloat16"), rows(rng, n, 1, d, "bfloat16")
+    v = ((v.float().clamp(-2, 2) + 0.5) * size).bfloat16()
+    out, lse = uv.prompt_attention(q, k, v, starts([200]), starts([n]), lse=True)
+    want, wl, big, reach = M.prompt(f64(q), f64(k), f64(v), True, 1 / math.sqrt(d))
+    err, tol = np.abs(f64(out) - want) / size, tolerance(want / size, big / size, reach, "bfloat16")
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 @pytest.mark.parametrize("n", [1, 33, 150])
 def test_many_sequences_of_every_length(uv, n):
     """Entries over all lanes, and more than the ordered search takes."""

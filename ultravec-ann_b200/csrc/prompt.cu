@@ -33,7 +33,7 @@
 // Blocks of keys go from the last, masked ones to the first.  A row's weights
 // stand against a reference, the maximum of the first keys that it sees, and no
 // maximum is taken after that: as long as the sums of its weights stay below
-// 2^14 (2^15 of halves) the reference serves as well.  Where one does not, the row takes a new
+// 2^14 times the reference's (2^7 of halves) it serves as well.  Where one does not, the row takes a new
 // reference and its warp rescales O in TMEM.
 //
 // What a row does not see must not reach it, but a weight of zero times a value
@@ -75,13 +75,16 @@ constexpr int kPoly = 2, kPolyOf = 8;
 // (An output waits for its piece's last one; by then at most the next piece's are mended,
 // and 256 rows end within three blocks.)
 constexpr int kMends = 4;
-// Weights (sums of 32 of them) up to kGrow stay unanswered; a row's reference weighs
-// 2^lift.  Halves are exact to 2^-25 at their small end: lifted by 8, a weight keeps 11
-// bits down to 2^-22 of its row's largest, and what the others may grow by, 2^7, is
-// still beyond what the maximum of a row's first keys is usually passed by.
+// A row's reference weighs 2^lift, and weights (sums of 32 of them) up to kGrow stay
+// unanswered.  Halves are exact to 2^-25 at their small end: lifted by 8, a weight keeps
+// 11 bits down to 2^-22 of its row's largest, and what the others may grow by, 2^7, is
+// still beyond what the maximum of a row's first keys is usually passed by.  Bfloats
+// have the exponents to spare: lowered by 20, the sums of a million of the largest
+// values are floats.
 template <bool BF16>
 struct Weights {
-  static constexpr float kLift = BF16 ? 0.0f : 8.0f, kGrow = BF16 ? 16384.0f : 32768.0f;
+  static constexpr float kLift = BF16 ? -20.0f : 8.0f;
+  static constexpr float kGrow = BF16 ? 0x1p-6f : 0x1p15f;
 };
 
 __device__ __forceinline__ int bounded(int x, int hi) { return x < 0 ? 0 : (x < hi ? x : hi); }
