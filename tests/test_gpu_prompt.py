@@ -264,6 +264,20 @@ def test_values_near_the_largest_number(uv, d, n, size):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_row_whose_scores_are_all_minus_infinity(uv, d):
+    """It has no softmax (NaN, and a sum of zero), other than a row that sees nothing."""
+    rng = np.random.default_rng(d)
+    q, k, v = rows(rng, 200, 2, d, "float16"), rows(rng, 160, 1, d, "float16"), rows(rng, 160, 1, d, "float16")
+    q[:, :, 0] = 1
+    k[:150, :, 0] = -math.inf  # rows 40 .. 189 see those alone, rows 0 .. 39 none at all
+    out, lse = uv.prompt_attention(q, k[:160], v, starts([0, 200]), starts([0, 160]), lse=True)
+    assert bool((out[:40] == 0).all()) and bool((lse[:40] == -math.inf).all())
+    assert bool(out[40:190].isnan().all()) and bool((lse[40:190] == -math.inf).all())
+    want, wl, size, reach = M.prompt(f64(q[190:]), f64(k[150:]), f64(v[150:]), True, 1 / math.sqrt(d))
+    assert (np.abs(f64(out[190:]) - want) <= tolerance(want, size, reach, "float16")).all()
+
+
 @pytest.mark.parametrize("n", [1, 33, 150])
 def test_many_sequences_of_every_length(uv, n):
     """Entries over all lanes, and more than the ordered search takes."""

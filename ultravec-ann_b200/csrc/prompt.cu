@@ -653,10 +653,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       settle(!*abort_s);
       if (!ok) *abort_s = 1;
       tc::tc_fence_after();
-      const bool none = blocks == 0 || m == -INFINITY, live = row < it.nq;
+      const bool none = blocks == 0 || lim == 0, live = row < it.nq;
       const bool odds = flagged > 0 && *(volatile int *)&any_odd[k & 1] != 0;
       // (the sums of a row that sees nothing are zeros: its keys' values are mended)
-      const float inv = !ok ? NAN : none ? 0.0f : __fdiv_rn(1.0f, sum);  // NaN: a wait gave up
+      // NaN: a wait gave up, or every score that the row sees is -inf
+      const float inv = !ok ? NAN : none ? 0.0f : m == -INFINITY ? NAN : __fdiv_rn(1.0f, sum);
       uint16_t *to = (uint16_t *)a.out +
                      ((int64_t)(it.q0 + row - (lane & 3)) * a.q_heads + it.head[t]) * D + 8 * (lane & 3);
 #pragma unroll 1
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
       }
       if (live && a.lse != nullptr)
         a.lse[(int64_t)(it.q0 + row) * a.q_heads + it.head[t]] =
-            none ? -INFINITY
+            none || m == -INFINITY ? -INFINITY
                  : ok ? __fmul_rn(__fmaf_rn(m, c, __log2f(sum) - kLift), kLn2) : NAN;
       tc::tc_fence_before();
       // (in this order: who finds piece k + 2 finds out_done past piece k, so that a
