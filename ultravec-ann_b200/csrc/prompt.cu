@@ -44,9 +44,10 @@
 // at a time) and go through it value by value only where there is one.
 //
 // Bound: per 128 x 128 tile and D = 128 the two products take 1024 cycles of
-// the tensor core, the exponentials 1024 of the MUFU (16 a cycle) if it computes
-// them all (a quarter goes to a polynomial in the FMA pipe), and their arguments,
-// sums and packing about as many issue cycles.  A tile's chain (scores, 128
+// the tensor core, the exponentials 1024 of the MUFU (16 a cycle), and their arguments,
+// sums and packing about as many issue cycles.  (A polynomial in the FMA pipe for a
+// quarter of them takes issue slots instead: texts 39.2 us with it and 33.7 without,
+// 8192 tokens 543 and 542, packed prompts 124 and 123.)  A tile's chain (scores, 128
 // exponentials a thread at about 7 cycles, product) takes 2300 cycles with the
 // other tile beside it, so 3500 pass for two tiles, of which the tensor core
 // works 2048: 1000 TFLOP/s for 8192 tokens and 32 heads (0.55 ms), at the 1.69 GHz
@@ -63,13 +64,6 @@ namespace prompt {
 
 constexpr int kRows = 128, kKeys = 128;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// 2^f on [-1/2, 1/2], relative error below 2.7e-6: a least-squares fit of the relative
-// error with weights that drive it to its minimax, made for this file
-constexpr float kC0 = 0.9999992847442627f, kC1 = 0.6931217908859253f, kC2 = 0.240247443318367f,
-                kC3 = 0.05591785907745361f, kC4 = 0.009570101276040077f;
-// Of kPolyOf columns, kPoly take the polynomial: packed prompts take 177 us with 0,
-// 172 with 1, 170 with 2; one long prompt 522, 533 and 522, texts of D = 64 48 with any.
-constexpr int kPoly = 2, kPolyOf = 8;
 // Barriers of mended values, in turn: the ring holds at most three blocks of values whose
 // product is still to be issued, so none completes a second time before it was waited for.
 // (An output waits for its piece's last one; by then at most the next piece's are mended,
@@ -131,26 +125,6 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   f2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x for two x in the FMA pipe: x = n + f with f in [-1/2, 1/2], 2^f by the
-// polynomial of degree 4, n added to the exponent.  x above 127 gives 2^127, and so
-// does NaN (the caller takes a new reference then, which makes the row NaN where a
-// score was), below -126 2^-126 (the caller makes masked weights exact zeros).
-__device__ __forceinline__ float2 exp2_poly(f2 x) {
-  const float2 v = split(x);
-  x = pair(fmaxf(fminf(v.x, 127.0f), -126.0f), fmaxf(fminf(v.y, 127.0f), -126.0f));
-  const f2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
-  const f2 n = add2(x, magic), whole = add2(n, minus);
-  const f2 f = fma2(whole, pair(-1.0f, -1.0f), x);
-  f2 p = pair(kC4, kC4);
-  p = fma2(p, f, pair(kC3, kC3));
-  p = fma2(p, f, pair(kC2, kC2));
-  p = fma2(p, f, pair(kC1, kC1));
-  p = fma2(p, f, pair(kC0, kC0));
-  const float2 pf = split(p), nf = split(n);
-  return make_float2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(nf.x) << 23)),
-                     __int_as_float(__float_as_int(pf.y) + (__float_as_int(nf.y) << 23)));
 }
 
 // ---- tensor core plumbing beside uv_tc.cuh ----
@@ -602,16 +576,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
             for (int e = 0; e < 64; e += 2) {
               const uint32_t *x = &r[2 * h + e / 32][e % 32];
               const f2 z = fma2(pair(__uint_as_float(x[0]), __uint_as_float(x[1])), cc, bb);
-              float2 y;
-              if (e % kPolyOf < kPoly) {
-                y = exp2_poly(z);
-              } else {
-                const float2 v = split(z);
-                y = make_float2(exp2_fast(v.x), exp2_fast(v.y));
-              }
-              if (e % 4) b1 = add2(b1, pair(y.x, y.y));
-              else b0 = add2(b0, pair(y.x, y.y));
-              p[e / 32][e % 32 / 2] = kv::pack2<BF16>(y.x, y.y);
+              const float2 v = split(z);
+              const float x0 = exp2_fast(v.x), x1 = exp2_fast(v.y);
+              if (e % 4) b1 = add2(b1, pair(x0, x1));
+              else b0 = add2(b0, pair(x0, x1));
+              p[e / 32][e % 32 / 2] = kv::pack2<BF16>(x0, x1);
             }
             sum = add2(b0, b1);
             // weights beyond kGrow (or NaN): take a new reference and start over, once
@@ -624,15 +593,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kBlocks)
           }
           if (!ok) break;
           l = add2(l, sum);
-          if (masked) {
-            asm volatile("");
-#pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              if (e % kPolyOf >= kPoly) continue;  // the MUFU's are zeros already
-              if (64 * h + e >= seen) p[e / 32][e % 32 / 2] &= 0xffff0000u;
-              if (64 * h + e + 1 >= seen) p[e / 32][e % 32 / 2] &= 0x0000ffffu;
-            }
-          }
           tmem_st16(s_at + 64 * h, p[0]);
           tmem_st16(s_at + 64 * h + 16, p[1]);
           tmem_st_wait();
