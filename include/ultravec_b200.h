@@ -657,8 +657,8 @@ int uv_kv_attend(const uv_kv *kv, int32_t layer, const int32_t *seqs, const int3
  * [starts_q[b], starts_q[b + 1]) and key rows [starts_k[b], starts_k[b + 1])
  * (NULL: the same), its queries being the last of its keys: with causal, row i
  * sees keys 0 .. i + keys - queries.  head_dim 64 or 128; strides, out, lse
- * and scale as above.  What a row does not see has no influence on it, whatever
- * it holds; should a bounded device wait give up, the rows concerned are NaN. */
+ * and scale as above; a row whose scores are all -inf is NaN (its lse -inf).
+ * What a row does not see has no influence on it, whatever it holds; should a bounded device wait give up, the rows concerned are NaN. */
 int uv_prompt_attention(int32_t device, const int32_t *starts_q, const int32_t *starts_k,
                         int32_t n, int32_t rows_q, int32_t rows_k, int32_t q_heads,
                         int32_t kv_heads, int32_t head_dim, int32_t causal, float scale,

@@ -6,7 +6,7 @@
 //
 // Bound: HBM, D + 8 bytes a token and key head; the work behind each byte is
 // unpacking (5 instructions for 8 codes) and two products with 8 columns.  64
-// sequences of 1k to 20k tokens (448 MB of cache): 104 us, 4.3 TB/s; without any
+// sequences of 1k to 20k tokens (448 MB of cache): 106 us, 4.2 TB/s; without any
 // work on the tiles it takes 87.
 // The columns of a block are (row, query head of the group) pairs of one
 // sequence and key head, so the codes are read and unpacked once for the whole
@@ -92,8 +92,8 @@ __device__ __forceinline__ unsigned long long get_flag(const unsigned long long 
 
 // What a job costs beside its tiles (its queries, the join of its parts), in
 // tiles: the pieces of the line are equal in time, not in tiles.  64 sequences of
-// 1k to 20k tokens take 114 us at 4, 108 at 14, 102 at 20, 109 at 32; 16 of 0.7k
-// to 8k 35, 30, 32 and 32; drafts of 8 sequences of 33 to 4.5k 30, 23, 23 and -.
+// 1k to 20k tokens take 119 us at 4, 113 at 14, 105 at 20, 107 at 32; 16 of 0.7k
+// to 8k 37, 33, 35 and 31; drafts of 8 sequences of 33 to 4.5k 33, 25, 25 and 25.
 constexpr int kJobCost = 20;
 
 struct Job {

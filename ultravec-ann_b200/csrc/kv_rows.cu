@@ -8,10 +8,12 @@
 // 4 lanes.  Positions outside the call's rows are computed as zeros and not
 // stored.
 //
-// Bound: HBM would allow 13 us each way for 16k tokens of 8 heads of 128 (2 D
-// bytes of a row in, D / 2 + 4 out, and the reverse); the instructions, about 16 a
-// value into the cache and 10 out of it, take 35 and 28 us.  For a token each it
-// is latency (four dependent loads find the row's place).
+// Bound: HBM would allow 11 us each way for 14k tokens of 8 heads of 128 (2 D
+// bytes of a row in, D / 2 + 4 out, and the reverse).  They take 37 and 29 us: 20
+// instructions a value into the cache and 12 out of it (16 and 10 us of issue slots,
+// had they no gaps), at three warps a scheduler, all that 160 registers leave, which
+// do not cover the rows' loads.  For a token each it is latency (four dependent loads
+// find the row's place).
 #include "uv_kv.h"
 
 namespace uvb {
@@ -381,8 +383,8 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(Cache c, int layer, R
 }
 
 // Parts a warp takes: one while that leaves the card room (a token each), four
-// where there are many blocks (16k tokens, in and out: 72 us with one, 65 with
-// two or four, 69 with eight).
+// where there are many blocks (14k tokens, in and out: 84 us with one, 72 with two, 67
+// with four, 88 with eight).
 static int parts_each(int64_t blocks, int heads) { return blocks * 2 * heads > 148 * 16 ? 4 : 1; }
 
 static int64_t block_bound(const Rows &r) {

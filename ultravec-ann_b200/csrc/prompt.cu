@@ -50,7 +50,7 @@
 // 8192 tokens 543 and 542, packed prompts 124 and 123.)  A tile's chain (scores, 128
 // exponentials a thread at about 7 cycles, product) takes 2300 cycles with the
 // other tile beside it, so 3500 pass for two tiles, of which the tensor core
-// works 2048: 1000 TFLOP/s for 8192 tokens and 32 heads (0.55 ms), at the 1.69 GHz
+// works 2048: 1010 TFLOP/s for 8192 tokens and 32 heads (0.54 ms), at the 1.69 GHz
 // that the power limit then leaves.
 #include <cfloat>
 #include <climits>
@@ -329,8 +329,8 @@ __device__ __forceinline__ void describe(const Args &a, int b, int64_t i0, int h
 // blocks, most first, so that no long one is left for the end: how many tiles of
 // an entry have c blocks or more is a division, so the u-th tile is a binary
 // search over c, with the entries over the lanes.  (One sequence of 6000 tokens
-// ahead of 90 of 300, 8 heads of 128: 211 us in the order of the pack, from its
-// end, 200 so.)  Past 128 entries the order is the pack's.
+// ahead of 90 of 300, 8 heads of 128: 226 us in the order of the pack, from its
+// end, 152 so.)  Past 128 entries the order is the pack's.
 template <int TILES>
 __device__ __forceinline__ bool find_item(const Args &a, int block, Item *it) {
   constexpr int kEach = 4;

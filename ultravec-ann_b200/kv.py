@@ -6,6 +6,7 @@ estimator of src/trellis.rs:1483-1536), attended to without being decoded.
 `prompt_attention` attends over packed prompts.  Arrays are CUDA torch
 tensors; every call is ordered on torch's current stream of their device, and
 none but `check` waits for it, so a serving step can be captured in a graph.
+They infer only: outputs carry no gradient, also where an input asks for one.
 
 A step for sequences that already have tokens:
 
@@ -226,7 +227,8 @@ class KvCache:
     def append(self, seqs, k, v, starts=None, *, layer: int = 0) -> None:
         """Quantises k and v (rows x kv_heads x head_dim) into the last tokens
         of the sequences: rows [starts[b], starts[b + 1]) are the last of
-        seqs[b] (one row each without starts)."""
+        seqs[b] (one row each without starts).  All or nothing: a sequence out
+        of range or listed twice, or a shared page, is left to `check`."""
         i, n, dtype = self._index, seqs.shape[0], _dtype(k)
         if v.dtype is not k.dtype or v.shape != k.shape:
             raise ValueError("k and v must have one type and one shape")
