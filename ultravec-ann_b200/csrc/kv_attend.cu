@@ -756,15 +756,15 @@ __global__ void __launch_bounds__(kAttendThreads, Fit<D, NT, BF16>::kBlocks)
       __syncthreads();
       if (tid == 0) set_flag(&sc.flag[part], a.call);
       // Whoever finds every part written joins them, in their order.  Between a
-      // block's own flag and its look at the others' stands a fence.sc: those
-      // fences have one order, and the block whose fence is the last in it sees
-      // every flag (or zeros, from a block that saw them all and joins).  Release
-      // and acquire alone would let two blocks miss each other's.  Two that
-      // finish together may both join, and write the same bytes.  Nothing waits,
-      // and no counter has to start at zero.
+      // block's own flag and its look at the others' stands a fence.sc (by the lane
+      // that set the flag; the warp looks behind it): those fences have one order,
+      // and the block whose fence is the last in it sees every flag (or zeros, from a
+      // block that saw them all and joins).  Release and acquire alone would let two
+      // blocks miss each other's.  Two that finish together may both join, and write
+      // the same bytes.  Nothing waits, and no counter has to start at zero.
       const int64_t first = seg.number + seg.first_block;
       if (warp == 0) {
-        fence_sc();
+        if (lane == 0) fence_sc();
         __syncwarp();
         bool all = true;
         for (int i = lane; i < seg.blocks; i += 32) all = all && get_flag(&sc.flag[first + i]) == a.call;
